@@ -1,0 +1,441 @@
+"""Operators around the attention of a transformer's training step, as cases that can be measured.
+
+Kinds of work
+  attention  attention whose scores are capped by a tanh or get a bias that falls with distance, over the keys that a
+             document, prefix or padding mask leaves; key and value heads may be shared by several query heads.
+             Forward alone or with the gradients of q, k and v.
+  ranges     the masks' form: for each query row the range of keys it sees, from document starts and prefix lengths
+  rotary     rotary positions with one to four axes on q and k, forward and the gradient
+  clip       the norm over many gradient tensors, and the clipped gradients
+
+`run` computes the plain form with elementary torch operations, or, where `own` is true, makes the calls of the
+framework.  Import with the repository root first in sys.path.
+"""
+import importlib
+import math
+import random
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def _ffk():
+    return importlib.import_module("flexflow-train_amd")
+
+
+# ---------------------------------------------------------------------------
+# The cases
+# ---------------------------------------------------------------------------
+def listed():
+    return [
+        # the benchmark's encoder layer (batch 8, 512 tokens, 16 heads of 64) on rows packed from several documents
+        {"name": "attn_encoder_documents", "op": "attention", "dtype": "bf16", "batch": 8, "seq_q": 512, "seq_kv": 512, "heads": 16, "kv_heads": 16,
+         "dim": 64, "causal": False, "documents": 4, "prefix": 0, "padding": 37, "given": False, "cap": 0.0, "bias": False, "train": True},
+        # the benchmark's causal attention (batch 4, 4096 tokens, 32 heads of 128), packed rows, capped scores, four query heads to a key head
+        {"name": "attn_decoder_capped", "op": "attention", "dtype": "bf16", "batch": 4, "seq_q": 4096, "seq_kv": 4096, "heads": 32, "kv_heads": 8,
+         "dim": 128, "causal": True, "documents": 3, "prefix": 0, "padding": 0, "given": False, "cap": 30.0, "bias": False, "train": True},
+        # one long row without documents, distances as a bias in place of positions
+        {"name": "attn_long_distance", "op": "attention", "dtype": "bf16", "batch": 1, "seq_q": 8192, "seq_kv": 8192, "heads": 16, "kv_heads": 16,
+         "dim": 128, "causal": True, "documents": 0, "prefix": 0, "padding": 0, "given": False, "cap": 0.0, "bias": True, "train": True},
+        # a prompt that sees itself whole and an answer that sees what is before it, odd length, heads of 80, evaluation
+        {"name": "attn_prefix_odd", "op": "attention", "dtype": "bf16", "batch": 3, "seq_q": 1531, "seq_kv": 1531, "heads": 12, "kv_heads": 4,
+         "dim": 80, "causal": True, "documents": 2, "prefix": 200, "padding": 11, "given": False, "cap": 0.0, "bias": True, "train": False},
+        # the reference's own data type at a size where launches count
+        {"name": "attn_small_fp32", "op": "attention", "dtype": "fp32", "batch": 2, "seq_q": 100, "seq_kv": 100, "heads": 4, "kv_heads": 2,
+         "dim": 64, "causal": True, "documents": 2, "prefix": 9, "padding": 3, "given": False, "cap": 20.0, "bias": True, "train": True},
+        # one query row to each sequence over keys of different lengths: a token that follows, or a pooled query
+        {"name": "attn_one_row", "op": "attention", "dtype": "bf16", "batch": 16, "seq_q": 1, "seq_kv": 8192, "heads": 32, "kv_heads": 8,
+         "dim": 128, "causal": False, "documents": 0, "prefix": 0, "padding": 0, "given": True, "cap": 30.0, "bias": False, "train": False},
+        # the masks of one small batch, and of a large packed one
+        {"name": "ranges_small", "op": "ranges", "batch": 8, "seq": 512, "causal": False, "documents": 4, "prefix": 0},
+        {"name": "ranges_packed", "op": "ranges", "batch": 64, "seq": 16384, "causal": True, "documents": 50, "prefix": 64},
+        # image patches, two axes, the reference's data type; and a decoder's tokens with time, height and width
+        {"name": "rotary_image_fp32", "op": "rotary", "dtype": "fp32", "batch": 2, "seq": 196, "heads": 12, "kv_heads": 12, "dim": 64,
+         "sections": "16,16", "interleaved": True, "far": 14},
+        {"name": "rotary_video_bf16", "op": "rotary", "dtype": "bf16", "batch": 4, "seq": 4096, "heads": 32, "kv_heads": 8, "dim": 128,
+         "sections": "16,24,24", "interleaved": False, "far": 100000},
+        # the gradients of one encoder layer in fp32, and of a decoder's stack in bf16 with fp32 norms between
+        {"name": "clip_encoder_fp32", "op": "clip", "dtype": "fp32", "layers": 1, "width": 1024, "inner": 4096, "max_norm": 1.0},
+        {"name": "clip_stack_bf16", "op": "clip", "dtype": "bf16", "layers": 6, "width": 4096, "inner": 16384, "max_norm": 1.0},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["attention", "attention", "attention", "attention", "ranges", "rotary", "rotary", "clip", "clip"])
+    if op == "ranges":
+        return {"op": "ranges", "batch": _log_int(rng, 1, 64), "seq": _log_int(rng, 64, 16384), "causal": rng.random() < 0.7,
+                "documents": _log_int(rng, 1, 200), "prefix": rng.choice([0, 1, _log_int(rng, 1, 300)])}
+    if op == "rotary":
+        dim = rng.choice([32, 64, 64, 80, 96, 128, 128, 256])
+        axes = rng.randint(1, 4)
+        half = rng.choice([dim // 2, dim // 2, dim // 4])
+        cuts = sorted(rng.sample(range(1, half), axes - 1))
+        sections = [b - a for a, b in zip([0] + cuts, cuts + [half])]
+        kv = rng.choice([1, 2, 4, 8, 12])
+        heads = kv * rng.choice([1, 1, 2, 4])
+        batch = rng.randint(1, 8)
+        most = 80_000_000 // (batch * (heads + kv) * dim)
+        return {"op": "rotary", "dtype": rng.choice(["bf16", "bf16", "fp32"]), "batch": batch, "seq": _log_int(rng, 1, min(8192, most)), "heads": heads,
+                "kv_heads": kv, "dim": dim, "sections": ",".join(str(s) for s in sections), "interleaved": rng.random() < 0.5, "far": rng.choice([64, 4096, 1000000])}
+    if op == "clip":
+        width = rng.choice([64, 100, 513, 768, 1000, 1024, 2048, 4096])
+        layers = rng.randint(1, 6)
+        return {"op": "clip", "dtype": rng.choice(["bf16", "fp32"]), "layers": layers, "width": width, "inner": _log_int(rng, width, 4 * width) if width < 4096 else 8192,
+                "max_norm": rng.choice([0.5, 1.0, 1e6])}
+    dtype = rng.choice(["bf16", "bf16", "bf16", "fp32"])
+    one_row = dtype == "bf16" and rng.random() < 0.2
+    dim = rng.choice([32, 64, 64, 80, 96, 128, 128, 256] if dtype == "bf16" else [32, 64, 128])
+    kv = rng.choice([1, 2, 4, 8])
+    heads = kv * rng.choice([1, 1, 2, 4])
+    batch = rng.randint(1, 8)
+    # scores of a pass: fp32 products take several times the time of bf16 ones
+    budget = (1 << 30) * 128 // dim if dtype == "bf16" else 1 << 26
+    most = max(8, int(math.sqrt(budget / (batch * heads))))
+    if one_row:
+        seq_q, seq_kv, given = rng.randint(1, 4), _log_int(rng, 1, 16384), True
+    else:
+        seq_q = seq_kv = _log_int(rng, 1, min(8192, most))
+        given = rng.random() < 0.15
+        if given:
+            seq_q = _log_int(rng, 1, min(8192, most))
+    documents = 0 if given else rng.choice([0, 1, rng.randint(1, 12)])
+    causal = False if given else rng.random() < 0.7
+    return {"op": "attention", "dtype": dtype, "batch": batch, "seq_q": seq_q, "seq_kv": seq_kv, "heads": heads, "kv_heads": kv, "dim": dim, "causal": causal,
+            "documents": documents, "prefix": rng.choice([0, _log_int(rng, 1, 300)]) if causal else 0, "padding": rng.randint(0, seq_kv // 4) if documents else 0,
+            "given": given, "cap": rng.choice([0.0, 0.0, 20.0, 50.0]), "bias": rng.random() < 0.4, "train": not one_row and rng.random() < 0.7}
+
+
+# ---------------------------------------------------------------------------
+# Inputs
+# ---------------------------------------------------------------------------
+def _document_lengths(documents, room):
+    """Lengths that differ by up to a factor of about four and fill `room`."""
+    weights = [1.0 + 3.0 * ((i * 7 + 3) % 11) / 10.0 for i in range(documents)]
+    ends, total, run = [], sum(weights), 0.0
+    for w in weights:
+        run += w
+        ends.append(int(round(room * run / total)))
+    return [b - a for a, b in zip([0] + ends, ends)]
+
+
+def _starts(documents, padding, batch, seq, seed):
+    """int32 [batch, documents + 1]: every row holds the same lengths in an order of its own, padding behind the last."""
+    rng, rows = random.Random(seed), []
+    for _ in range(batch):
+        lengths = _document_lengths(documents, seq - padding)
+        rng.shuffle(lengths)
+        row = [0]
+        for n in lengths:
+            row.append(row[-1] + n)
+        rows.append(row)
+    return torch.tensor(rows, dtype=torch.int32)
+
+
+def _key_lengths(batch, seq_kv):
+    """How many keys each sequence has where the ranges are given: half of them to all."""
+    return [max(1, seq_kv - (b * 5 % 8) * seq_kv // 16) for b in range(batch)]
+
+
+def _clip_sizes(case):
+    """(element count, whether it is a norm's parameter) of a stack of layers: projections, inner products, norms and biases."""
+    w, n = case["width"], case["inner"]
+    one = [(w, True), (w, True), (4 * w * w, False), (w, True), (w, True), (n * w, False), (n, False), (w * n, False), (w, False)]
+    return one * case["layers"]
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed * 1000003 + 17)
+
+    def normal(shape, dtype, std=1.0):
+        return (torch.randn(shape, generator=gen, device=dev) * std).to(dtype)
+
+    state = dict(case)
+    if case["op"] == "clip":
+        dtype = DTYPES[case["dtype"]]
+        # weight gradients: small and unequal from tensor to tensor
+        state["grads"] = [normal((n,), torch.float32 if norm else dtype, 1e-3 * (1 + i % 5)) for i, (n, norm) in enumerate(_clip_sizes(case))]
+        return state
+    if case["op"] == "rotary":
+        dtype = DTYPES[case["dtype"]]
+        sections = [int(s) for s in case["sections"].split(",")]
+        half = sum(sections)
+        shape_q, shape_k = (case["batch"], case["seq"], case["heads"], case["dim"]), (case["batch"], case["seq"], case["kv_heads"], case["dim"])
+        for name, shape in (("q", shape_q), ("k", shape_k), ("dq", shape_q), ("dk", shape_k)):
+            state[name] = normal(shape, dtype)
+        state["positions"] = torch.randint(0, case["far"], (len(sections), case["batch"], case["seq"]), generator=gen, device=dev, dtype=torch.int32)
+        state["frequencies"] = torch.tensor([10000.0 ** (-i / half) for i in range(half)], dtype=torch.float32, device=dev)
+        state["sections_list"] = sections
+        return state
+    if case["op"] == "ranges":
+        # documents of any lengths, empty ones among them, with positions before the first and behind the last that are none's
+        cuts = torch.randint(0, case["seq"] + 1, (case["batch"], case["documents"] + 1), generator=gen, device=dev, dtype=torch.int32)
+        state["starts"] = cuts.sort(dim=1).values.contiguous()
+        shape = (case["batch"], case["documents"])
+        state["prefixes"] = torch.randint(0, case["prefix"] + 1, shape, generator=gen, device=dev, dtype=torch.int32) if case["prefix"] else None
+        return state
+    dtype = DTYPES[case["dtype"]]
+    B, Sq, Skv, H, KH, D = (case[n] for n in ("batch", "seq_q", "seq_kv", "heads", "kv_heads", "dim"))
+    # capped scores are large ones: that is what the cap is for
+    state["q"] = normal((B, Sq, H, D), dtype, 3.0 if case["cap"] else 1.0)
+    state["k"], state["v"] = normal((B, Skv, KH, D), dtype), normal((B, Skv, KH, D), dtype)
+    state["d_o"] = normal((B, Sq, H, D), dtype) if case["train"] else None
+    state["slopes"] = torch.tensor([2.0 ** (-8.0 * (h + 1) / H) for h in range(H)], dtype=torch.float32, device=dev) if case["bias"] else None
+    state["starts"] = _starts(case["documents"], case["padding"], B, Skv, seed).to(dev) if case["documents"] else None
+    state["prefixes"] = torch.full((B, max(1, case["documents"])), case["prefix"], dtype=torch.int32, device=dev) if case["prefix"] else None
+    if case["given"]:
+        lengths = _key_lengths(B, Skv)
+        random.Random(seed).shuffle(lengths)
+        hi = torch.tensor(lengths, dtype=torch.int32, device=dev)[:, None].expand(B, Sq)
+        state["ranges"] = torch.stack([torch.zeros_like(hi), hi], dim=-1).contiguous()
+    else:
+        state["ranges"] = None
+    return state
+
+
+# ---------------------------------------------------------------------------
+# The plain forms
+# ---------------------------------------------------------------------------
+def _plain_ranges(starts, prefixes, batch, seq, causal):
+    """int32 [batch, seq, 2]: the keys lo <= j < hi that each position sees; nothing is [0, 0)."""
+    dev = starts.device if starts is not None else prefixes.device if prefixes is not None else torch.device("cuda")
+    pos = torch.arange(seq, device=dev)[None, :].expand(batch, seq)
+    if starts is not None:
+        s = starts.long()
+        doc = torch.searchsorted(s.contiguous(), pos.contiguous(), right=True) - 1  # the last document that begins at or before the position
+        inside = (doc >= 0) & (doc < s.shape[1] - 1)
+        doc = doc.clamp(0, s.shape[1] - 2)
+        lo, end = s.gather(1, doc), s.gather(1, doc + 1)
+    else:
+        doc, inside = torch.zeros_like(pos), torch.ones_like(pos, dtype=torch.bool)
+        lo, end = torch.zeros_like(pos), torch.full_like(pos, seq)
+    hi = end
+    if causal:
+        hi = pos + 1
+        if prefixes is not None:
+            hi = torch.maximum(hi, lo + prefixes.long().gather(1, doc))
+        hi = torch.minimum(hi, end)
+    zero = torch.zeros_like(lo)
+    return torch.stack([torch.where(inside, lo, zero), torch.where(inside, hi, zero)], dim=-1).to(torch.int32)
+
+
+def _plain_attention(st):
+    B, Sq, Skv, H, KH, D = (st[n] for n in ("batch", "seq_q", "seq_kv", "heads", "kv_heads", "dim"))
+    G, scale, cap = H // KH, D ** -0.5, st["cap"]
+    ranges = st["ranges"] if st["ranges"] is not None else _plain_ranges(st["starts"], st["prefixes"], B, Skv, st["causal"])
+
+    def heads(t):  # [B, S, h, D] -> float [B * H, S, D], shared heads repeated
+        t = t.float().permute(0, 2, 1, 3)
+        if t.shape[1] != H:
+            t = t.repeat_interleave(G, dim=1)
+        return t.reshape(B * H, t.shape[2], D).contiguous()
+
+    q, k, v = heads(st["q"]), heads(st["k"]), heads(st["v"])
+    s = torch.matmul(q, k.transpose(1, 2).contiguous()).mul_(scale)
+    t = None
+    if cap:
+        t = s.div_(cap).tanh_()
+        s = t * cap
+    s = s.view(B, H, Sq, Skv)
+    j = torch.arange(Skv, device=s.device)
+    if st["slopes"] is not None:
+        distance = (torch.arange(Sq, device=s.device)[:, None] - j[None, :]).abs().float()
+        s = s.sub_(st["slopes"][None, :, None, None] * distance) if cap == 0 else s - st["slopes"][None, :, None, None] * distance
+    hidden = (j[None, None, :] < ranges[:, :, :1]) | (j[None, None, :] >= ranges[:, :, 1:])
+    s = s.masked_fill_(hidden[:, None], float("-inf"))
+    m = s.max(dim=-1, keepdim=True).values
+    empty = m == float("-inf")
+    m = m.masked_fill(empty, 0.0)
+    p = s.sub_(m).exp_()
+    total = p.sum(dim=-1, keepdim=True)
+    lse = torch.where(empty, float("-inf"), m + total.log()).view(B, H, Sq)
+    p = p.div_(total.masked_fill(empty, 1.0)).view(B * H, Sq, Skv)
+    o = torch.matmul(p, v)
+    out = {"o": o.view(B, H, Sq, D).permute(0, 2, 1, 3).to(st["q"].dtype).contiguous(), "lse": lse}
+    if st["train"]:
+        g = heads(st["d_o"])
+        ds = torch.matmul(g, v.transpose(1, 2).contiguous())
+        ds = ds.sub_((o * g).sum(dim=-1, keepdim=True)).mul_(p)
+        if t is not None:
+            ds = ds.mul_(t.view_as(ds).square_().neg_().add_(1.0))
+        ds = ds.mul_(scale)
+        dq = torch.matmul(ds, k)
+        dk = torch.matmul(ds.transpose(1, 2).contiguous(), q)
+        dv = torch.matmul(p.transpose(1, 2).contiguous(), g)
+        out["dq"] = dq.view(B, H, Sq, D).permute(0, 2, 1, 3).to(st["q"].dtype).contiguous()
+        out["dk"] = dk.view(B, KH, G, Skv, D).sum(dim=2).permute(0, 2, 1, 3).to(st["q"].dtype).contiguous()
+        out["dv"] = dv.view(B, KH, G, Skv, D).sum(dim=2).permute(0, 2, 1, 3).to(st["q"].dtype).contiguous()
+    return out
+
+
+def _plain_rotary(st):
+    axis = torch.repeat_interleave(torch.arange(len(st["sections_list"]), device="cuda"), torch.tensor(st["sections_list"], device="cuda"))
+    angle = st["positions"].double()[axis].permute(1, 2, 0) * st["frequencies"].double()  # [B, S, half]
+    cos, sin = angle.cos().float()[:, :, None], angle.sin().float()[:, :, None]
+    half = cos.shape[-1]
+
+    def turn(x, sin):
+        y = x.float()
+        if st["interleaved"]:
+            a, b = y[..., 0:2 * half:2], y[..., 1:2 * half:2]
+            r = torch.stack([a * cos - b * sin, a * sin + b * cos], dim=-1).flatten(-2)
+        else:
+            a, b = y[..., :half], y[..., half:2 * half]
+            r = torch.cat([a * cos - b * sin, a * sin + b * cos], dim=-1)
+        return torch.cat([r, y[..., 2 * half:]], dim=-1).to(x.dtype)
+
+    return {"q": turn(st["q"], sin), "k": turn(st["k"], sin), "dq": turn(st["dq"], -sin), "dk": turn(st["dk"], -sin)}
+
+
+def _plain_clip(st):
+    norm = torch.stack([g.float().square().sum(dtype=torch.float64) for g in st["grads"]]).sum().sqrt()
+    factor = torch.clamp(st["max_norm"] / (norm + 1e-6), max=1.0).float()
+    return {"norm": norm.float(), "clipped": [(g.float() * factor).to(g.dtype) for g in st["grads"]]}
+
+
+# ---------------------------------------------------------------------------
+# One pass
+# ---------------------------------------------------------------------------
+def run(state):
+    st = state
+    if own:
+        ffk = _ffk()
+        if st["op"] == "ranges":
+            return ffk.attention_key_ranges(st["batch"], st["seq"], st["seq"], causal=st["causal"], document_starts=st["starts"], prefix_lengths=st["prefixes"])
+        if st["op"] == "rotary":
+            q, k = ffk.rotary_forward(st["q"], st["k"], st["positions"], st["frequencies"], st["sections_list"], interleaved=st["interleaved"])
+            dq, dk = ffk.rotary_backward(st["dq"], st["dk"], st["positions"], st["frequencies"], st["sections_list"], interleaved=st["interleaved"])
+            return {"q": q, "k": k, "dq": dq, "dk": dk}
+        if st["op"] == "clip":
+            clipped, norm = ffk.clip_grad_norm(st["grads"], st["max_norm"], out=[torch.empty_like(g) for g in st["grads"]])
+            return {"norm": norm, "clipped": clipped}
+        ranges = st["ranges"]
+        if ranges is None:
+            ranges = ffk.attention_key_ranges(st["batch"], st["seq_q"], st["seq_kv"], causal=st["causal"], document_starts=st["starts"],
+                                              prefix_lengths=st["prefixes"])
+        how = dict(score_cap=st["cap"], key_ranges=ranges, distance_slopes=st["slopes"])
+        o, lse = ffk.masked_attention_forward(st["q"], st["k"], st["v"], st["dim"] ** -0.5, **how)
+        out = {"o": o, "lse": lse}
+        if st["train"]:
+            out["dq"], out["dk"], out["dv"] = ffk.masked_attention_backward(st["q"], st["k"], st["v"], o, st["d_o"], lse, st["dim"] ** -0.5, **how)
+        return out
+    if st["op"] == "ranges":
+        return _plain_ranges(st["starts"], st["prefixes"], st["batch"], st["seq"], st["causal"])
+    return {"attention": _plain_attention, "rotary": _plain_rotary, "clip": _plain_clip}[st["op"]](st)
+
+
+# ---------------------------------------------------------------------------
+# What a pass cannot do without
+# ---------------------------------------------------------------------------
+def _visible_pairs(case):
+    if case["given"]:
+        return case["seq_q"] * sum(_key_lengths(case["batch"], case["seq_kv"]))
+    lengths = _document_lengths(case["documents"], case["seq_kv"] - case["padding"]) if case["documents"] else [case["seq_kv"]]
+    if not case["causal"]:
+        return case["batch"] * sum(n * n for n in lengths)
+    return case["batch"] * sum(n * (n + 1) // 2 + min(n, case["prefix"]) * max(0, min(n, case["prefix"]) - 1) // 2 for n in lengths)
+
+
+def work(case):
+    if case["op"] == "clip":
+        size = DTYPES[case["dtype"]].itemsize
+        return {"bytes": sum(2 * n * (4 if norm else size) for n, norm in _clip_sizes(case)), "flops": sum(3 * n for n, _ in _clip_sizes(case))}
+    if case["op"] == "ranges":
+        docs = case["documents"]
+        return {"bytes": 8 * case["batch"] * case["seq"] + 4 * case["batch"] * (docs + 1 + (docs if case["prefix"] else 0)), "flops": 0}
+    size = DTYPES[case["dtype"]].itemsize
+    if case["op"] == "rotary":
+        tokens = case["batch"] * case["seq"]
+        axes = case["sections"].count(",") + 1
+        elems = tokens * (case["heads"] + case["kv_heads"]) * case["dim"]
+        return {"bytes": 4 * elems * size + 4 * axes * tokens, "flops": 6 * elems}
+    B, Sq, Skv, H, KH, D = (case[n] for n in ("batch", "seq_q", "seq_kv", "heads", "kv_heads", "dim"))
+    keys = sum(_key_lengths(B, Skv)) if case["given"] else B * Skv
+    q_elems, k_elems = B * Sq * H * D, keys * KH * D
+    forward = (2 * q_elems + 2 * k_elems) * size + 4 * B * H * Sq
+    return {"bytes": forward + ((2 * q_elems + 2 * k_elems) * size if case["train"] else 0), "flops": (14 if case["train"] else 4) * D * H * _visible_pairs(case)}
+
+
+# ---------------------------------------------------------------------------
+# The definitions in 64 bits
+# ---------------------------------------------------------------------------
+def _exact_visible(st, b):
+    """bool [Sq, Skv]: what sequence b's rows see, from the masks' definitions."""
+    dev = st["q"].device
+    i, j = torch.arange(st["seq_q"], device=dev)[:, None], torch.arange(st["seq_kv"], device=dev)[None, :]
+    if st["ranges"] is not None:
+        return (j >= st["ranges"][b, :, :1]) & (j < st["ranges"][b, :, 1:])
+    starts = st["starts"][b].tolist() if st["starts"] is not None else [0, st["seq_kv"]]
+    of_document = torch.full((st["seq_kv"],), -1, device=dev)
+    prefix = torch.zeros((st["seq_kv"],), dtype=torch.bool, device=dev)
+    for d, (a, z) in enumerate(zip(starts, starts[1:])):
+        of_document[a:z] = d
+        if st["prefixes"] is not None:
+            prefix[a:min(z, a + int(st["prefixes"][b, d]))] = True
+    same = (of_document[:, None] == of_document[None, :]) & (of_document[:, None] >= 0)
+    return same & ((j <= i) | prefix[None, :]) if st["causal"] else same
+
+
+def exact(case, seed):
+    if case["op"] == "ranges":
+        return None
+    st = prepare(case, seed)
+    if case["op"] == "clip":
+        squares = sum(float(torch.dot(g.double(), g.double())) for g in st["grads"])
+        norm = math.sqrt(squares)
+        factor = min(1.0, case["max_norm"] / (norm + 1e-6))
+        return {"norm": norm, "clipped": [g.double() * factor for g in st["grads"]]}
+    if case["op"] == "rotary":
+        half = sum(st["sections_list"])
+        axis = [a for a, n in enumerate(st["sections_list"]) for _ in range(n)]
+        first = [2 * i if case["interleaved"] else i for i in range(half)]
+        second = [2 * i + 1 if case["interleaved"] else i + half for i in range(half)]
+        theta = st["positions"][axis].double() * st["frequencies"].double()[:, None, None]  # [half, B, S]
+        turn = torch.polar(torch.ones_like(theta), theta).permute(1, 2, 0)[:, :, None]
+        out = {}
+        for name in ("q", "k", "dq", "dk"):
+            x = st[name].double()
+            z = torch.complex(x[..., first], x[..., second]) * (turn.conj() if name.startswith("d") else turn)
+            x[..., first], x[..., second] = z.real, z.imag
+            out[name] = x
+        return out
+    B, Sq, Skv, H, KH, D = (case[n] for n in ("batch", "seq_q", "seq_kv", "heads", "kv_heads", "dim"))
+    out = {"o": torch.zeros((B, Sq, H, D), dtype=torch.float64, device="cuda"), "lse": torch.zeros((B, H, Sq), dtype=torch.float64, device="cuda")}
+    if case["train"]:
+        out.update(dq=torch.zeros_like(out["o"]), dk=torch.zeros((B, Skv, KH, D), dtype=torch.float64, device="cuda"))
+        out["dv"] = torch.zeros_like(out["dk"])
+    steps = (torch.arange(Sq, device="cuda")[:, None] - torch.arange(Skv, device="cuda")[None, :]).abs().double() if case["bias"] else None
+    for b in range(B):
+        visible = _exact_visible(st, b)
+        for h in range(H):
+            q, k, v = st["q"][b, :, h].double(), st["k"][b, :, h * KH // H].double(), st["v"][b, :, h * KH // H].double()
+            score = (q @ k.t()) / math.sqrt(D)
+            slope = None
+            if case["cap"]:
+                tanh = torch.tanh(score / case["cap"])
+                score, slope = case["cap"] * tanh, 1 - tanh * tanh
+            if case["bias"]:
+                score = score - st["slopes"][h].double() * steps
+            score = torch.where(visible, score, float("-inf"))
+            lse = torch.logsumexp(score, dim=1)
+            p = torch.exp(score - torch.where(lse == float("-inf"), 0.0, lse)[:, None])
+            o = p @ v
+            out["o"][b, :, h], out["lse"][b, h] = o, lse
+            if case["train"]:
+                g = st["d_o"][b, :, h].double()
+                ds = p * (g @ v.t() - (g * o).sum(dim=1, keepdim=True))
+                if slope is not None:
+                    ds = ds * slope
+                ds = ds / math.sqrt(D)
+                out["dq"][b, :, h] = ds @ k
+                out["dk"][b, :, h * KH // H] += ds.t() @ q
+                out["dv"][b, :, h * KH // H] += p.t() @ g
+    return out
