@@ -163,6 +163,8 @@ def prepare(case, seed):
         dtype = DTYPES[case["dtype"]]
         # weight gradients: small and unequal from tensor to tensor
         state["grads"] = [normal((n,), torch.float32 if norm else dtype, 1e-3 * (1 + i % 5)) for i, (n, norm) in enumerate(_clip_sizes(case))]
+        # the update reads the clipped ones, which a program keeps beside the gradients that it adds into
+        state["clipped"] = [torch.empty_like(g) for g in state["grads"]]
         return state
     if case["op"] == "rotary":
         dtype = DTYPES[case["dtype"]]
@@ -315,7 +317,7 @@ def run(state):
             dq, dk = ffk.rotary_backward(st["dq"], st["dk"], st["positions"], st["frequencies"], st["sections_list"], interleaved=st["interleaved"])
             return {"q": q, "k": k, "dq": dq, "dk": dk}
         if st["op"] == "clip":
-            clipped, norm = ffk.clip_grad_norm(st["grads"], st["max_norm"], out=[torch.empty_like(g) for g in st["grads"]])
+            clipped, norm = ffk.clip_grad_norm(st["grads"], st["max_norm"], out=st["clipped"])
             return {"norm": norm, "clipped": clipped}
         ranges = st["ranges"]
         if ranges is None:
