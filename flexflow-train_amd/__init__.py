@@ -80,6 +80,25 @@ class EncoderLayerParams(ctypes.Structure):
                                    "w1", "b1", "w2", "b2")]
 
 
+class MaskedAttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i64), ("heads", c_i64), ("kv_heads", c_i64), ("seq_q", c_i64), ("seq_kv", c_i64),
+        ("head_dim", c_i64), ("v_head_dim", c_i64),  # v_head_dim 0 = head_dim
+        ("q_batch_stride", c_i64), ("q_seq_stride", c_i64),
+        ("k_batch_stride", c_i64), ("k_seq_stride", c_i64),
+        ("v_batch_stride", c_i64), ("v_seq_stride", c_i64),
+        ("o_batch_stride", c_i64), ("o_seq_stride", c_i64),
+        ("query_offset", c_i64), ("scale", c_f), ("score_cap", c_f), ("causal", c_int),
+    ]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [(n, c_i64) for n in (
+        "batch", "seq", "q_heads", "k_heads", "head_dim", "q_batch_stride", "q_seq_stride", "k_batch_stride", "k_seq_stride",
+        "q_out_batch_stride", "q_out_seq_stride", "k_out_batch_stride", "k_out_seq_stride", "num_axes")]
+    _fields_ += [("sections", c_i64 * 4), ("interleaved", c_i64)]
+
+
 # name -> (restype, argtypes); must list every symbol include/ffk.h declares.
 SIGNATURES = {
     "ffk_last_error": (ctypes.c_char_p, []),
@@ -180,6 +199,18 @@ SIGNATURES = {
                                       c_p, c_p]),
     "ffk_attention_backward": (c_int, [c_p, c_int, ctypes.POINTER(AttentionDesc), c_p, c_p, c_p,
                                        c_p, c_p, c_p, c_p, c_p, c_p, c_p]),
+    "ffk_attention_key_ranges": (c_int, [c_p, c_i64, c_i64, c_i64, c_i64, c_int, c_p, c_i64, c_p, c_p]),
+    "ffk_masked_attention_forward_workspace_bytes": (c_sz, [ctypes.POINTER(MaskedAttentionDesc), c_int]),
+    "ffk_masked_attention_forward": (c_int, [c_p, c_int, ctypes.POINTER(MaskedAttentionDesc), c_p, c_p, c_p, c_p, c_p,
+                                             c_p, c_p, c_p, c_sz]),
+    "ffk_masked_attention_backward_workspace_bytes": (c_sz, [ctypes.POINTER(MaskedAttentionDesc), c_int]),
+    "ffk_masked_attention_backward": (c_int, [c_p, c_int, ctypes.POINTER(MaskedAttentionDesc), c_p, c_p, c_p, c_p, c_p,
+                                              c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_sz]),
+    "ffk_rotary_forward": (c_int, [c_p, c_int, ctypes.POINTER(RotaryDesc), c_p, c_p, c_p, c_p, c_p, c_p]),
+    "ffk_rotary_backward": (c_int, [c_p, c_int, ctypes.POINTER(RotaryDesc), c_p, c_p, c_p, c_p, c_p, c_p]),
+    "ffk_grad_norm_workspace_bytes": (c_sz, [c_int]),
+    "ffk_global_grad_norm": (c_int, [c_p, c_p, c_p, c_p, c_int, c_p, c_p, c_sz]),
+    "ffk_clip_grad_norm": (c_int, [c_p, c_p, c_p, c_p, c_p, c_int, c_f, c_p, c_p, c_sz]),
     "ffk_mha_weight_elements": (c_sz, [ctypes.POINTER(MHADesc)]),
     "ffk_mha_reserve_bytes": (c_sz, [ctypes.POINTER(MHADesc), c_int]),
     "ffk_mha_forward": (c_int, [c_p, c_int, ctypes.POINTER(MHADesc), c_p, c_p, c_p, c_p, c_p,
@@ -573,6 +604,47 @@ def adam_update(weight, grad, adam_m, adam_v, alpha_t, beta1=0.9, beta2=0.999, w
     return weight
 
 
+def _grad_list(grads):
+    n = len(grads)
+    return (n, (c_int * n)(*[dtype_of(g) for g in grads]), (c_p * n)(*[ptr(g) for g in grads]),
+            (c_i64 * n)(*[g.numel() for g in grads]))
+
+
+def _grad_norm_buffers(grads, norm, workspace):
+    torch = _torch()
+    device = grads[0].device if grads else "cuda"
+    if norm is None:
+        norm = torch.empty((), dtype=torch.float32, device=device)
+    elif norm.dtype != torch.float32:
+        raise ValueError("norm: float32 expected")
+    if workspace is None:
+        workspace = torch.empty((_call.ffk_grad_norm_workspace_bytes(len(grads)),), dtype=torch.uint8, device=device)
+    return norm, workspace
+
+
+def global_grad_norm(grads, norm=None, workspace=None):
+    """The norm over all tensors of the list (fp32 and bf16 in any order), as a float32 tensor on the device."""
+    n, dtypes, ptrs, elems = _grad_list(grads)
+    norm, workspace = _grad_norm_buffers(grads, norm, workspace)
+    _call.ffk_global_grad_norm(dtypes, ptrs, elems, n, norm, workspace, workspace.numel())
+    return norm
+
+
+def clip_grad_norm(grads, max_norm, out=None, norm=None, workspace=None):
+    """Scales the gradients to a norm of at most max_norm, in place or into `out`; (the scaled ones, their norm before)."""
+    n, dtypes, ptrs, elems = _grad_list(grads)
+    outs = ptrs
+    if out is None:
+        out = grads
+    else:
+        if len(out) != n or any(a.dtype != b.dtype or a.numel() != b.numel() for a, b in zip(out, grads)):
+            raise ValueError("clip_grad_norm: out does not fit grads")
+        outs = (c_p * n)(*[ptr(g) for g in out])
+    norm, workspace = _grad_norm_buffers(grads, norm, workspace)
+    _call.ffk_clip_grad_norm(dtypes, ptrs, outs, elems, n, max_norm, norm, workspace, workspace.numel())
+    return out, norm
+
+
 def sparse_categorical_crossentropy_loss_backward(logit, label, num_samples, num_classes, k,
                                                   scale_factor, out=None):
     torch = _torch()
@@ -685,6 +757,126 @@ def attention_backward(q, k, v, o, d_o, lse, scale, causal, desc=None):
     delta = torch.empty_like(lse)
     _call.ffk_attention_backward(dtype_of(q), desc, q, k, v, o, d_o, lse, delta, dq, dk, dv)
     return dq, dk, dv
+
+
+def _int32(t, shape, what):
+    torch = _torch()
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape):
+        raise ValueError("%s: int32 %s expected, %s %s given" % (what, list(shape), t.dtype, list(t.shape)))
+    return t
+
+
+def attention_key_ranges(batch, seq_q, seq_kv, causal=False, document_starts=None, prefix_lengths=None, query_offset=0,
+                         out=None, device="cuda"):
+    """int32 [batch, seq_q, 2]: the keys lo <= j < hi that each query row sees (ffk_attention_key_ranges)."""
+    torch = _torch()
+    docs = 1
+    if document_starts is not None:
+        docs = document_starts.shape[-1] - 1
+        _int32(document_starts, (batch, docs + 1), "document_starts")
+    _int32(prefix_lengths, (batch, docs), "prefix_lengths")
+    if out is None:
+        like = document_starts if document_starts is not None else prefix_lengths
+        out = torch.empty((batch, seq_q, 2), dtype=torch.int32, device=device if like is None else like.device)
+    _int32(out, (batch, seq_q, 2), "out")
+    _call.ffk_attention_key_ranges(batch, seq_q, seq_kv, query_offset, int(causal), document_starts, docs, prefix_lengths, out)
+    return out
+
+
+def masked_attention_desc(q, k, v, scale, causal=False, score_cap=0.0, query_offset=0):
+    """Descriptor for dense q [B, Sq, H, D], k [B, Skv, KH, D], v [B, Skv, KH, Dv] tensors."""
+    B, Sq, H, D = q.shape
+    _, Skv, KH, _ = k.shape
+    Dv = v.shape[3]
+    if k.shape[0] != B or k.shape[3] != D or tuple(v.shape[:3]) != (B, Skv, KH):
+        raise ValueError("masked attention: q %s, k %s and v %s do not fit each other" % (list(q.shape), list(k.shape), list(v.shape)))
+    return MaskedAttentionDesc(B, H, KH, Sq, Skv, D, Dv, Sq * H * D, H * D, Skv * KH * D, KH * D, Skv * KH * Dv, KH * Dv,
+                               Sq * H * Dv, H * Dv, query_offset, scale, score_cap, int(causal))
+
+
+def _masked_attention_args(q, k, v, desc, key_ranges, distance_slopes):
+    torch = _torch()
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("masked attention: q, k and v have one data type")
+    _int32(key_ranges, (desc.batch, desc.seq_q, 2), "key_ranges")
+    if distance_slopes is not None and (distance_slopes.dtype != torch.float32 or distance_slopes.numel() != desc.heads):
+        raise ValueError("distance_slopes: float32 [%d] expected" % desc.heads)
+
+
+def masked_attention_forward(q, k, v, scale, causal=False, score_cap=0.0, key_ranges=None, distance_slopes=None,
+                             query_offset=0, desc=None, out=None, lse=None, workspace=None):
+    """(o, lse).  desc: strides of its own (q, k, v are then the tensors it points into, out the one for o)."""
+    torch = _torch()
+    desc = desc or masked_attention_desc(q, k, v, scale, causal, score_cap, query_offset)
+    _masked_attention_args(q, k, v, desc, key_ranges, distance_slopes)
+    if out is None:
+        out = torch.empty((desc.batch, desc.seq_q, desc.heads, desc.v_head_dim or desc.head_dim), dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((desc.batch, desc.heads, desc.seq_q), dtype=torch.float32, device=q.device)
+    dtype = dtype_of(q)
+    if workspace is None:
+        need = _call.ffk_masked_attention_forward_workspace_bytes(desc, dtype)
+        if need:
+            workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    _call.ffk_masked_attention_forward(dtype, desc, q, k, v, key_ranges, distance_slopes, out, lse, workspace,
+                                       0 if workspace is None else workspace.numel())
+    return out, lse
+
+
+def masked_attention_backward(q, k, v, o, d_o, lse, scale, causal=False, score_cap=0.0, key_ranges=None, distance_slopes=None,
+                              query_offset=0, desc=None, grads=None, workspace=None):
+    """(dq, dk, dv), each with the strides of its tensor."""
+    torch = _torch()
+    desc = desc or masked_attention_desc(q, k, v, scale, causal, score_cap, query_offset)
+    _masked_attention_args(q, k, v, desc, key_ranges, distance_slopes)
+    if o.dtype != q.dtype or d_o.dtype != q.dtype or lse.dtype != torch.float32:
+        raise ValueError("masked attention: o and d_o have the data type of q, lse is float32")
+    dq, dk, dv = grads if grads is not None else (torch.empty_like(q), torch.empty_like(k), torch.empty_like(v))
+    dtype = dtype_of(q)
+    if workspace is None:
+        workspace = torch.empty((_call.ffk_masked_attention_backward_workspace_bytes(desc, dtype),), dtype=torch.uint8, device=q.device)
+    _call.ffk_masked_attention_backward(dtype, desc, q, k, v, key_ranges, distance_slopes, o, d_o, lse, dq, dk, dv, workspace,
+                                        workspace.numel())
+    return dq, dk, dv
+
+
+def rotary_desc(q, k, sections, interleaved=False):
+    """Descriptor for dense q [B, S, H, D], k [B, S, KH, D] (or None) and outputs laid out the same."""
+    B, S, H, D = q.shape
+    KH = 0 if k is None else k.shape[2]
+    if k is not None and (tuple(k.shape[:2]) != (B, S) or k.shape[3] != D):
+        raise ValueError("rotary: q %s and k %s do not fit each other" % (list(q.shape), list(k.shape)))
+    sections = [int(s) for s in sections]
+    if not 1 <= len(sections) <= 4:
+        raise ValueError("rotary: one to four axes, not %d" % len(sections))
+    return RotaryDesc(B, S, H, KH, D, S * H * D, H * D, S * KH * D, KH * D, S * H * D, H * D, S * KH * D, KH * D, len(sections),
+                      (c_i64 * 4)(*sections), int(interleaved))
+
+
+def _rotary(entry, q, k, positions, frequencies, sections, interleaved, desc, q_out, k_out):
+    torch = _torch()
+    desc = desc or rotary_desc(q, k, sections, interleaved)
+    _int32(positions, (desc.num_axes, desc.batch, desc.seq), "positions")
+    if frequencies.dtype != torch.float32 or frequencies.numel() != sum(desc.sections[:desc.num_axes]):
+        raise ValueError("frequencies: float32 [%d] expected" % sum(desc.sections[:desc.num_axes]))
+    if q_out is None:
+        q_out = torch.empty_like(q)
+    if k_out is None and k is not None:
+        k_out = torch.empty_like(k)
+    if any(t is not None and t.dtype != q.dtype for t in (k, q_out, k_out)):
+        raise ValueError("rotary: all tensors have one data type")
+    entry(dtype_of(q), desc, q, k, positions, frequencies, q_out, k_out)
+    return q_out, k_out
+
+
+def rotary_forward(q, k, positions, frequencies, sections, interleaved=False, desc=None, q_out=None, k_out=None):
+    """(q_out, k_out): q and k turned by their tokens' positions; q_out=q, k_out=k works in place."""
+    return _rotary(_call.ffk_rotary_forward, q, k, positions, frequencies, sections, interleaved, desc, q_out, k_out)
+
+
+def rotary_backward(dq_out, dk_out, positions, frequencies, sections, interleaved=False, desc=None, dq=None, dk=None):
+    """(dq, dk): the gradients turned back."""
+    return _rotary(_call.ffk_rotary_backward, dq_out, dk_out, positions, frequencies, sections, interleaved, desc, dq, dk)
 
 
 def mha_desc(num_samples, num_heads, q_size, k_size, v_size, q_proj, k_proj, v_proj, o_proj,

@@ -35,7 +35,7 @@ HIP_FLAGS = [
 ]
 
 
-# Per-file additions.  attention.hip: its backward kernels keep 128-160
+# Per-file additions.  attention.hip, masked_attention_*.hip: their kernels keep 128-160
 # accumulator registers live across the loop; by default the compiler selects
 # the MFMA form whose accumulators sit in accumulation registers and then
 # copies every accumulator in and out of them around each step (several hundred
@@ -47,6 +47,12 @@ EXTRA_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
     "attention_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "masked_attention_fwd_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "masked_attention_fwd_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "masked_attention_dq_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "masked_attention_dq_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "masked_attention_dkdv_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "masked_attention_dkdv_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "optimizer.hip": ["-ffp-contract=off"],
     "loss.hip": ["-ffp-contract=off"],
 }

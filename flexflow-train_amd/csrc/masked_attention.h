@@ -1,0 +1,206 @@
+// Masked attention: what its forward and backward kernels share.
+//
+// For batch b, query head h (which reads key head h / G, G = heads / kv_heads), query row i at position
+// p_i = query_offset + i and key j:
+//   x = scale q_i . k_j      s = cap tanh(x / cap)  (cap 0: x)  - slope_h |p_i - j|
+//   j is seen iff lo_i <= j < hi_i   (and j <= p_i if causal)
+//   P = softmax over the seen keys, O = P V, lse = log sum exp(s); a row that sees nothing: O = 0, lse = -inf
+//   delta_i = O_i . dO_i     dS = P (dO V^T - delta)     dX = dS (1 - tanh^2) scale
+//   dQ = dX K      dK = dX^T Q, dV = P^T dO, summed over the G heads that read the key head
+//
+// The G query heads of a key head are one longer axis of rows, r = i G + g: they share the tiles of K and V that a
+// workgroup brings into LDS, the keys' gradients are sums over that one axis (no atomics), and a few query rows still
+// fill an MFMA tile.  All kernels compute scores transposed or not such that a lane owns a row's (forward, dQ) or a
+// key's (dK, dV) column of the 32 x 32 accumulator, and feed the accumulator to the next product from registers:
+//   MFMA 32x32: A operand row l%32, B operand column l%32, both k = 8*(l/32)..+7 of a step of 16; accumulator element
+//   r: row 8*(r/4) + 4*(l/32) + r%4, column l%32.  An accumulator's elements 8s..8s+7 are the k-slots of step s of
+//   the next product; its other operand is read with the same permutation.  fp32 takes a step of 16 as eight
+//   32x32x2 instructions on the same slots, so that both types share every index below.
+#pragma once
+#include "attention_common.h"
+
+namespace ffk {
+
+// Rows that a summary of ranges covers: the dQ kernels write one for every 32 rows, the dK/dV kernels skip by them.
+struct RangeSummary {
+  int lo_min, hi_max;  // every key that some row sees lies in [lo_min, hi_max)
+  int lo_max, hi_min;  // every row sees all of [lo_max, hi_min)
+};
+
+struct MaskedAttnParams {
+  void const *q, *k, *v;
+  void *o;
+  void const *d_o;
+  float *lse;
+  float *delta;
+  void *dq, *dk, *dv;
+  int const *ranges;    // [B, Sq, 2] or NULL
+  float const *slopes;  // [H] or NULL
+  RangeSummary *summary;  // [B, ceil(Sq G / 32)]
+  int B, H, KH, G, Sq, Skv, Dq, Dv, R;  // R = Sq G rows of a key head
+  int64_t q_bs, q_ss, k_bs, k_ss, v_bs, v_ss, o_bs, o_ss;
+  int q_offset;
+  float scale, scale_log2;
+  float cap_in;   // 2 log2(e) scale / cap: tanh(x / cap) = 1 - 2 / (1 + 2^(cap_in raw))
+  float cap_out;  // cap log2(e)
+  float inv_cap_scale;  // scale / cap
+  int causal;
+  FastDiv group;
+  // forward, split over the keys: partial O (unnormalised), maximum and sum of each part
+  int splits;
+  float *part_o, *part_ml;
+};
+
+__device__ __forceinline__ void row_of(MaskedAttnParams const &p, int r, int &i, int &g) {
+  uint32_t a, b;
+  p.group.divmod((uint32_t)r, a, b);
+  i = (int)a;
+  g = (int)b;
+}
+// The keys that row i of batch b sees, within [0, Skv]; nothing is (INT_MAX / 2, 0), which widens no window.
+__device__ __forceinline__ void row_range(MaskedAttnParams const &p, int b, int i, int &lo, int &hi) {
+  lo = 0;
+  hi = p.Skv;
+  if (p.ranges != nullptr) {
+    int2 const v = reinterpret_cast<int2 const *>(p.ranges)[(int64_t)b * p.Sq + i];
+    lo = max(v.x, 0);
+    hi = min(v.y, p.Skv);
+  }
+  if (p.causal) hi = min(hi, p.q_offset + i + 1);
+  if (lo >= hi) {
+    lo = 1 << 30;
+    hi = 0;
+  }
+}
+
+// ---- one step of 16 of a product, for either type -------------------------
+template <typename T>
+struct Frag;
+template <>
+struct Frag<bf16> {
+  bf16x8 v;
+};
+template <>
+struct Frag<float> {
+  f32x4 a, b;
+};
+__device__ __forceinline__ void mma(f32x16 &acc, Frag<bf16> const &a, Frag<bf16> const &b) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16 &acc, Frag<float> const &a, Frag<float> const &b) {
+#pragma unroll
+  for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.a[j], b.a[j], acc, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.b[j], b.b[j], acc, 0, 0, 0);
+}
+// 8 elements from d0 on of a row in memory, zeros past the head size D (a multiple of 8, fp32: of 4)
+__device__ __forceinline__ Frag<bf16> frag_row(bf16 const *row, int d0, int D) {
+  union {
+    u32x4 u;
+    bf16x8 b;
+  } x;
+  x.u = u32x4{0u, 0u, 0u, 0u};
+  if (d0 < D) x.u = *reinterpret_cast<u32x4 const *>(row + d0);
+  return Frag<bf16>{x.b};
+}
+__device__ __forceinline__ Frag<float> frag_row(float const *row, int d0, int D) {
+  Frag<float> f = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+  if (d0 < D) f.a = *reinterpret_cast<f32x4 const *>(row + d0);
+  if (d0 + 4 < D) f.b = *reinterpret_cast<f32x4 const *>(row + d0 + 4);
+  return f;
+}
+// 8 elements of a row of an LDS tile
+__device__ __forceinline__ Frag<bf16> frag_lds(bf16 const *p) { return Frag<bf16>{*reinterpret_cast<bf16x8 const *>(p)}; }
+__device__ __forceinline__ Frag<float> frag_lds(float const *p) {
+  return Frag<float>{*reinterpret_cast<f32x4 const *>(p), *reinterpret_cast<f32x4 const *>(p + 4)};
+}
+// The slots of step s of an accumulator whose rows are the tile's rows, down the columns col0 + l%32: `tile` points at
+// the lane's place (turn_off) of the tile's first row.
+template <typename T>
+__device__ __forceinline__ int turn_off(int stride, int lane);
+template <>
+__device__ __forceinline__ int turn_off<bf16>(int stride, int lane) { return lane_tr_off(stride, lane); }
+template <>
+__device__ __forceinline__ int turn_off<float>(int stride, int lane) { return 4 * (lane >> 5) * stride + (lane & 31); }
+__device__ __forceinline__ Frag<bf16> frag_turned(bf16 const *tile, int stride, int s, int col0) {
+  return Frag<bf16>{frag_tr_acc(tile, stride, 0, s, col0)};
+}
+__device__ __forceinline__ Frag<float> frag_turned(float const *tile, int stride, int s, int col0) {
+  Frag<float> f;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    f.a[j] = tile[(16 * s + j) * stride + col0];
+    f.b[j] = tile[(16 * s + 8 + j) * stride + col0];
+  }
+  return f;
+}
+__device__ __forceinline__ Frag<bf16> frag_acc(float const *v, bf16 const *) { return Frag<bf16>{pack8(v)}; }
+__device__ __forceinline__ Frag<float> frag_acc(float const *v, float const *) {
+  return Frag<float>{{v[0], v[1], v[2], v[3]}, {v[4], v[5], v[6], v[7]}};
+}
+
+// Row strides of LDS tiles, in elements.  A tile that is read by rows (16 bytes a lane, 16 rows at a time) wants rows
+// 4 banks apart, one that is read turned (bf16: 4 rows x 64 bytes) 16 banks apart, one that is read both ways 20.
+template <typename T, int DP>
+struct TileStride {
+  static constexpr int row = sizeof(T) == 2 ? DP + 8 : DP + 4;
+  static constexpr int turned = sizeof(T) == 2 ? (DP % 64 == 0 ? DP + 32 : DP) : DP + 4;
+  static constexpr int both = sizeof(T) == 2 ? (DP % 64 == 0 ? DP + 40 : DP + 8) : DP + 4;
+};
+
+// A tile of N rows on its way from memory to LDS.  Columns past the head size are zeros, rows outside [first, last]
+// repeat a row inside: whatever lies in memory that no row of the workgroup sees is not read.
+template <typename T, int DP, int N>
+struct TileRegs {
+  static constexpr int kE = 16 / (int)sizeof(T);  // elements of a 16-byte chunk
+  static constexpr int kCPR = DP / kE;
+  static constexpr int kN = (N * kCPR + 255) / 256;
+  u32x4 r[kN];
+  template <typename ROW>
+  __device__ __forceinline__ void load(ROW row_pointer, int D, int t) {
+#pragma unroll
+    for (int n = 0; n < kN; n++) {
+      int const c = t + n * 256, row = c / kCPR, ch = c % kCPR;
+      r[n] = u32x4{0u, 0u, 0u, 0u};
+      if ((N * kCPR % 256 == 0 || c < N * kCPR) && ch * kE < D)
+        r[n] = *reinterpret_cast<u32x4 const *>(row_pointer(row) + ch * kE);
+    }
+  }
+  __device__ __forceinline__ void store(T *tile, int stride, int t) const {
+#pragma unroll
+    for (int n = 0; n < kN; n++) {
+      int const c = t + n * 256, row = c / kCPR, ch = c % kCPR;
+      if (N * kCPR % 256 == 0 || c < N * kCPR) *reinterpret_cast<u32x4 *>(tile + row * stride + ch * kE) = r[n];
+    }
+  }
+};
+
+// tanh(scale raw / cap).  bf16 kernels: 1 - 2 / (1 + 2^(cap_in raw)) on the hardware's exponential and reciprocal,
+// about 2^-22 off in absolute terms, which the cap multiplies to a few 1e-6 of a score, far below what bf16 scores carry.
+// fp32 kernels, whose matrix products take sixteen times as long, take the library's.
+template <typename T>
+__device__ __forceinline__ float cap_tanh(MaskedAttnParams const &p, float raw) {
+  if constexpr (sizeof(T) == 2) {
+    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * p.cap_in));
+  } else {
+    return tanhf(raw * p.inv_cap_scale);
+  }
+}
+
+// A wave's smallest and largest of an integer, scalar.
+__device__ __forceinline__ int wave_min_int(int v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_int(int v) { return -wave_min_int(-v); }
+
+// Writes 4 consecutive elements.
+__device__ __forceinline__ void store4(bf16 *p, float a, float b, float c, float d) {
+  *reinterpret_cast<u32x2 *>(p) = u32x2{pack_bf16x2(a, b), pack_bf16x2(c, d)};
+}
+__device__ __forceinline__ void store4(float *p, float a, float b, float c, float d) {
+  *reinterpret_cast<f32x4 *>(p) = f32x4{a, b, c, d};
+}
+
+}  // namespace ffk

@@ -1,0 +1,432 @@
+// Masked attention, backward: any head size, either type (see masked_attention.h for the mathematics and layouts).
+// Templates that masked_attention_bwd_*.hip instantiate, so that they compile side by side.
+//
+// Two kernels without atomics, both of which compute P again from the saved log-sum-exp.  The dQ kernel owns 32 RG rows
+// and runs over the keys in their ranges; it also leaves delta = rowsum(O dO) and, for every 32 rows, a summary of their
+// ranges in memory for the dK/dV kernel, which runs behind it.  That one owns 128 keys of one key head, 32 to a wave, and
+// runs over the rows of all query heads that read it, without the tiles of rows that see none of its keys.
+#pragma once
+#include "masked_attention.h"
+
+namespace ffk {
+
+template <typename T, int DP, int RG>
+struct MaskedDq {
+  static constexpr int kKW = 4 / RG;
+  static constexpr int kT = 32 * kKW;
+  static constexpr int kKS = TileStride<T, DP>::both, kVS = TileStride<T, DP>::row;
+  static constexpr int kTile = kT * (kKS + kVS) * (int)sizeof(T);
+  static constexpr int kBuffers = 2 * kTile <= 152 * 1024 ? 2 : 1;
+  static constexpr int kMerge = (kKW - 1) * RG * DP * 32 * 4;
+  static constexpr int kBytes = kBuffers * kTile > kMerge ? kBuffers * kTile : kMerge;
+  static_assert(kBytes <= 156 * 1024, "LDS of a CU");
+};
+
+template <typename T, int DP, int RG, bool EXTRA>
+__global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
+  using C = MaskedDq<T, DP, RG>;
+  constexpr int KW = C::kKW;
+  extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
+  __shared__ int window[2][4];
+  int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
+  int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  int const qw = wave / KW, kw = wave % KW;
+  int const nrb = (p.R + 32 * RG - 1) / (32 * RG);
+  int const hb = blockIdx.x % (p.KH * p.B);
+  int const rb = nrb - 1 - blockIdx.x / (p.KH * p.B);
+  int const kh = hb % p.KH, b = hb / p.KH;
+  int const row0 = rb * 32 * RG + qw * 32;
+  int const row = row0 + (lane & 31);
+  int qi, qg;
+  row_of(p, min(row, p.R - 1), qi, qg);
+  int const head = kh * p.G + qg;
+  int lo, hi;
+  row_range(p, b, qi, lo, hi);
+  if (row >= p.R) {
+    lo = 1 << 30;
+    hi = 0;
+  }
+  int const w_lo_min = wave_min_int(lo), w_hi_max = wave_max_int(hi), w_lo_max = wave_max_int(lo), w_hi_min = wave_min_int(hi);
+  if (lane == 0) {
+    window[0][wave] = w_lo_min;
+    window[1][wave] = w_hi_max;
+    if (kh == 0 && kw == 0 && row0 < p.R)
+      p.summary[(int64_t)b * ((p.R + 31) / 32) + row0 / 32] = RangeSummary{w_lo_min, w_hi_max, w_lo_max, w_hi_min};
+  }
+  __syncthreads();
+  int const lo_all = __builtin_amdgcn_readfirstlane(min(min(window[0][0], window[0][1]), min(window[0][2], window[0][3])));
+  int const hi_all = __builtin_amdgcn_readfirstlane(max(max(window[1][0], window[1][1]), max(window[1][2], window[1][3])));
+  int const ntiles = hi_all > lo_all ? (hi_all - lo_all + C::kT - 1) / C::kT : 0;
+
+  int64_t const o_at = (int64_t)b * p.o_bs + (int64_t)qi * p.o_ss + (int64_t)head * p.Dv;
+  T const *qp = static_cast<T const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * p.Dq;
+  T const *gp = static_cast<T const *>(p.d_o) + o_at;
+  T const *op = static_cast<T const *>(p.o) + o_at;
+  T const *kp = static_cast<T const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * p.Dq;
+  T const *vp = static_cast<T const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * p.Dv;
+  float const slope2 = EXTRA && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.0f;
+  int const position = p.q_offset + qi;
+
+  Frag<T> qf[DP / 16], gf[DP / 16];
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; kk++) {
+    qf[kk] = frag_row(qp, kk * 16 + h32 * 8, p.Dq);
+    gf[kk] = frag_row(gp, kk * 16 + h32 * 8, p.Dv);
+  }
+  // delta: a lane holds half of its row's columns (8 of every 16), lane ^ 32 the others
+  float delta = 0.0f;
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; kk++) {
+    Frag<T> const of = frag_row(op, kk * 16 + h32 * 8, p.Dv);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) delta += (float)of.v[e] * (float)gf[kk].v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) delta += of.a[e] * gf[kk].a[e] + of.b[e] * gf[kk].b[e];
+    }
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  int64_t const stat_at = ((int64_t)b * p.H + head) * p.Sq + qi;
+  float const lse = p.lse[stat_at];
+  if (h32 == 0 && kw == 0 && row < p.R) p.delta[stat_at] = delta;
+  float const lse2 = lse * kLog2e;
+
+  f32x16 dq[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) dq[i][r] = 0.0f;
+
+  auto k_tile = [&](int buf) { return reinterpret_cast<T *>(pool + buf * C::kTile); };
+  auto v_tile = [&](int buf) { return k_tile(buf) + C::kT * C::kKS; };
+  TileRegs<T, DP, C::kT> tk, tv;
+  auto fetch = [&](int kv0) {
+    tk.load([&](int r) { return kp + (int64_t)min(kv0 + r, hi_all - 1) * p.k_ss; }, p.Dq, t);
+    tv.load([&](int r) { return vp + (int64_t)min(kv0 + r, hi_all - 1) * p.v_ss; }, p.Dv, t);
+  };
+  auto stash = [&](int buf) {
+    tk.store(k_tile(buf), C::kKS, t);
+    tv.store(v_tile(buf), C::kVS, t);
+  };
+  int const koff = lane_k_off(C::kKS, lane), voff = lane_k_off(C::kVS, lane), toff = turn_off<T>(C::kKS, lane);
+  if (ntiles > 0) {
+    fetch(lo_all);
+    stash(0);
+  }
+  __syncthreads();
+  int cur = 0;
+  for (int it = 0; it < ntiles; it++) {
+    bool const more = it + 1 < ntiles;
+    if (more) fetch(lo_all + (it + 1) * C::kT);
+    int const kv0 = lo_all + it * C::kT + kw * 32;
+    if (kv0 < w_hi_max && kv0 + 32 > w_lo_min) {
+      T const *kt = k_tile(cur) + kw * 32 * C::kKS, *vt = v_tile(cur) + kw * 32 * C::kVS + voff;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        s[r] = 0.0f;
+        dp[r] = 0.0f;
+      }
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; kk++) {
+        mma(s, frag_lds(kt + koff + kk * 16), qf[kk]);
+        mma(dp, frag_lds(vt + kk * 16), gf[kk]);
+      }
+      float ds[16];
+      bool const whole = kv0 >= w_lo_max && kv0 + 32 <= w_hi_min;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        int const kv = kv0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
+        float x = s[r] * p.scale_log2, slope = p.scale;
+        if constexpr (EXTRA) {
+          if (p.cap_out != 0.0f) {
+            float const tanh = cap_tanh<T>(p, s[r]);
+            x = p.cap_out * tanh;
+            slope *= 1.0f - tanh * tanh;
+          }
+          x -= slope2 * (float)abs(position - kv);
+        }
+        float const e = __builtin_amdgcn_exp2f(x - lse2);
+        ds[r] = e * (dp[r] - delta) * slope;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          int const kv = kv0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
+          if (kv < lo || kv >= hi) ds[r] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; s2++) {
+        Frag<T> const df = frag_acc(ds + 8 * s2, kp);
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) mma(dq[i], frag_turned(kt + toff, C::kKS, s2, i * 32), df);
+      }
+    }
+    if constexpr (C::kBuffers == 2) {
+      if (more) stash(cur ^ 1);
+      __syncthreads();
+      cur ^= 1;
+    } else {
+      __syncthreads();
+      if (more) stash(0);
+      __syncthreads();
+    }
+  }
+
+  if constexpr (KW > 1) {
+    float *const area = reinterpret_cast<float *>(pool);
+    __syncthreads();
+    if (kw > 0) {
+      float *to = area + ((kw - 1) * RG + qw) * DP * 32;
+#pragma unroll
+      for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) to[(i * 16 + r) * 64 + lane] = dq[i][r];
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int w = 0; w < KW - 1; w++) {
+      float const *from = area + (w * RG + qw) * DP * 32;
+#pragma unroll
+      for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) dq[i][r] += from[(i * 16 + r) * 64 + lane];
+    }
+  }
+  if (row >= p.R) return;
+  T *dqp = static_cast<T *>(p.dq) + (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * p.Dq;
+#pragma unroll
+  for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      int const d = i * 32 + 8 * g + 4 * h32;
+      if (d < p.Dq) store4(dqp + d, dq[i][4 * g], dq[i][4 * g + 1], dq[i][4 * g + 2], dq[i][4 * g + 3]);
+    }
+}
+
+// What a row brings along into LDS: its range, statistics, slope and position.
+struct RowStats {
+  float lse2[32], delta[32], slope2[32];
+  int lo[32], hi[32], position[32];
+};
+
+template <typename T, int DP>
+struct MaskedDkdv {
+  static constexpr int kS = TileStride<T, DP>::both;
+  static constexpr int kTile = 2 * 32 * kS * (int)sizeof(T);  // Q and dO
+  static constexpr int kBytes = 2 * kTile;
+  static_assert(kBytes <= 150 * 1024, "LDS of a CU");
+};
+
+// WHAT: bit 0 dV, bit 1 dK.  Both from one launch, but where the owned K and V rows and both accumulators are more than
+// a wave's registers.
+template <typename T, int DP, int WHAT, bool EXTRA>
+__global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
+  using C = MaskedDkdv<T, DP>;
+  constexpr bool kDv = (WHAT & 1) != 0, kDk = (WHAT & 2) != 0;
+  extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
+  __shared__ RowStats stats[2];
+  int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
+  int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  int const hb = blockIdx.x % (p.KH * p.B);
+  int const kh = hb % p.KH, b = hb / p.KH;
+  int const kv0 = (int)(blockIdx.x / (p.KH * p.B)) * 128;  // under a causal mask the first keys are seen by most rows
+  int const wkv0 = kv0 + wave * 32, kv = wkv0 + (lane & 31);
+  int const nsum = (p.R + 31) / 32;
+  RangeSummary const *sums = p.summary + (int64_t)b * nsum;
+
+  T const *kp = static_cast<T const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)min(kv, p.Skv - 1) * p.k_ss + (int64_t)kh * p.Dq;
+  T const *vp = static_cast<T const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)min(kv, p.Skv - 1) * p.v_ss + (int64_t)kh * p.Dv;
+  T const *qp = static_cast<T const *>(p.q) + (int64_t)b * p.q_bs;
+  T const *gp = static_cast<T const *>(p.d_o) + (int64_t)b * p.o_bs;
+
+  Frag<T> kf[DP / 16], vf[kDk ? DP / 16 : 1];
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; kk++) {
+    kf[kk] = frag_row(kp, kk * 16 + h32 * 8, p.Dq);
+    if constexpr (kDk) vf[kk] = frag_row(vp, kk * 16 + h32 * 8, p.Dv);
+  }
+  f32x16 dk[kDk ? DP / 32 : 1], dv[kDv ? DP / 32 : 1];
+#pragma unroll
+  for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      if constexpr (kDk) dk[i][r] = 0.0f;
+      if constexpr (kDv) dv[i][r] = 0.0f;
+    }
+
+  auto q_tile = [&](int buf) { return reinterpret_cast<T *>(pool + buf * C::kTile); };
+  auto g_tile = [&](int buf) { return q_tile(buf) + 32 * C::kS; };
+  // the next tile at or behind `tile` in which a row sees a key of this workgroup
+  auto next = [&](int tile) {
+    while (tile < nsum) {
+      RangeSummary const s = sums[tile];
+      if (s.lo_min < kv0 + 128 && s.hi_max > kv0) break;
+      tile++;
+    }
+    return tile;
+  };
+  using Regs = TileRegs<T, DP, 32>;
+  Regs tq, tg;
+  int2 seen[Regs::kN];  // the ranges of this thread's rows: one that sees none of the keys is a row of zeros in LDS
+  float st_lse2, st_delta, st_slope2;
+  int st_lo, st_hi, st_position;
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int n = 0; n < Regs::kN; n++) {
+      int const r = tile * 32 + (t + n * 256) / Regs::kCPR;
+      int i, g;
+      row_of(p, min(r, p.R - 1), i, g);
+      row_range(p, b, i, seen[n].x, seen[n].y);
+      if (r >= p.R) seen[n].y = 0;
+    }
+    auto offset = [&](int r, int64_t seq_stride, int D) {
+      int i, g;
+      row_of(p, min(tile * 32 + r, p.R - 1), i, g);
+      return (int64_t)i * seq_stride + (int64_t)(kh * p.G + g) * D;
+    };
+    tq.load([&](int r) { return qp + offset(r, p.q_ss, p.Dq); }, p.Dq, t);
+    tg.load([&](int r) { return gp + offset(r, p.o_ss, p.Dv); }, p.Dv, t);
+    if (t < 32) {
+      int const r = tile * 32 + t;
+      int i, g;
+      row_of(p, min(r, p.R - 1), i, g);
+      int const head = kh * p.G + g;
+      row_range(p, b, i, st_lo, st_hi);
+      if (r >= p.R) st_hi = 0;
+      st_lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + i] * kLog2e;
+      st_delta = p.delta[((int64_t)b * p.H + head) * p.Sq + i];
+      st_slope2 = EXTRA && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.0f;
+      st_position = p.q_offset + i;
+    }
+  };
+  auto stash = [&](int buf) {
+#pragma unroll
+    for (int n = 0; n < Regs::kN; n++) {
+      if (!(seen[n].x < kv0 + 128 && seen[n].y > kv0)) {
+        tq.r[n] = u32x4{0u, 0u, 0u, 0u};
+        tg.r[n] = u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+    tq.store(q_tile(buf), C::kS, t);
+    tg.store(g_tile(buf), C::kS, t);
+    if (t < 32) {
+      stats[buf].lse2[t] = st_lse2;
+      stats[buf].delta[t] = st_delta;
+      stats[buf].slope2[t] = st_slope2;
+      stats[buf].lo[t] = st_lo;
+      stats[buf].hi[t] = st_hi;
+      stats[buf].position[t] = st_position;
+    }
+  };
+  int const roff = lane_k_off(C::kS, lane), toff = turn_off<T>(C::kS, lane);
+  int tile = next(0);
+  if (tile < nsum) {
+    fetch(tile);
+    stash(0);
+  }
+  __syncthreads();
+  int cur = 0;
+  while (tile < nsum) {
+    int const after = next(tile + 1);
+    if (after < nsum) fetch(after);
+    RangeSummary const sum = sums[tile];
+    if (wkv0 < p.Skv && sum.lo_min < wkv0 + 32 && sum.hi_max > wkv0) {
+      T const *qt = q_tile(cur), *gt = g_tile(cur);
+      RowStats const &rs = stats[cur];
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        s[r] = 0.0f;
+        dp[r] = 0.0f;
+      }
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; kk++) {
+        mma(s, frag_lds(qt + roff + kk * 16), kf[kk]);
+        if constexpr (kDk) mma(dp, frag_lds(gt + roff + kk * 16), vf[kk]);
+      }
+      float pv[16], ds[16];
+      bool const whole = wkv0 >= sum.lo_max && wkv0 + 32 <= sum.hi_min;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        int const at = 8 * (r >> 2) + 4 * h32 + (r & 3);
+        float x = s[r] * p.scale_log2, slope = p.scale;
+        if constexpr (EXTRA) {
+          if (p.cap_out != 0.0f) {
+            float const tanh = cap_tanh<T>(p, s[r]);
+            x = p.cap_out * tanh;
+            slope *= 1.0f - tanh * tanh;
+          }
+          x -= rs.slope2[at] * (float)abs(rs.position[at] - kv);
+        }
+        pv[r] = __builtin_amdgcn_exp2f(x - rs.lse2[at]);
+        if constexpr (kDk) ds[r] = pv[r] * (dp[r] - rs.delta[at]) * slope;
+        if (!whole && (kv < rs.lo[at] || kv >= rs.hi[at])) {
+          pv[r] = 0.0f;
+          if constexpr (kDk) ds[r] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; s2++) {
+        if constexpr (kDv) {
+          Frag<T> const pf = frag_acc(pv + 8 * s2, kp);
+#pragma unroll
+          for (int i = 0; i < DP / 32; i++) mma(dv[i], frag_turned(gt + toff, C::kS, s2, i * 32), pf);
+        }
+        if constexpr (kDk) {
+          Frag<T> const df = frag_acc(ds + 8 * s2, kp);
+#pragma unroll
+          for (int i = 0; i < DP / 32; i++) mma(dk[i], frag_turned(qt + toff, C::kS, s2, i * 32), df);
+        }
+      }
+    }
+    if (after < nsum) stash(cur ^ 1);
+    __syncthreads();
+    cur ^= 1;
+    tile = after;
+  }
+  if (kv >= p.Skv) return;
+#pragma unroll
+  for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      int const d = i * 32 + 8 * g + 4 * h32;
+      if constexpr (kDk) {
+        T *out = static_cast<T *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kv * p.k_ss + (int64_t)kh * p.Dq;
+        if (d < p.Dq) store4(out + d, dk[i][4 * g], dk[i][4 * g + 1], dk[i][4 * g + 2], dk[i][4 * g + 3]);
+      }
+      if constexpr (kDv) {
+        T *out = static_cast<T *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kv * p.v_ss + (int64_t)kh * p.Dv;
+        if (d < p.Dv) store4(out + d, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
+      }
+    }
+}
+
+template <typename T, int DP, int RG, bool EXTRA>
+static hipError_t masked_dq_launch(hipStream_t st, MaskedAttnParams const &p) {
+  static LdsOptIn opt_in;
+  using C = MaskedDq<T, DP, RG>;
+  auto kernel = &masked_dq_kernel<T, DP, RG, EXTRA>;
+  hipError_t e = opt_in.ensure(reinterpret_cast<void const *>(kernel), C::kBytes);
+  if (e != hipSuccess) return e;
+  int64_t const grid = ceil_div(p.R, 32 * RG) * p.KH * p.B;
+  kernel<<<dim3((unsigned)grid), 256, C::kBytes, st>>>(p);
+  return hipGetLastError();
+}
+
+template <typename T, int DP, int WHAT, bool EXTRA>
+static hipError_t masked_dkdv_launch(hipStream_t st, MaskedAttnParams const &p) {
+  static LdsOptIn opt_in;
+  using C = MaskedDkdv<T, DP>;
+  auto kernel = &masked_dkdv_kernel<T, DP, WHAT, EXTRA>;
+  hipError_t e = opt_in.ensure(reinterpret_cast<void const *>(kernel), C::kBytes);
+  if (e != hipSuccess) return e;
+  int64_t const grid = ceil_div(p.Skv, 128) * p.KH * p.B;
+  kernel<<<dim3((unsigned)grid), 256, C::kBytes, st>>>(p);
+  return hipGetLastError();
+}
+
+}  // namespace ffk

@@ -181,7 +181,11 @@ PyMethodDef methods[] = {
     ENTRY(ffk_linear_dropout_add_forward), ENTRY(ffk_linear_backward_dropout_gelu),
     ENTRY(ffk_linear_backward_dropout_gelu_bias_grad), ENTRY(ffk_embedding_forward), ENTRY(ffk_embedding_backward),
     ENTRY(ffk_embedding_backward_workspace_bytes), ENTRY(ffk_embedding_backward_typed), ENTRY(ffk_attention_forward),
-    ENTRY(ffk_attention_backward), ENTRY(ffk_mha_reserve_bytes), ENTRY(ffk_mha_forward), ENTRY(ffk_mha_backward),
+    ENTRY(ffk_attention_backward), ENTRY(ffk_attention_key_ranges), ENTRY(ffk_masked_attention_forward),
+    ENTRY(ffk_masked_attention_forward_workspace_bytes), ENTRY(ffk_masked_attention_backward),
+    ENTRY(ffk_masked_attention_backward_workspace_bytes), ENTRY(ffk_rotary_forward), ENTRY(ffk_rotary_backward),
+    ENTRY(ffk_grad_norm_workspace_bytes), ENTRY_HOST_INTS(ffk_global_grad_norm), ENTRY_HOST_INTS(ffk_clip_grad_norm),
+    ENTRY(ffk_mha_reserve_bytes), ENTRY(ffk_mha_forward), ENTRY(ffk_mha_backward),
     ENTRY(ffk_mha_backward_workspace_bytes), ENTRY(ffk_mha_backward_with_workspace),
     ENTRY(ffk_encoder_layer_workspace_bytes), ENTRY(ffk_encoder_layer_forward), ENTRY(ffk_encoder_layer_backward),
     ENTRY(ffk_sgd_update), ENTRY(ffk_adam_update), ENTRY(ffk_sparse_categorical_crossentropy_loss_backward),

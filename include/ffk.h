@@ -617,6 +617,126 @@ int ffk_attention_backward(ffk_stream_t stream, int dtype,
                            void *dq, void *dk, void *dv);
 
 /* ------------------------------------------------------------------------ */
+/* Masked attention: the attention core for packed and padded batches, with
+ * capped or distance-biased scores and key heads that query heads share.  No
+ * counterpart in the reference, whose attention has neither masks nor a bias
+ * (attention_kernels.cu:73-92).
+ *
+ * ffk_attention_key_ranges: the masks' form, one launch for all layers that
+ *   share a batch.  key_ranges [batch, seq_q, 2] int32: query row i of a batch
+ *   entry sees the keys  lo <= j < hi; (0, 0) is a row that sees none.  The row
+ *   stands at position query_offset + i among the keys.
+ *   document_starts [batch, num_documents + 1] int32, not descending, or NULL
+ *     (one document, all keys): document d holds the positions starts[d] <= p <
+ *     starts[d+1]; a position sees its document only, and a position before the
+ *     first or behind the last document sees nothing.  Documents may be empty.
+ *   causal != 0: a position sees up to itself, and, with prefix_lengths
+ *     [batch, num_documents] (or [batch, 1] without document_starts) int32, the
+ *     first prefix_lengths keys of its document whatever its position (a prefix
+ *     longer than its document is the document).  prefix_lengths without causal
+ *     is FFK_ERR_INVALID.  Ranges of any other making do as well.
+ *
+ * ffk_masked_attention_forward / _backward: tensors, layouts and strides as in
+ *   ffk_attention_forward / _backward, but that k and v (and dk, dv) have
+ *   kv_heads heads, of which key head h / (heads / kv_heads) is the one that
+ *   query head h reads.  Scores of query row i at position p_i = query_offset + i:
+ *     x = scale * q_i . k_j;  s = score_cap * tanh(x / score_cap)  (score_cap 0: x)
+ *     s -= distance_slopes[h] * |p_i - j|        (distance_slopes [heads] fp32 or NULL)
+ *   over the keys of its range (key_ranges NULL: all keys), of which causal != 0
+ *   leaves those with j <= p_i.  A row that sees no key has o = 0, lse = -inf and
+ *   gives and takes no gradient.  What lies in k and v outside of every range of
+ *   a workgroup's rows is not read; next to it, a key that is NaN or infinite
+ *   must be one that no row sees only if it is more than 127 keys away from all
+ *   that are seen, since a masked probability is 0 and 0 times it is not.
+ *   Ranges are cut to [0, seq_kv].  distance_slopes and key_ranges have no gradient.
+ *   dtype FFK_BF16 (head sizes multiples of 8 up to 256, strides multiples of 8
+ *   elements) or FFK_FLOAT (multiples of 4); 16-byte aligned tensors, key_ranges
+ *   8-byte aligned.  dq, dk, dv have the strides of q, k, v and are overwritten;
+ *   lse may be NULL in the forward.
+ *   workspace of the forward: ffk_masked_attention_forward_workspace_bytes(...)
+ *   bytes (0: none), 16-byte aligned; without it few rows over long keys are not
+ *   split over workgroups, which costs time and gives the sums another order, so
+ *   other last bits.  workspace of the backward: required (FFK_ERR_WORKSPACE).
+ *   Both are scratch: calls that overlap need one each.  No atomics: the same
+ *   call gives the same bits.                                                  */
+/* ------------------------------------------------------------------------ */
+int ffk_attention_key_ranges(ffk_stream_t stream, int64_t batch, int64_t seq_q,
+                             int64_t seq_kv, int64_t query_offset, int causal,
+                             int32_t const *document_starts,
+                             int64_t num_documents,
+                             int32_t const *prefix_lengths, int32_t *key_ranges);
+typedef struct {
+  int64_t batch, heads, kv_heads, seq_q, seq_kv, head_dim;
+  int64_t v_head_dim; /* head size of v, o (and their gradients); 0 = head_dim */
+  int64_t q_batch_stride, q_seq_stride;
+  int64_t k_batch_stride, k_seq_stride;
+  int64_t v_batch_stride, v_seq_stride;
+  int64_t o_batch_stride, o_seq_stride;
+  int64_t query_offset; /* position of query row 0 among the keys */
+  float scale;
+  float score_cap; /* 0: none */
+  int causal;
+} ffk_masked_attention_desc_t;
+
+size_t ffk_masked_attention_forward_workspace_bytes(
+    ffk_masked_attention_desc_t const *desc, int dtype);
+int ffk_masked_attention_forward(ffk_stream_t stream, int dtype,
+                                 ffk_masked_attention_desc_t const *desc,
+                                 void const *q, void const *k, void const *v,
+                                 int32_t const *key_ranges,
+                                 float const *distance_slopes, void *o,
+                                 float *lse, void *workspace,
+                                 size_t workspace_bytes);
+size_t ffk_masked_attention_backward_workspace_bytes(
+    ffk_masked_attention_desc_t const *desc, int dtype);
+int ffk_masked_attention_backward(ffk_stream_t stream, int dtype,
+                                  ffk_masked_attention_desc_t const *desc,
+                                  void const *q, void const *k, void const *v,
+                                  int32_t const *key_ranges,
+                                  float const *distance_slopes, void const *o,
+                                  void const *d_o, float const *lse, void *dq,
+                                  void *dk, void *dv, void *workspace,
+                                  size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------ */
+/* Rotary positions with one to four axes (a text's one, an image's height and
+ * width, a video's time as well) on q [batch, seq, q_heads, head_dim] and k
+ * [batch, seq, k_heads, head_dim] (k_heads 0: q alone, k and k_out NULL).  No
+ * counterpart in the reference, whose models have no positions.
+ *   n = sum of sections pairs of a head's columns turn: j and j + n (interleaved
+ *   0), or 2j and 2j + 1 (interleaved 1); columns from 2n on pass through.
+ *   sections[a] pairs, in order, belong to axis a; pair j of a token turns by
+ *     theta = positions[axis of j][token] * frequencies[j]
+ *     (a, b) -> (a cos theta - b sin theta, a sin theta + b cos theta)
+ *   positions [num_axes, batch, seq] int32, frequencies [n] fp32 in radians a
+ *   position (any scaling of them is the caller's); the product is taken in 64
+ *   bits, so far positions are as exact as near ones.
+ * backward: the gradient of q and k, the turn by -theta.
+ * FLOAT or BF16 (fp32 arithmetic, one rounding).  Token (b, s) of a tensor
+ * begins at b * batch_stride + s * seq_stride elements, its heads follow each
+ * other (a fused QKV buffer is read in place).  q_out / k_out may be q / k, with
+ * the same strides, or lie apart from them; rows of any alignment, whole 16
+ * bytes are fastest.                                                          */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  int64_t batch, seq, q_heads, k_heads, head_dim;
+  int64_t q_batch_stride, q_seq_stride, k_batch_stride, k_seq_stride;
+  int64_t q_out_batch_stride, q_out_seq_stride, k_out_batch_stride, k_out_seq_stride;
+  int64_t num_axes;
+  int64_t sections[4];
+  int64_t interleaved;
+} ffk_rotary_desc_t;
+
+int ffk_rotary_forward(ffk_stream_t stream, int dtype,
+                       ffk_rotary_desc_t const *desc, void const *q,
+                       void const *k, int32_t const *positions,
+                       float const *frequencies, void *q_out, void *k_out);
+int ffk_rotary_backward(ffk_stream_t stream, int dtype,
+                        ffk_rotary_desc_t const *desc, void const *q_out_grad,
+                        void const *k_out_grad, int32_t const *positions,
+                        float const *frequencies, void *q_grad, void *k_grad);
+
+/* ------------------------------------------------------------------------ */
 /* MultiHeadAttention -- Kernels::MultiHeadAttention::gpu_forward_kernel /
  * gpu_backward_kernel (attention_kernels_gpu.h:27-45; CUDA body
  * lib/kernels/src/cuda/ops/attention_kernels.cu:215-303).
@@ -785,6 +905,31 @@ int ffk_adam_update(ffk_stream_t stream, int grad_dtype, float alpha_t,
                     void const *weight_grad, int64_t num_elements,
                     int num_replicas, float *weight, float *adam_v,
                     float *adam_m, void *weight_lowp);
+
+/* ------------------------------------------------------------------------ */
+/* The norm over all gradients of a step, and the gradients held to a largest
+ * norm, for the updates above.  No counterpart in the reference, which updates
+ * with gradients as they are.
+ *   ffk_global_grad_norm: *norm (fp32, device) = sqrt(sum of all squares)
+ *   ffk_clip_grad_norm:   clipped[i] = grads[i] * min(1, max_norm / (norm + 1e-6)),
+ *     and *norm (may be NULL) the norm before.  clipped[i] may be grads[i] (which
+ *     is then left alone where the factor is 1) or lie apart from all grads.
+ * dtypes (FFK_FLOAT / FFK_BF16), grads, clipped, elems: host arrays of
+ * num_tensors entries; tensors of any size, 0 among them, aligned to their
+ * elements.  Squares are summed in 64 bits in a fixed order.  A norm that is
+ * infinite or NaN scales as the formula says (factor 0 or NaN).
+ * workspace: ffk_grad_norm_workspace_bytes(num_tensors) bytes, 8-byte aligned
+ * (FFK_ERR_WORKSPACE); scratch, calls that overlap need one each.             */
+/* ------------------------------------------------------------------------ */
+size_t ffk_grad_norm_workspace_bytes(int num_tensors);
+int ffk_global_grad_norm(ffk_stream_t stream, int const *dtypes,
+                         void const *const *grads, int64_t const *elems,
+                         int num_tensors, float *norm, void *workspace,
+                         size_t workspace_bytes);
+int ffk_clip_grad_norm(ffk_stream_t stream, int const *dtypes,
+                       void const *const *grads, void *const *clipped,
+                       int64_t const *elems, int num_tensors, float max_norm,
+                       float *norm, void *workspace, size_t workspace_bytes);
 
 /* ------------------------------------------------------------------------ */
 /* Loss-function backward -- *_loss_backward_kernel
