@@ -27,17 +27,22 @@ struct RangeSummary {
   int lo_max, hi_min;  // every row sees all of [lo_max, hi_min)
 };
 
+// What the dQ kernels leave in memory of every row for the dK/dV kernels: arrays of padded_rows entries, one set for each
+// (batch, key head), which a tile's rows are read from in order.  Rows behind the last one see nothing.
+enum { kRowLse2 = 0, kRowDelta = 1, kRowLo = 2, kRowHi = 3, kRowSlope2 = 4, kRowPosition = 5, kRowFields = 6 };
+
 struct MaskedAttnParams {
   void const *q, *k, *v;
   void *o;
   void const *d_o;
   float *lse;
-  float *delta;
+  float *rows;  // [B, KH, kRowFields, padded_rows], integers by their bits
   void *dq, *dk, *dv;
   int const *ranges;    // [B, Sq, 2] or NULL
   float const *slopes;  // [H] or NULL
   RangeSummary *summary;  // [B, ceil(Sq G / 32)]
   int B, H, KH, G, Sq, Skv, Dq, Dv, R;  // R = Sq G rows of a key head
+  int padded_rows;                      // R up to whole tiles of 64
   int64_t q_bs, q_ss, k_bs, k_ss, v_bs, v_ss, o_bs, o_ss;
   int q_offset;
   float scale, scale_log2;
@@ -71,6 +76,25 @@ __device__ __forceinline__ void row_range(MaskedAttnParams const &p, int b, int 
     lo = 1 << 30;
     hi = 0;
   }
+}
+
+__device__ __forceinline__ void write_row(MaskedAttnParams const &p, int b, int kh, int row, float lse2, float delta, int lo, int hi,
+                                          float slope2, int position) {
+  if (row >= p.padded_rows) return;
+  float *rows = p.rows + (int64_t)(b * p.KH + kh) * kRowFields * p.padded_rows + row;
+  int64_t const n = p.padded_rows;
+  rows[kRowLse2 * n] = lse2;
+  rows[kRowDelta * n] = delta;
+  rows[kRowLo * n] = __int_as_float(lo);
+  rows[kRowHi * n] = __int_as_float(hi);
+  if (p.slopes != nullptr) {
+    rows[kRowSlope2 * n] = slope2;
+    rows[kRowPosition * n] = __int_as_float(position);
+  }
+}
+// the rows from `first` on that no workgroup of the dQ kernel owns
+__device__ __forceinline__ void write_padding(MaskedAttnParams const &p, int b, int kh, int first, int t) {
+  for (int row = first + t; row < p.padded_rows; row += 256) write_row(p, b, kh, row, 0.0f, 0.0f, 1 << 30, 0, 0.0f, 0);
 }
 
 // ---- one step of 16 of a product, for either type -------------------------

@@ -6,12 +6,16 @@
 namespace ffk {
 
 // instances: masked_attention_{fwd,dq,dkdv}_{bf16,f32}.hip
-hipError_t masked_attention_fwd_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra, int groups);
-hipError_t masked_attention_fwd_f32(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra, int groups);
-hipError_t masked_attention_dq_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra, int groups);
-hipError_t masked_attention_dq_f32(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra, int groups);
-hipError_t masked_attention_dkdv_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra);
-hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra);
+hipError_t masked_attention_fwd_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
+hipError_t masked_attention_fwd_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
+hipError_t masked_attention_dq_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
+hipError_t masked_attention_dq_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
+hipError_t masked_attention_dkdv_bf16(hipStream_t st, MaskedAttnParams const &p, int padded);
+hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded);
+// bf16, head sizes 64 and 128: masked_attention_wide_{fwd,dq,dkdv}.hip
+hipError_t masked_attention_fwd_wide(hipStream_t st, MaskedAttnParams const &p);
+hipError_t masked_attention_dq_wide(hipStream_t st, MaskedAttnParams const &p);
+hipError_t masked_attention_dkdv_wide(hipStream_t st, MaskedAttnParams const &p);
 
 // --------------------------------------------------------------------------
 // key ranges
@@ -180,14 +184,33 @@ static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, void con
     p.inv_cap_scale = d->scale / d->score_cap;
   }
   p.causal = d->causal != 0;
+  p.padded_rows = (p.R + 63) / 64 * 64;
   p.group = make_fast_div((uint32_t)p.G);
   p.splits = 1;
   return p;
 }
 
-static size_t delta_bytes(ffk_masked_attention_desc_t const *d) {
-  size_t const n = (size_t)d->batch * d->heads * d->seq_q * sizeof(float);
-  return (n + 255) / 256 * 256;
+// The backward's scratch: what the dQ kernels leave of the rows, and the summaries of their ranges.
+static size_t row_bytes(ffk_masked_attention_desc_t const *d) {
+  return (size_t)d->batch * d->kv_heads * kRowFields * (size_t)(ceil_div(rows_of(d), 64) * 64) * sizeof(float);
+}
+static size_t backward_bytes(ffk_masked_attention_desc_t const *d) {
+  return row_bytes(d) + (size_t)d->batch * ceil_div(rows_of(d), 32) * sizeof(RangeSummary);
+}
+
+// The kernels of masked_attention_wide_*.hip: bf16, one head size of 64 or 128, rows that 32-bit byte offsets reach.
+static bool wide_kernels(ffk_masked_attention_desc_t const *d, int dtype) {
+  int64_t const lim = (int64_t)1 << 32;
+  return dtype == FFK_BF16 && (d->head_dim == 64 || d->head_dim == 128) && (d->v_head_dim == 0 || d->v_head_dim == d->head_dim) &&
+         d->seq_q * d->q_seq_stride * 2 < lim && d->seq_q * d->o_seq_stride * 2 < lim;
+}
+
+// 64 rows to a wave, 256 to a workgroup, one workgroup on a CU: where every CU has one and keys are long.
+static bool wide_forward(ffk_masked_attention_desc_t const *d, int dtype) {
+  // (its direct loads reach a tile of 64 keys with 32-bit byte offsets)
+  if (!wide_kernels(d, dtype) || d->k_seq_stride >= (1 << 24) || d->v_seq_stride >= (1 << 24)) return false;
+  int const variant = option(FFK_OPTION_ATTENTION_VARIANT);
+  return variant == 2 || (variant == 0 && d->seq_kv >= 1024 && ceil_div(rows_of(d), 256) * d->kv_heads * d->batch >= kNumCU);
 }
 
 }  // namespace ffk
@@ -238,9 +261,12 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = p.part_o + (int64_t)splits * p.B * p.KH * p.R * p.Dv;
   }
-  bool const extra = d->score_cap != 0.0f || distance_slopes != nullptr;
+  if (wide_forward(d, dtype)) {
+    FFK_HIP(masked_attention_fwd_wide(st, p));
+    return FFK_OK;
+  }
   auto const launch = dtype == FFK_BF16 ? masked_attention_fwd_bf16 : masked_attention_fwd_f32;
-  FFK_HIP(launch(st, p, padded_head(d), extra, row_groups(d, dtype)));
+  FFK_HIP(launch(st, p, padded_head(d), row_groups(d, dtype)));
   if (p.splits > 1) {
     dim3 const grid((unsigned)ceil_div((int64_t)p.B * p.KH * p.R, 4));
     if (dtype == FFK_BF16) masked_merge_kernel<bf16><<<grid, 256, 0, st>>>(p);
@@ -252,7 +278,7 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
 
 extern "C" size_t ffk_masked_attention_backward_workspace_bytes(ffk_masked_attention_desc_t const *d, int dtype) {
   if (check("masked_attention_backward", dtype, d) != FFK_OK) return 0;
-  return delta_bytes(d) + (size_t)d->batch * ceil_div(rows_of(d), 32) * sizeof(RangeSummary);
+  return backward_bytes(d);
 }
 
 extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk_masked_attention_desc_t const *d, void const *q,
@@ -265,7 +291,7 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
   FFK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(d_o) && aligned16(dq) && aligned16(dk) && aligned16(dv),
               "masked_attention_backward: tensors must be 16-byte aligned");
   FFK_REQUIRE(reinterpret_cast<uintptr_t>(key_ranges) % 8 == 0, "masked_attention_backward: key_ranges must be 8-byte aligned");
-  size_t const need = delta_bytes(d) + (size_t)d->batch * ceil_div(rows_of(d), 32) * sizeof(RangeSummary);
+  size_t const need = backward_bytes(d);
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need) {
     return fail(FFK_ERR_WORKSPACE, "masked_attention_backward: workspace must hold %zu bytes, 16-byte aligned (%zu given)", need,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
@@ -277,14 +303,16 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
   p.dq = dq;
   p.dk = dk;
   p.dv = dv;
-  p.delta = static_cast<float *>(workspace);
-  p.summary = reinterpret_cast<RangeSummary *>(static_cast<uint8_t *>(workspace) + delta_bytes(d));
+  p.rows = static_cast<float *>(workspace);
+  p.summary = reinterpret_cast<RangeSummary *>(static_cast<uint8_t *>(workspace) + row_bytes(d));
   hipStream_t const st = as_stream(stream);
-  bool const extra = d->score_cap != 0.0f || distance_slopes != nullptr;
   int const padded = padded_head(d);
   auto const launch_dq = dtype == FFK_BF16 ? masked_attention_dq_bf16 : masked_attention_dq_f32;
   auto const launch_dkdv = dtype == FFK_BF16 ? masked_attention_dkdv_bf16 : masked_attention_dkdv_f32;
-  FFK_HIP(launch_dq(st, p, padded, extra, row_groups(d, dtype)));
-  FFK_HIP(launch_dkdv(st, p, padded, extra));
+  int const groups = row_groups(d, dtype);
+  if (groups == 4 && wide_kernels(d, dtype)) FFK_HIP(masked_attention_dq_wide(st, p));
+  else FFK_HIP(launch_dq(st, p, padded, groups));
+  if (wide_kernels(d, dtype)) FFK_HIP(masked_attention_dkdv_wide(st, p));
+  else FFK_HIP(launch_dkdv(st, p, padded));
   return FFK_OK;
 }

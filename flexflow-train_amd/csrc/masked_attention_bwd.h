@@ -22,10 +22,11 @@ struct MaskedDq {
   static_assert(kBytes <= 156 * 1024, "LDS of a CU");
 };
 
-template <typename T, int DP, int RG, bool EXTRA>
+template <typename T, int DP, int RG, int EXTRA>
 __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
   using C = MaskedDq<T, DP, RG>;
   constexpr int KW = C::kKW;
+  constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ int window[2][4];
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
   T const *op = static_cast<T const *>(p.o) + o_at;
   T const *kp = static_cast<T const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * p.Dq;
   T const *vp = static_cast<T const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * p.Dv;
-  float const slope2 = EXTRA && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.0f;
+  float const slope2 = kBias ? p.slopes[head] * kLog2e : 0.0f;
   int const position = p.q_offset + qi;
 
   Frag<T> qf[DP / 16], gf[DP / 16];
@@ -87,10 +88,9 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
     }
   }
   delta += __shfl_xor(delta, 32, 64);
-  int64_t const stat_at = ((int64_t)b * p.H + head) * p.Sq + qi;
-  float const lse = p.lse[stat_at];
-  if (h32 == 0 && kw == 0 && row < p.R) p.delta[stat_at] = delta;
-  float const lse2 = lse * kLog2e;
+  float const lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + qi] * kLog2e;
+  if (h32 == 0 && kw == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope2, position);
+  if (rb == nrb - 1) write_padding(p, b, kh, nrb * 32 * RG, t);
 
   f32x16 dq[DP / 32];
 #pragma unroll
@@ -139,14 +139,12 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
       for (int r = 0; r < 16; r++) {
         int const kv = kv0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
         float x = s[r] * p.scale_log2, slope = p.scale;
-        if constexpr (EXTRA) {
-          if (p.cap_out != 0.0f) {
-            float const tanh = cap_tanh<T>(p, s[r]);
-            x = p.cap_out * tanh;
-            slope *= 1.0f - tanh * tanh;
-          }
-          x -= slope2 * (float)abs(position - kv);
+        if constexpr (kCap) {
+          float const tanh = cap_tanh<T>(p, s[r]);
+          x = p.cap_out * tanh;
+          slope *= 1.0f - tanh * tanh;
         }
+        if constexpr (kBias) x = __builtin_fmaf(-slope2, (float)abs(position - kv), x);
         float const e = __builtin_amdgcn_exp2f(x - lse2);
         ds[r] = e * (dp[r] - delta) * slope;
       }
@@ -223,10 +221,11 @@ struct MaskedDkdv {
 
 // WHAT: bit 0 dV, bit 1 dK.  Both from one launch, but where the owned K and V rows and both accumulators are more than
 // a wave's registers.
-template <typename T, int DP, int WHAT, bool EXTRA>
+template <typename T, int DP, int WHAT, int EXTRA>
 __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
   using C = MaskedDkdv<T, DP>;
   constexpr bool kDv = (WHAT & 1) != 0, kDk = (WHAT & 2) != 0;
+  constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ RowStats stats[2];
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
@@ -297,9 +296,10 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
       int const head = kh * p.G + g;
       row_range(p, b, i, st_lo, st_hi);
       if (r >= p.R) st_hi = 0;
-      st_lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + i] * kLog2e;
-      st_delta = p.delta[((int64_t)b * p.H + head) * p.Sq + i];
-      st_slope2 = EXTRA && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.0f;
+      float const *rows = p.rows + (int64_t)hb * kRowFields * p.padded_rows + r;
+      st_lse2 = rows[kRowLse2 * (int64_t)p.padded_rows];
+      st_delta = rows[kRowDelta * (int64_t)p.padded_rows];
+      st_slope2 = kBias ? p.slopes[head] * kLog2e : 0.0f;
       st_position = p.q_offset + i;
     }
   };
@@ -354,14 +354,12 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
       for (int r = 0; r < 16; r++) {
         int const at = 8 * (r >> 2) + 4 * h32 + (r & 3);
         float x = s[r] * p.scale_log2, slope = p.scale;
-        if constexpr (EXTRA) {
-          if (p.cap_out != 0.0f) {
-            float const tanh = cap_tanh<T>(p, s[r]);
-            x = p.cap_out * tanh;
-            slope *= 1.0f - tanh * tanh;
-          }
-          x -= rs.slope2[at] * (float)abs(rs.position[at] - kv);
+        if constexpr (kCap) {
+          float const tanh = cap_tanh<T>(p, s[r]);
+          x = p.cap_out * tanh;
+          slope *= 1.0f - tanh * tanh;
         }
+        if constexpr (kBias) x = __builtin_fmaf(-rs.slope2[at], (float)abs(rs.position[at] - kv), x);
         pv[r] = __builtin_amdgcn_exp2f(x - rs.lse2[at]);
         if constexpr (kDk) ds[r] = pv[r] * (dp[r] - rs.delta[at]) * slope;
         if (!whole && (kv < rs.lo[at] || kv >= rs.hi[at])) {
@@ -405,8 +403,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
     }
 }
 
-template <typename T, int DP, int RG, bool EXTRA>
-static hipError_t masked_dq_launch(hipStream_t st, MaskedAttnParams const &p) {
+template <typename T, int DP, int RG, int EXTRA>
+static hipError_t masked_dq_launch_as(hipStream_t st, MaskedAttnParams const &p) {
   static LdsOptIn opt_in;
   using C = MaskedDq<T, DP, RG>;
   auto kernel = &masked_dq_kernel<T, DP, RG, EXTRA>;
@@ -417,8 +415,8 @@ static hipError_t masked_dq_launch(hipStream_t st, MaskedAttnParams const &p) {
   return hipGetLastError();
 }
 
-template <typename T, int DP, int WHAT, bool EXTRA>
-static hipError_t masked_dkdv_launch(hipStream_t st, MaskedAttnParams const &p) {
+template <typename T, int DP, int WHAT, int EXTRA>
+static hipError_t masked_dkdv_launch_as(hipStream_t st, MaskedAttnParams const &p) {
   static LdsOptIn opt_in;
   using C = MaskedDkdv<T, DP>;
   auto kernel = &masked_dkdv_kernel<T, DP, WHAT, EXTRA>;
@@ -427,6 +425,24 @@ static hipError_t masked_dkdv_launch(hipStream_t st, MaskedAttnParams const &p) 
   int64_t const grid = ceil_div(p.Skv, 128) * p.KH * p.B;
   kernel<<<dim3((unsigned)grid), 256, C::kBytes, st>>>(p);
   return hipGetLastError();
+}
+
+template <typename T, int DP, int RG>
+static hipError_t masked_dq_launch(hipStream_t st, MaskedAttnParams const &p) {
+  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
+  return cap && bias ? masked_dq_launch_as<T, DP, RG, 3>(st, p)
+         : cap       ? masked_dq_launch_as<T, DP, RG, 1>(st, p)
+         : bias      ? masked_dq_launch_as<T, DP, RG, 2>(st, p)
+                     : masked_dq_launch_as<T, DP, RG, 0>(st, p);
+}
+
+template <typename T, int DP, int WHAT>
+static hipError_t masked_dkdv_launch(hipStream_t st, MaskedAttnParams const &p) {
+  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
+  return cap && bias ? masked_dkdv_launch_as<T, DP, WHAT, 3>(st, p)
+         : cap       ? masked_dkdv_launch_as<T, DP, WHAT, 1>(st, p)
+         : bias      ? masked_dkdv_launch_as<T, DP, WHAT, 2>(st, p)
+                     : masked_dkdv_launch_as<T, DP, WHAT, 0>(st, p);
 }
 
 }  // namespace ffk

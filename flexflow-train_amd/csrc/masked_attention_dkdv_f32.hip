@@ -4,22 +4,22 @@
 namespace ffk {
 
 template <int DP>
-static hipError_t by_parts(hipStream_t st, MaskedAttnParams const &p, bool extra) {
+static hipError_t by_parts(hipStream_t st, MaskedAttnParams const &p) {
   if constexpr (DP <= 128) {
-    return extra ? masked_dkdv_launch<float, DP, 3, true>(st, p) : masked_dkdv_launch<float, DP, 3, false>(st, p);
+    return masked_dkdv_launch<float, DP, 3>(st, p);
   } else {
-    hipError_t const e = extra ? masked_dkdv_launch<float, DP, 1, true>(st, p) : masked_dkdv_launch<float, DP, 1, false>(st, p);
+    hipError_t const e = masked_dkdv_launch<float, DP, 1>(st, p);
     if (e != hipSuccess) return e;
-    return extra ? masked_dkdv_launch<float, DP, 2, true>(st, p) : masked_dkdv_launch<float, DP, 2, false>(st, p);
+    return masked_dkdv_launch<float, DP, 2>(st, p);
   }
 }
 
-hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra) {
+hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded) {
   switch (padded) {
-    case 64: return by_parts<64>(st, p, extra);
-    case 96: return by_parts<96>(st, p, extra);
-    case 128: return by_parts<128>(st, p, extra);
-    default: return by_parts<256>(st, p, extra);
+    case 64: return by_parts<64>(st, p);
+    case 96: return by_parts<96>(st, p);
+    case 128: return by_parts<128>(st, p);
+    default: return by_parts<256>(st, p);
   }
 }
 

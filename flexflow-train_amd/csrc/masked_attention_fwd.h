@@ -23,10 +23,11 @@ struct MaskedFwd {
   static_assert(kBytes <= 156 * 1024, "LDS of a CU");
 };
 
-template <typename T, int DP, int RG, bool EXTRA>
+template <typename T, int DP, int RG, int EXTRA>
 __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
   using C = MaskedFwd<T, DP, RG>;
   constexpr int J = C::kJ, KW = C::kKW;
+  constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ int window[2][4];
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
   T const *qp = static_cast<T const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * p.Dq;
   T const *kp = static_cast<T const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * p.Dq;
   T const *vp = static_cast<T const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * p.Dv;
-  float const slope2 = EXTRA && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.0f;
+  float const slope2 = kBias ? p.slopes[head] * kLog2e : 0.0f;
   int const position = p.q_offset + qi;
 
   Frag<T> qf[DP / 16];
@@ -120,13 +121,8 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           float x = s[j][r];
-          if constexpr (EXTRA) {
-            x = p.cap_out != 0.0f ? p.cap_out * cap_tanh<T>(p, x) : x * p.scale_log2;
-            int const kv = kv0 + j * 32 + 8 * (r >> 2) + 4 * h32 + (r & 3);
-            x -= slope2 * (float)abs(position - kv);
-          } else {
-            x *= p.scale_log2;
-          }
+          x = kCap ? p.cap_out * cap_tanh<T>(p, x) : x * p.scale_log2;
+          if constexpr (kBias) x = __builtin_fmaf(-slope2, (float)abs(position - (kv0 + j * 32 + 8 * (r >> 2) + 4 * h32 + (r & 3))), x);
           s[j][r] = x;
         }
       }
@@ -257,8 +253,8 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
     p.lse[((int64_t)b * p.H + head) * p.Sq + qi] = l_run == 0.0f ? -INFINITY : (m_run + __log2f(l_run)) * kLn2;
 }
 
-template <typename T, int DP, int RG, bool EXTRA>
-static hipError_t masked_fwd_launch(hipStream_t st, MaskedAttnParams const &p) {
+template <typename T, int DP, int RG, int EXTRA>
+static hipError_t masked_fwd_launch_as(hipStream_t st, MaskedAttnParams const &p) {
   static LdsOptIn opt_in;
   using C = MaskedFwd<T, DP, RG>;
   auto kernel = &masked_fwd_kernel<T, DP, RG, EXTRA>;
@@ -267,6 +263,15 @@ static hipError_t masked_fwd_launch(hipStream_t st, MaskedAttnParams const &p) {
   int64_t const grid = ceil_div(p.R, 32 * RG) * p.splits * p.KH * p.B;
   kernel<<<dim3((unsigned)grid), 256, C::kBytes, st>>>(p);
   return hipGetLastError();
+}
+
+template <typename T, int DP, int RG>
+static hipError_t masked_fwd_launch(hipStream_t st, MaskedAttnParams const &p) {
+  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
+  return cap && bias ? masked_fwd_launch_as<T, DP, RG, 3>(st, p)
+         : cap       ? masked_fwd_launch_as<T, DP, RG, 1>(st, p)
+         : bias      ? masked_fwd_launch_as<T, DP, RG, 2>(st, p)
+                     : masked_fwd_launch_as<T, DP, RG, 0>(st, p);
 }
 
 }  // namespace ffk

@@ -4,17 +4,17 @@
 namespace ffk {
 
 template <int DP>
-static hipError_t by_rows(hipStream_t st, MaskedAttnParams const &p, bool extra, int groups) {
-  if (groups == 1) return extra ? masked_fwd_launch<bf16, DP, 1, true>(st, p) : masked_fwd_launch<bf16, DP, 1, false>(st, p);
-  return extra ? masked_fwd_launch<bf16, DP, 4, true>(st, p) : masked_fwd_launch<bf16, DP, 4, false>(st, p);
+static hipError_t by_rows(hipStream_t st, MaskedAttnParams const &p, int groups) {
+  if (groups == 1) return masked_fwd_launch<bf16, DP, 1>(st, p);
+  return masked_fwd_launch<bf16, DP, 4>(st, p);
 }
 
-hipError_t masked_attention_fwd_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, bool extra, int groups) {
+hipError_t masked_attention_fwd_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, int groups) {
   switch (padded) {
-    case 64: return by_rows<64>(st, p, extra, groups);
-    case 96: return by_rows<96>(st, p, extra, groups);
-    case 128: return by_rows<128>(st, p, extra, groups);
-    default: return by_rows<256>(st, p, extra, groups);
+    case 64: return by_rows<64>(st, p, groups);
+    case 96: return by_rows<96>(st, p, groups);
+    case 128: return by_rows<128>(st, p, groups);
+    default: return by_rows<256>(st, p, groups);
   }
 }
 

@@ -1,0 +1,389 @@
+// Masked attention, dK and dV for bf16 heads of 64 and 128 (see masked_attention.h for the mathematics and layouts).
+//
+// One workgroup owns 128 keys of one key head, 32 to a wave, whose K and V rows are MFMA operands in registers for the
+// whole kernel next to the accumulators; one wave runs on a SIMD.  It streams the rows of all query heads that read the key
+// head in tiles of 64, two halves of 32: Q, dO and what the dQ kernel left of the rows arrive by direct loads in three LDS
+// buffers, two tiles ahead.  Vector and matrix work overlap inside the wave: the exponentials and dS of one half are cut
+// into units that sit behind the MFMAs of the other half's products, fenced against the scheduler.
+//   Which tiles: a list in LDS of those with a row that sees one of the 128 keys, from the summaries of ranges, made for
+// 512 tiles at a time.  A wave passes over a tile none of whose rows sees its 32 keys, and compares ranges element by
+// element only where not all rows see all of them.  Rows that see none of the 128 keys are cleared in LDS before use: what
+// lies in them must not meet the zeros of the masked probabilities.
+//   A tile lies in LDS as in memory, [64 rows][D], the 16-byte chunks of a row permuted on the fetching side such that
+// both ways it is read (16 bytes a lane by rows, and turned) are free of bank conflicts.
+#include "masked_attention.h"
+#include "lds_dma.h"
+
+namespace ffk {
+
+template <int D>
+struct WideDkdv {
+  static constexpr int kKeys = 128, kRows = 64;
+  static constexpr int kCPR = D / 8;                // 16-byte chunks of a row
+  static constexpr int kLoads = kRows * kCPR / 256; // direct loads of a thread, per tensor and tile
+  static constexpr int kRowsPerLoad = 256 / kCPR;
+  static constexpr int kTile = kRows * D;
+  static constexpr int kList = 512;  // tiles listed at a time
+  static_assert(D == 64 || D == 128, "permutations are written for these two");
+  __device__ static int swz(int row) {
+    return D == 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+  }
+};
+
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void masked_dkdv_wide_kernel(MaskedAttnParams p) {
+  using C = WideDkdv<D>;
+  constexpr int NBUF = 3;
+  __shared__ __attribute__((aligned(1024))) bf16 Qs[NBUF][C::kTile];
+  __shared__ __attribute__((aligned(1024))) bf16 Gs[NBUF][C::kTile];
+  __shared__ __attribute__((aligned(256))) float Rows[NBUF][BIAS ? 6 : 4][64];  // the fields of a tile's rows
+  __shared__ __attribute__((aligned(256))) float Unused[64];
+  __shared__ int list_tile[C::kList];
+  __shared__ RangeSummary list_sum[C::kList];
+  __shared__ int wave_count[4];
+  int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
+  int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  int const hb = blockIdx.x % (p.KH * p.B);
+  int const kh = hb % p.KH, b = hb / p.KH;
+  int const kv0 = (int)(blockIdx.x / (p.KH * p.B)) * C::kKeys;  // under a causal mask the first keys are seen by most rows
+  int const wkv0 = kv0 + wave * 32, kvcol = wkv0 + (lane & 31);
+  bf16 const *qp = static_cast<bf16 const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)kh * p.G * D;
+  bf16 const *gp = static_cast<bf16 const *>(p.d_o) + (int64_t)b * p.o_bs + (int64_t)kh * p.G * D;
+  bf16 const *kp = static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * D;
+  bf16 const *vp = static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * D;
+  float const *rowp = p.rows + (int64_t)hb * kRowFields * p.padded_rows;
+
+  bf16x8 kf[D / 16], vf[D / 16];
+  {
+    int const r = min(kvcol, p.Skv - 1);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; kk++) {
+      kf[kk] = *reinterpret_cast<bf16x8 const *>(kp + (int64_t)r * p.k_ss + kk * 16 + h32 * 8);
+      vf[kk] = *reinterpret_cast<bf16x8 const *>(vp + (int64_t)r * p.v_ss + kk * 16 + h32 * 8);
+    }
+  }
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      dk[i][r] = 0.0f;
+      dv[i][r] = 0.0f;
+    }
+
+  // Direct loads of a tile: thread slot c (of 256 a load) writes LDS chunk c of the load's 4 KB and fetches the chunk that
+  // the permutation puts there.  The rows' fields: one load of 64 values to each wave (two with slopes and positions;
+  // waves 2 and 3 then fetch theirs a second time to where nobody reads), so that one wait count fits all waves.
+  int const slot_row = t / C::kCPR, slot_lc = (t % C::kCPR) ^ C::swz(t / C::kCPR);
+  unsigned const qs_addr = lds_address_of(&Qs[0][0]), gs_addr = lds_address_of(&Gs[0][0]), rows_addr = lds_address_of(&Rows[0][0][0]);
+  unsigned const unused_addr = lds_address_of(&Unused[0]);
+  i32x4 const rq = buffer_resource(qp), rg = buffer_resource(gp);
+  i32x4 const rr = buffer_resource(rowp + (int64_t)wave * p.padded_rows);
+  i32x4 const rx = buffer_resource(rowp + (int64_t)(kRowSlope2 + (wave & 1)) * p.padded_rows);
+  constexpr int kFields = BIAS ? 6 : 4;
+  constexpr int kLoadsPerTile = 2 * C::kLoads + (BIAS ? 2 : 1);
+  auto issue_tile = [&](int row0, int buf) {
+#pragma unroll
+    for (int i = 0; i < C::kLoads; i++) {
+      int qi, g;
+      row_of(p, min(row0 + slot_row + i * C::kRowsPerLoad, p.R - 1), qi, g);
+      unsigned const dst = (unsigned)(buf * C::kTile * 2 + (i * 4 + wave) * 1024);
+      unsigned const in_row = (unsigned)(g * D + slot_lc * 8) * 2u;
+      lds_dma16(rq, (unsigned)qi * ((unsigned)p.q_ss * 2u) + in_row, 0u, qs_addr + dst);
+      lds_dma16(rg, (unsigned)qi * ((unsigned)p.o_ss * 2u) + in_row, 0u, gs_addr + dst);
+    }
+    unsigned const at = (unsigned)(row0 + lane) * 4u;  // padded_rows is whole tiles
+    lds_dma4(rr, at, 0u, rows_addr + (unsigned)(buf * kFields + wave) * 256u);
+    if constexpr (BIAS)
+      lds_dma4(rx, at, 0u, wave >= 2 ? unused_addr : rows_addr + (unsigned)(buf * kFields + kRowSlope2 + wave) * 256u);
+  };
+
+  // Per-lane LDS offsets (in elements) of the two ways a tile is read (32 rows from its first row on).
+  int row_off[D / 16], tr_off[D / 32][2];
+  {
+    int const r = lane & 31;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; kk++) row_off[kk] = r * D + (((2 * kk + h32) ^ C::swz(r)) << 3);
+    int const i16 = lane & 15, q = i16 >> 2, bb = (lane >> 4) & 1, c = i16 & 3;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+#pragma unroll
+      for (int sec = 0; sec < 2; sec++) {
+        int const row = 8 * sec + 4 * h32 + q, chunk = 4 * i + 2 * bb + (c >> 1);
+        tr_off[i][sec] = row * D + ((chunk ^ C::swz(row)) << 3) + 4 * (c & 1);
+      }
+  }
+  auto turned = [&](bf16 const *tile, int s, int i) __attribute__((always_inline)) -> bf16x8 {
+    union {
+      s16x4 h2[2];
+      bf16x8 v;
+    } u;
+    u.h2[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tr_off[i][0] + 16 * s * D));
+    u.h2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tr_off[i][1] + 16 * s * D));
+    return u.v;
+  };
+
+  int const nsum = (p.R + 31) / 32, ntiles = (p.R + 63) / 64;
+  RangeSummary const *sums = p.summary + (int64_t)b * nsum;
+  for (int chunk = 0; chunk < ntiles; chunk += C::kList) {
+    // the tiles of this chunk that are worked on, in order
+    int count = 0;
+#pragma unroll
+    for (int part = 0; part < C::kList / 256; part++) {
+      int const tile = chunk + part * 256 + t;
+      RangeSummary s = {1 << 30, 0, 1 << 30, 0};
+      if (tile < ntiles) {
+        s = sums[2 * tile];
+        RangeSummary const s1 = 2 * tile + 1 < nsum ? sums[2 * tile + 1] : RangeSummary{1 << 30, 0, 1 << 30, 0};
+        s = RangeSummary{min(s.lo_min, s1.lo_min), max(s.hi_max, s1.hi_max), max(s.lo_max, s1.lo_max), min(s.hi_min, s1.hi_min)};
+      }
+      bool const wanted = s.lo_min < kv0 + C::kKeys && s.hi_max > kv0;
+      uint64_t const mask = __builtin_amdgcn_ballot_w64(wanted);
+      __syncthreads();  // the counts (and, in the first part, the lists) are free
+      if (lane == 0) wave_count[wave] = __builtin_popcountll(mask);
+      __syncthreads();
+      int at = count;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        int const n = __builtin_amdgcn_readfirstlane(wave_count[w]);
+        if (w < wave) at += n;
+        count += n;
+      }
+      if (wanted) {
+        at += __builtin_popcountll(mask & ((1ull << lane) - 1));
+        list_tile[at] = tile;
+        list_sum[at] = s;
+      }
+    }
+    __syncthreads();
+    if (count == 0) continue;  // uniform
+
+    auto row0_of = [&](int n) { return __builtin_amdgcn_readfirstlane(list_tile[n]) * C::kRows; };
+    issue_tile(row0_of(0), 0);
+    issue_tile(row0_of(min(1, count - 1)), 1);
+    int next_row0 = row0_of(min(2, count - 1));
+    // tiles 0 and 1 have landed, and so have the K and V fragments: told to the compiler
+    wait_all_vmem_known_to_compiler();
+    __syncthreads();
+    int cur = 0;
+    for (int it = 0; it < count; it++) {
+      // buffer (it+2) % 3 was read during step it-1; every wave has passed the barrier that ended it.  Past the end the last
+      // tile is fetched again into a buffer nobody reads: the count of loads in flight is the same at every wait.
+      issue_tile(next_row0, cur == 0 ? 2 : cur - 1);
+      RangeSummary const sum = list_sum[it];
+      int const lo_min = __builtin_amdgcn_readfirstlane(sum.lo_min), hi_max = __builtin_amdgcn_readfirstlane(sum.hi_max);
+      int const lo_max = __builtin_amdgcn_readfirstlane(sum.lo_max), hi_min = __builtin_amdgcn_readfirstlane(sum.hi_min);
+      next_row0 = row0_of(min(it + 3, count - 1));
+      bf16 *qt = Qs[cur], *gt = Gs[cur];
+      float const *fields = &Rows[cur][0][0];
+      int const *row_lo = reinterpret_cast<int const *>(fields + kRowLo * 64), *row_hi = reinterpret_cast<int const *>(fields + kRowHi * 64);
+      if (lo_max >= kv0 + C::kKeys || hi_min <= kv0) {  // uniform: a row here sees none of the keys
+        int const row = t >> 2;
+        if (row_lo[row] >= kv0 + C::kKeys || row_hi[row] <= kv0) {
+#pragma unroll
+          for (int c = 0; c < D / 32; c++) {
+            *reinterpret_cast<u32x4 *>(qt + row * D + (c * 4 + (t & 3)) * 8) = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4 *>(gt + row * D + (c * 4 + (t & 3)) * 8) = u32x4{0u, 0u, 0u, 0u};
+          }
+        }
+        __syncthreads();
+      }
+      if (lo_min < wkv0 + 32 && hi_max > wkv0) {
+        bool const edge = lo_max > wkv0 || hi_min < wkv0 + 32;
+        constexpr int NM = D / 8;     // MFMAs of a phase
+        constexpr int UPM = 16 / NM;  // units of vector work behind each
+        constexpr int kAhead = 3;     // an LDS fragment is read this many MFMAs ahead of its use
+        constexpr int NI = D / 32;
+        // S = Q K^T and dP = dO V^T of one half: rows = its 32 rows, column = key; MFMA m: d step m / 2, Q (even) or dO
+        auto sdp_frag = [&](int h, int m) __attribute__((always_inline)) {
+          return *reinterpret_cast<bf16x8 const *>(((m & 1) ? gt : qt) + h * 32 * D + row_off[m >> 1]);
+        };
+        // dV += P^T dO, dK += dS^T Q of one half; MFMA m: step m / (2 NI), d block (m / 2) % NI, dO (even) or Q
+        auto grad_frag = [&](int h, int m) __attribute__((always_inline)) {
+          return turned(((m & 1) ? qt : gt) + h * 32 * D, m / (2 * NI), (m >> 1) % NI);
+        };
+        // The vector work of a half, 16 units of one score each.  Unit 4 g reads the fields of rows 8 g + 4 (l/32) .. + 3.
+        float pv[2][16], dsv[2][16];
+        f32x4 lrow, drow, srow;
+        i32x4 prow;
+        auto unit = [&](int h, int u, f32x16 const &s, f32x16 const &dp) __attribute__((always_inline)) {
+          int const at = h * 32 + 2 * u + 4 * h32;
+          if ((u & 3) == 0) {
+            lrow = *reinterpret_cast<f32x4 const *>(fields + kRowLse2 * 64 + at);
+            drow = *reinterpret_cast<f32x4 const *>(fields + kRowDelta * 64 + at);
+            if constexpr (BIAS) {
+              srow = *reinterpret_cast<f32x4 const *>(fields + kRowSlope2 * 64 + at);
+              prow = *reinterpret_cast<i32x4 const *>(fields + kRowPosition * 64 + at);
+            }
+          }
+          float x, slope = p.scale;
+          if constexpr (CAP) {
+            float const tanh = cap_tanh<bf16>(p, s[u]);
+            x = __builtin_fmaf(p.cap_out, tanh, -lrow[u & 3]);
+            slope = __builtin_fmaf(-tanh * p.scale, tanh, p.scale);
+          } else {
+            x = __builtin_fmaf(s[u], p.scale_log2, -lrow[u & 3]);
+          }
+          if constexpr (BIAS) x = __builtin_fmaf(-srow[u & 3], (float)abs(prow[u & 3] - kvcol), x);
+          float const e = __builtin_amdgcn_exp2f(x);
+          pv[h][u] = e;
+          dsv[h][u] = e * ((dp[u] - drow[u & 3]) * slope);
+          pin_here(pv[h][u]);
+          pin_here(dsv[h][u]);
+        };
+        auto mask_half = [&](int h) {
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            i32x4 const lo4 = *reinterpret_cast<i32x4 const *>(row_lo + h * 32 + 8 * g + 4 * h32);
+            i32x4 const hi4 = *reinterpret_cast<i32x4 const *>(row_hi + h * 32 + 8 * g + 4 * h32);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              bool const masked = kvcol < lo4[e] || kvcol >= hi4[e];
+              pv[h][4 * g + e] = masked ? 0.0f : pv[h][4 * g + e];
+              dsv[h][4 * g + e] = masked ? 0.0f : dsv[h][4 * g + e];
+            }
+          }
+        };
+        f32x16 s[2], dp[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            s[h][r] = 0.0f;
+            dp[h][r] = 0.0f;
+          }
+        bf16x8 fr[NM];
+
+        // ---- phase 1: S, dP of half 0 ----
+#pragma unroll
+        for (int m = 0; m < kAhead; m++) fr[m] = sdp_frag(0, m);
+        static_for<0, NM>([&](auto mc) {
+          constexpr int m = decltype(mc)::value;
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m % 2 == 0) {
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[m], kf[m / 2], s[0], 0, 0, 0);
+          } else {
+            dp[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[m], vf[m / 2], dp[0], 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m + kAhead < NM) fr[m + kAhead] = sdp_frag(0, m + kAhead);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- phase 2: S, dP of half 1 on the matrix pipe, P and dS of half 0 on the vector ALU ----
+        bf16x8 fr2[NM];
+#pragma unroll
+        for (int m = 0; m < kAhead; m++) fr2[m] = sdp_frag(1, m);
+        static_for<0, NM>([&](auto mc) {
+          constexpr int m = decltype(mc)::value;
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m % 2 == 0) {
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr2[m], kf[m / 2], s[1], 0, 0, 0);
+          } else {
+            dp[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr2[m], vf[m / 2], dp[1], 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m + kAhead < NM) fr2[m + kAhead] = sdp_frag(1, m + kAhead);
+          static_for<0, UPM>([&](auto uc) { unit(0, m * UPM + decltype(uc)::value, s[0], dp[0]); });
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        if (edge) mask_half(0);
+        bf16x8 pa[2][2], da[2][2];
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++) {
+          pa[0][s2] = pack8(pv[0] + 8 * s2);
+          da[0][s2] = pack8(dsv[0] + 8 * s2);
+        }
+
+        // ---- phase 3: dV, dK of half 0 on the matrix pipe, P and dS of half 1 on the vector ALU ----
+        bf16x8 fr3[NM];
+#pragma unroll
+        for (int m = 0; m < kAhead; m++) fr3[m] = grad_frag(0, m);
+        static_for<0, NM>([&](auto mc) {
+          constexpr int m = decltype(mc)::value;
+          constexpr int s2 = m / (2 * NI), i = (m / 2) % NI;
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m % 2 == 0) {
+            dv[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa[0][s2], fr3[m], dv[i], 0, 0, 0);
+          } else {
+            dk[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da[0][s2], fr3[m], dk[i], 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m + kAhead < NM) fr3[m + kAhead] = grad_frag(0, m + kAhead);
+          static_for<0, UPM>([&](auto uc) { unit(1, m * UPM + decltype(uc)::value, s[1], dp[1]); });
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        if (edge) mask_half(1);
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++) {
+          pa[1][s2] = pack8(pv[1] + 8 * s2);
+          da[1][s2] = pack8(dsv[1] + 8 * s2);
+        }
+
+        // ---- phase 4: dV, dK of half 1 ----
+        bf16x8 fr4[NM];
+#pragma unroll
+        for (int m = 0; m < kAhead; m++) fr4[m] = grad_frag(1, m);
+        static_for<0, NM>([&](auto mc) {
+          constexpr int m = decltype(mc)::value;
+          constexpr int s2 = m / (2 * NI), i = (m / 2) % NI;
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m % 2 == 0) {
+            dv[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa[1][s2], fr4[m], dv[i], 0, 0, 0);
+          } else {
+            dk[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da[1][s2], fr4[m], dk[i], 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (m + kAhead < NM) fr4[m + kAhead] = grad_frag(1, m + kAhead);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_vmcnt<kLoadsPerTile>();  // this wave's part of the next tile has landed
+      __syncthreads();
+      cur = cur == 2 ? 0 : cur + 1;
+    }
+    wait_vmcnt<0>();
+    __syncthreads();  // the buffers are free: no load is in flight, no wave reads a tile
+  }
+
+  // Accumulators: row = key (8*(r/4) + 4*(l/32) + r%4 of the wave's 32), column = d.  Each wave turns its 32 x D block
+  // around in LDS (the tiles are done with) and writes whole 16-byte pieces of rows.
+  __syncthreads();
+  bf16 *const stage = (wave < 2 ? &Qs[0][0] : &Gs[0][0]) + (wave & 1) * 32 * D;
+  static_assert(2 * 32 * D <= NBUF * C::kTile, "staging fits the tile buffers");
+  auto write_out = [&](f32x16 const (&acc)[D / 32], bf16 *out, int64_t row_stride) {
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        VecIO<bf16>::store1(stage + (8 * (r >> 2) + 4 * h32 + (r & 3)) * D + i * 32 + (lane & 31), acc[i][r]);
+    // LDS operations of one wave complete in order: the reads below see the writes above
+#pragma unroll
+    for (int k = 0; k < 32 * (D / 8) / 64; k++) {
+      int const c = lane + k * 64;
+      int const row = c / (D / 8), ch = c % (D / 8);
+      u32x4 const v = *reinterpret_cast<u32x4 const *>(stage + row * D + ch * 8);
+      if (wkv0 + row < p.Skv) *reinterpret_cast<u32x4 *>(out + (int64_t)(wkv0 + row) * row_stride + ch * 8) = v;
+    }
+  };
+  write_out(dk, static_cast<bf16 *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kh * D, p.k_ss);
+  write_out(dv, static_cast<bf16 *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kh * D, p.v_ss);
+}
+
+template <int D>
+static void launch(hipStream_t st, MaskedAttnParams const &p) {
+  dim3 const grid((unsigned)(ceil_div(p.Skv, 128) * p.KH * p.B));
+  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
+  if (cap && bias) masked_dkdv_wide_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
+  else if (cap) masked_dkdv_wide_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
+  else if (bias) masked_dkdv_wide_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
+  else masked_dkdv_wide_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
+}
+
+hipError_t masked_attention_dkdv_wide(hipStream_t st, MaskedAttnParams const &p) {
+  if (p.Dq == 64) launch<64>(st, p);
+  else launch<128>(st, p);
+  return hipGetLastError();
+}
+
+}  // namespace ffk

@@ -149,6 +149,46 @@ def test_given_ranges(ffk, kind, D, dtype):
         assert all(not got[n].any() for n in ("o", "dq", "dk", "dv"))
 
 
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("kind", sorted(RANGES) + ["causal"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (20.0, False), (0.0, True), (5.0, True)])
+def test_both_forward_kernels(ffk, kind, D, cap, bias, variant):
+    """32 and 64 rows to a wave (the size decides otherwise), over every kind of range, with heads that share keys."""
+    say("masked attention, forward variant", variant, kind, D, cap, bias)
+    B, Sq, Skv, H, KH = 2, 210, 290, 6, 2
+    q, k, v, _ = make(D + 2, B, Sq, Skv, H, KH, D, D, BF, 3.0 if cap else 1.0)
+    ranges = None
+    if kind != "causal":
+        rows = RANGES[kind](B, Sq, Skv)
+        ranges = torch.tensor([rows, rows[::-1]], dtype=torch.int32).cuda()
+    slopes = slopes_of(H) if bias else None
+    ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, variant)
+    try:
+        o, lse = ffk.masked_attention_forward(q, k, v, D ** -0.5, causal=kind == "causal", score_cap=cap, key_ranges=ranges, distance_slopes=slopes)
+        torch.cuda.synchronize()
+    finally:
+        ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, 0)
+    want = attention(q, k, v, D ** -0.5, kind == "causal", cap, ranges, slopes, unit=2.0 ** -8)
+    check(o, want, "o")
+    check(lse, want, "lse")
+
+
+def test_forward_kernel_that_the_size_asks_for(ffk):
+    """256 workgroups of 256 rows over more than a thousand keys: 64 rows to a wave by itself."""
+    compare(ffk, *make(40, 4, 70, 1030, 64, 64, 64, 64, BF), causal=False, cap=20.0)
+
+
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (20.0, False), (0.0, True), (5.0, True)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_tiles_of_rows(ffk, D, cap, bias):
+    """More tiles of rows than the dK/dV kernel lists at a time, most of which see none of a workgroup's keys."""
+    B, Sq, Skv, H, KH = 1, 6000, 300, 6, 1
+    q, k, v, d_o = make(D + 3, B, Sq, Skv, H, KH, D, D, BF)
+    ranges = torch.tensor([[[0, 0] if i % 700 < 300 else [i * 37 % 250, i * 37 % 250 + 1 + i % 50] for i in range(Sq)]], dtype=torch.int32).cuda()
+    compare(ffk, q, k, v, d_o, ranges=ranges, cap=cap, slopes=slopes_of(H) if bias else None)
+
+
 def test_ranges_and_causal_both_apply(ffk):
     q, k, v, d_o = make(4, 1, 200, 200, 2, 2, 64, 64, BF)
     ranges = torch.tensor([[[i // 2, 200] for i in range(200)]], dtype=torch.int32).cuda()
