@@ -29,7 +29,7 @@ struct RangeSummary {
 
 // What the dQ kernels leave in memory of every row for the dK/dV kernels: arrays of padded_rows entries, one set for each
 // (batch, key head), which a tile's rows are read from in order.  Rows behind the last one see nothing.
-enum { kRowLse2 = 0, kRowDelta = 1, kRowLo = 2, kRowHi = 3, kRowSlope2 = 4, kRowPosition = 5, kRowFields = 6 };
+enum { kRowLse2 = 0, kRowDelta = 1, kRowLo = 2, kRowHi = 3, kRowSlope = 4, kRowPosition = 5, kRowFields = 6 };
 
 struct MaskedAttnParams {
   void const *q, *k, *v;
@@ -45,11 +45,12 @@ struct MaskedAttnParams {
   int padded_rows;                      // R up to whole tiles of 64
   int64_t q_bs, q_ss, k_bs, k_ss, v_bs, v_ss, o_bs, o_ss;
   int q_offset;
-  float scale, scale_log2;
-  float cap_in;   // 2 log2(e) scale / cap: tanh(x / cap) = 1 - 2 / (1 + 2^(cap_in raw))
-  float cap_out;  // cap log2(e)
-  float inv_cap_scale;  // scale / cap
-  int causal;
+  // A score in powers of two is  score_scale y + shift,  y = capped<T>(raw) - slope_unit slope_h |p_i - j|  (see capped);
+  // its derivative by the raw product, over ln 2, is score_scale times the derivative of capped.  What is the same for
+  // all scores of a row is taken out of the loops: the shift goes into the log-sum-exp, the gradients' factor to their store.
+  float score_scale, shift, slope_unit, grad_scale;
+  float cap_in;
+  int capped, causal;
   FastDiv group;
   // forward, split over the keys: partial O (unnormalised), maximum and sum of each part
   int splits;
@@ -79,7 +80,7 @@ __device__ __forceinline__ void row_range(MaskedAttnParams const &p, int b, int 
 }
 
 __device__ __forceinline__ void write_row(MaskedAttnParams const &p, int b, int kh, int row, float lse2, float delta, int lo, int hi,
-                                          float slope2, int position) {
+                                          float slope, int position) {
   if (row >= p.padded_rows) return;
   float *rows = p.rows + (int64_t)(b * p.KH + kh) * kRowFields * p.padded_rows + row;
   int64_t const n = p.padded_rows;
@@ -88,7 +89,7 @@ __device__ __forceinline__ void write_row(MaskedAttnParams const &p, int b, int 
   rows[kRowLo * n] = __int_as_float(lo);
   rows[kRowHi * n] = __int_as_float(hi);
   if (p.slopes != nullptr) {
-    rows[kRowSlope2 * n] = slope2;
+    rows[kRowSlope * n] = slope;
     rows[kRowPosition * n] = __int_as_float(position);
   }
 }
@@ -199,16 +200,26 @@ struct TileRegs {
   }
 };
 
-// tanh(scale raw / cap).  bf16 kernels: 1 - 2 / (1 + 2^(cap_in raw)) on the hardware's exponential and reciprocal,
-// about 2^-22 off in absolute terms, which the cap multiplies to a few 1e-6 of a score, far below what bf16 scores carry.
-// fp32 kernels, whose matrix products take sixteen times as long, take the library's.
-template <typename T>
-__device__ __forceinline__ float cap_tanh(MaskedAttnParams const &p, float raw) {
-  if constexpr (sizeof(T) == 2) {
-    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * p.cap_in));
+// The cap's part of a score that is not linear, and its derivative (1 without a cap, where y is the raw product).
+//   fp32: y = tanh(scale raw / cap), score_scale = cap log2(e), derivative 1 - y^2.
+//   bf16: y = -1 / (1 + 2^(cap_in raw)), cap_in = 2 log2(e) scale / cap, on the hardware's exponential and reciprocal: tanh is
+//   1 + 2 y, so score_scale = 2 cap log2(e), shift = cap log2(e), and 1 - tanh^2 = -4 (y + y^2), of which grad_scale has the
+//   -4.  Four vector instructions a score and two for the derivative; about 2^-22 off in absolute terms, which the cap
+//   multiplies to a few 1e-6 of a score, far below what bf16 scores carry.  (fp32's products take sixteen times as long: it
+//   can have the library's tanh.)
+template <typename T, bool CAP>
+__device__ __forceinline__ float capped(MaskedAttnParams const &p, float raw) {
+  if constexpr (!CAP) {
+    return raw;
+  } else if constexpr (sizeof(T) == 2) {
+    return -__builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * p.cap_in));
   } else {
-    return tanhf(raw * p.inv_cap_scale);
+    return tanhf(raw * p.cap_in);
   }
+}
+template <typename T>
+__device__ __forceinline__ float capped_slope(float y) {
+  return sizeof(T) == 2 ? __builtin_fmaf(y, y, y) : __builtin_fmaf(-y, y, 1.0f);
 }
 
 // A wave's smallest and largest of an integer, scalar.

@@ -10,12 +10,12 @@ hipError_t masked_attention_fwd_bf16(hipStream_t st, MaskedAttnParams const &p, 
 hipError_t masked_attention_fwd_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
 hipError_t masked_attention_dq_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
 hipError_t masked_attention_dq_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
-hipError_t masked_attention_dkdv_bf16(hipStream_t st, MaskedAttnParams const &p, int padded);
-hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded);
-// bf16, head sizes 64 and 128: masked_attention_wide_{fwd,dq,dkdv}.hip
-hipError_t masked_attention_fwd_wide(hipStream_t st, MaskedAttnParams const &p);
-hipError_t masked_attention_dq_wide(hipStream_t st, MaskedAttnParams const &p);
-hipError_t masked_attention_dkdv_wide(hipStream_t st, MaskedAttnParams const &p);
+hipError_t masked_attention_dkdv_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
+hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
+// bf16, head sizes 64 and 128: masked_attention_heads_{fwd,dq,dkdv}.hip
+hipError_t masked_attention_fwd_heads(hipStream_t st, MaskedAttnParams const &p);
+hipError_t masked_attention_dq_heads(hipStream_t st, MaskedAttnParams const &p);
+hipError_t masked_attention_dkdv_heads(hipStream_t st, MaskedAttnParams const &p);
 
 // --------------------------------------------------------------------------
 // key ranges
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void masked_merge_kernel(MaskedAttnParams p) {
     store4(static_cast<T *>(p.o) + (int64_t)b * p.o_bs + (int64_t)i * p.o_ss + (int64_t)head * p.Dv + d, o[0] * inv, o[1] * inv, o[2] * inv,
            o[3] * inv);
   if (lane == 0 && p.lse != nullptr)
-    p.lse[((int64_t)b * p.H + head) * p.Sq + i] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+    p.lse[((int64_t)b * p.H + head) * p.Sq + i] = l == 0.0f ? -INFINITY : (m + p.shift + __log2f(l)) * kLn2;
 }
 
 // --------------------------------------------------------------------------
@@ -149,12 +149,12 @@ static int check(char const *who, int dtype, ffk_masked_attention_desc_t const *
   FFK_REQUIRE(d->batch == 1 || (d->q_batch_stride >= qw && d->k_batch_stride >= kw && d->v_batch_stride >= vw && d->o_batch_stride >= ow),
               "%s: a batch stride is smaller than a row of heads", who);
   FFK_REQUIRE(d->scale > 0.0f && isfinite(d->scale), "%s: scale must be positive and finite", who);
-  FFK_REQUIRE(d->score_cap >= 0.0f && isfinite(d->score_cap) && (d->score_cap == 0.0f || isfinite(d->scale / d->score_cap * 4.0f)),
+  FFK_REQUIRE(d->score_cap >= 0.0f && isfinite(d->score_cap) && (d->score_cap == 0.0f || (isfinite(d->scale / d->score_cap * 4.0f) && isfinite(d->score_cap * 4.0f))),
               "%s: score_cap must be 0 (none) or positive, finite and not vanishing beside scale", who);
   return FFK_OK;
 }
 
-static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, void const *q, void const *k, void const *v, int32_t const *ranges,
+static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, int dtype, void const *q, void const *k, void const *v, int32_t const *ranges,
                                   float const *slopes) {
   MaskedAttnParams p = {};
   p.q = q;
@@ -176,13 +176,19 @@ static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, void con
   p.v_bs = d->v_batch_stride; p.v_ss = d->v_seq_stride;
   p.o_bs = d->o_batch_stride; p.o_ss = d->o_seq_stride;
   p.q_offset = (int)d->query_offset;
-  p.scale = d->scale;
-  p.scale_log2 = d->scale * kLog2e;
-  if (d->score_cap != 0.0f) {
+  p.capped = d->score_cap != 0.0f;
+  p.score_scale = d->scale * kLog2e;
+  p.grad_scale = d->scale;
+  if (p.capped && dtype == FFK_BF16) {
     p.cap_in = 2.0f * kLog2e * (d->scale / d->score_cap);
-    p.cap_out = d->score_cap * kLog2e;
-    p.inv_cap_scale = d->scale / d->score_cap;
+    p.score_scale = 2.0f * kLog2e * d->score_cap;
+    p.shift = kLog2e * d->score_cap;
+    p.grad_scale = -4.0f * d->scale;
+  } else if (p.capped) {
+    p.cap_in = d->scale / d->score_cap;
+    p.score_scale = kLog2e * d->score_cap;
   }
+  p.slope_unit = kLog2e / p.score_scale;
   p.causal = d->causal != 0;
   p.padded_rows = (p.R + 63) / 64 * 64;
   p.group = make_fast_div((uint32_t)p.G);
@@ -198,19 +204,18 @@ static size_t backward_bytes(ffk_masked_attention_desc_t const *d) {
   return row_bytes(d) + (size_t)d->batch * ceil_div(rows_of(d), 32) * sizeof(RangeSummary);
 }
 
-// The kernels of masked_attention_wide_*.hip: bf16, one head size of 64 or 128, rows that 32-bit byte offsets reach.
-static bool wide_kernels(ffk_masked_attention_desc_t const *d, int dtype) {
+// The kernels of masked_attention_heads_*.hip: bf16, one head size of 64 or 128, rows that 32-bit byte offsets reach (of
+// all rows of an entry in the dK/dV kernel, of a tile in the others).
+static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype) {
   int64_t const lim = (int64_t)1 << 32;
   return dtype == FFK_BF16 && (d->head_dim == 64 || d->head_dim == 128) && (d->v_head_dim == 0 || d->v_head_dim == d->head_dim) &&
-         d->seq_q * d->q_seq_stride * 2 < lim && d->seq_q * d->o_seq_stride * 2 < lim;
+         d->k_seq_stride < (1 << 24) && d->v_seq_stride < (1 << 24) && d->seq_q * d->q_seq_stride * 2 < lim && d->seq_q * d->o_seq_stride * 2 < lim;
 }
-
-// 64 rows to a wave, 256 to a workgroup, one workgroup on a CU: where every CU has one and keys are long.
-static bool wide_forward(ffk_masked_attention_desc_t const *d, int dtype) {
-  // (its direct loads reach a tile of 64 keys with 32-bit byte offsets)
-  if (!wide_kernels(d, dtype) || d->k_seq_stride >= (1 << 24) || d->v_seq_stride >= (1 << 24)) return false;
-  int const variant = option(FFK_OPTION_ATTENTION_VARIANT);
-  return variant == 2 || (variant == 0 && d->seq_kv >= 1024 && ceil_div(rows_of(d), 256) * d->kv_heads * d->batch >= kNumCU);
+// 32-key groups of a workgroup of the general dK/dV kernel, and whether it is to run in place of the one above: 4, or 1 whose
+// four waves share out the rows, where workgroups of 128 keys would leave half of the CUs idle.
+static int key_groups(ffk_masked_attention_desc_t const *d) {
+  if (padded_head(d) > 128) return 4;  // (no registers left for the rows' tiles)
+  return rows_of(d) > 32 && ceil_div(d->seq_kv, 128) * d->kv_heads * d->batch < kNumCU / 2 ? 1 : 4;
 }
 
 }  // namespace ffk
@@ -251,7 +256,7 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
   FFK_REQUIRE(q && k && v && o, "masked_attention_forward: NULL tensor");
   FFK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "masked_attention_forward: tensors must be 16-byte aligned");
   FFK_REQUIRE(reinterpret_cast<uintptr_t>(key_ranges) % 8 == 0, "masked_attention_forward: key_ranges must be 8-byte aligned");
-  MaskedAttnParams p = params_of(d, q, k, v, key_ranges, distance_slopes);
+  MaskedAttnParams p = params_of(d, dtype, q, k, v, key_ranges, distance_slopes);
   p.o = o;
   p.lse = lse;
   hipStream_t const st = as_stream(stream);
@@ -261,8 +266,8 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = p.part_o + (int64_t)splits * p.B * p.KH * p.R * p.Dv;
   }
-  if (wide_forward(d, dtype)) {
-    FFK_HIP(masked_attention_fwd_wide(st, p));
+  if (row_groups(d, dtype) == 4 && heads_kernels(d, dtype)) {
+    FFK_HIP(masked_attention_fwd_heads(st, p));
     return FFK_OK;
   }
   auto const launch = dtype == FFK_BF16 ? masked_attention_fwd_bf16 : masked_attention_fwd_f32;
@@ -296,7 +301,7 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
     return fail(FFK_ERR_WORKSPACE, "masked_attention_backward: workspace must hold %zu bytes, 16-byte aligned (%zu given)", need,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
   }
-  MaskedAttnParams p = params_of(d, q, k, v, key_ranges, distance_slopes);
+  MaskedAttnParams p = params_of(d, dtype, q, k, v, key_ranges, distance_slopes);
   p.o = const_cast<void *>(o);
   p.d_o = d_o;
   p.lse = const_cast<float *>(lse);
@@ -310,9 +315,10 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
   auto const launch_dq = dtype == FFK_BF16 ? masked_attention_dq_bf16 : masked_attention_dq_f32;
   auto const launch_dkdv = dtype == FFK_BF16 ? masked_attention_dkdv_bf16 : masked_attention_dkdv_f32;
   int const groups = row_groups(d, dtype);
-  if (groups == 4 && wide_kernels(d, dtype)) FFK_HIP(masked_attention_dq_wide(st, p));
+  if (groups == 4 && heads_kernels(d, dtype)) FFK_HIP(masked_attention_dq_heads(st, p));
   else FFK_HIP(launch_dq(st, p, padded, groups));
-  if (wide_kernels(d, dtype)) FFK_HIP(masked_attention_dkdv_wide(st, p));
-  else FFK_HIP(launch_dkdv(st, p, padded));
+  int const keys = key_groups(d);
+  if (keys == 4 && heads_kernels(d, dtype)) FFK_HIP(masked_attention_dkdv_heads(st, p));
+  else FFK_HIP(launch_dkdv(st, p, padded, keys));
   return FFK_OK;
 }

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
   T const *op = static_cast<T const *>(p.o) + o_at;
   T const *kp = static_cast<T const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * p.Dq;
   T const *vp = static_cast<T const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * p.Dv;
-  float const slope2 = kBias ? p.slopes[head] * kLog2e : 0.0f;
+  float const slope = kBias ? p.slopes[head] * p.slope_unit : 0.0f;
   int const position = p.q_offset + qi;
 
   Frag<T> qf[DP / 16], gf[DP / 16];
@@ -88,8 +88,8 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
     }
   }
   delta += __shfl_xor(delta, 32, 64);
-  float const lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + qi] * kLog2e;
-  if (h32 == 0 && kw == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope2, position);
+  float const lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + qi] * kLog2e - p.shift;
+  if (h32 == 0 && kw == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope, position);
   if (rb == nrb - 1) write_padding(p, b, kh, nrb * 32 * RG, t);
 
   f32x16 dq[DP / 32];
@@ -135,18 +135,14 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
       }
       float ds[16];
       bool const whole = kv0 >= w_lo_max && kv0 + 32 <= w_hi_min;
+      float const distance = (float)(position - (kv0 + 4 * h32));
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        int const kv = kv0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
-        float x = s[r] * p.scale_log2, slope = p.scale;
-        if constexpr (kCap) {
-          float const tanh = cap_tanh<T>(p, s[r]);
-          x = p.cap_out * tanh;
-          slope *= 1.0f - tanh * tanh;
-        }
-        if constexpr (kBias) x = __builtin_fmaf(-slope2, (float)abs(position - kv), x);
-        float const e = __builtin_amdgcn_exp2f(x - lse2);
-        ds[r] = e * (dp[r] - delta) * slope;
+        float const y = capped<T, kCap>(p, s[r]);
+        float x = y;
+        if constexpr (kBias) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
+        ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
+        if constexpr (kCap) ds[r] *= capped_slope<T>(y);
       }
       if (!whole) {
 #pragma unroll
@@ -201,40 +197,49 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
 #pragma unroll
     for (int g = 0; g < 4; g++) {
       int const d = i * 32 + 8 * g + 4 * h32;
-      if (d < p.Dq) store4(dqp + d, dq[i][4 * g], dq[i][4 * g + 1], dq[i][4 * g + 2], dq[i][4 * g + 3]);
+      if (d < p.Dq)
+        store4(dqp + d, dq[i][4 * g] * p.grad_scale, dq[i][4 * g + 1] * p.grad_scale, dq[i][4 * g + 2] * p.grad_scale, dq[i][4 * g + 3] * p.grad_scale);
     }
 }
 
 // What a row brings along into LDS: its range, statistics, slope and position.
+template <int N>
 struct RowStats {
-  float lse2[32], delta[32], slope2[32];
-  int lo[32], hi[32], position[32];
+  float lse2[N], delta[N], slope[N];
+  int lo[N], hi[N], position[N];
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int KG>
 struct MaskedDkdv {
+  static constexpr int kKW = 4 / KG;
+  static constexpr int kT = 32 * kKW;  // rows of a step
   static constexpr int kS = TileStride<T, DP>::both;
-  static constexpr int kTile = 2 * 32 * kS * (int)sizeof(T);  // Q and dO
-  static constexpr int kBytes = 2 * kTile;
-  static_assert(kBytes <= 150 * 1024, "LDS of a CU");
+  static constexpr int kTile = 2 * kT * kS * (int)sizeof(T);  // Q and dO
+  static constexpr int kBuffers = 2 * kTile <= 144 * 1024 ? 2 : 1;
+  static constexpr int kMerge = (kKW - 1) * KG * DP * 32 * 4;
+  static constexpr int kBytes = kBuffers * kTile > kMerge ? kBuffers * kTile : kMerge;
+  static_assert(kBytes <= 154 * 1024, "LDS of a CU");
 };
 
+// KG groups of 32 keys, whose KW = 4 / KG waves take the tiles of 32 rows in turn (their sums meet in LDS at the end).
 // WHAT: bit 0 dV, bit 1 dK.  Both from one launch, but where the owned K and V rows and both accumulators are more than
 // a wave's registers.
-template <typename T, int DP, int WHAT, int EXTRA>
+template <typename T, int DP, int KG, int WHAT, int EXTRA>
 __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
-  using C = MaskedDkdv<T, DP>;
+  using C = MaskedDkdv<T, DP, KG>;
+  constexpr int KW = C::kKW, kT = C::kT;
   constexpr bool kDv = (WHAT & 1) != 0, kDk = (WHAT & 2) != 0;
   constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
-  __shared__ RowStats stats[2];
+  __shared__ RowStats<kT> stats[C::kBuffers];
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  int const kg = wave / KW, kw = wave % KW;
   int const hb = blockIdx.x % (p.KH * p.B);
   int const kh = hb % p.KH, b = hb / p.KH;
-  int const kv0 = (int)(blockIdx.x / (p.KH * p.B)) * 128;  // under a causal mask the first keys are seen by most rows
-  int const wkv0 = kv0 + wave * 32, kv = wkv0 + (lane & 31);
-  int const nsum = (p.R + 31) / 32;
+  int const kv0 = (int)(blockIdx.x / (p.KH * p.B)) * 32 * KG;  // under a causal mask the first keys are seen by most rows
+  int const wkv0 = kv0 + kg * 32, kv = wkv0 + (lane & 31);
+  int const nsum = (p.R + 31) / 32, nsteps = (nsum + KW - 1) / KW;
   RangeSummary const *sums = p.summary + (int64_t)b * nsum;
 
   T const *kp = static_cast<T const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)min(kv, p.Skv - 1) * p.k_ss + (int64_t)kh * p.Dq;
@@ -258,25 +263,30 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
     }
 
   auto q_tile = [&](int buf) { return reinterpret_cast<T *>(pool + buf * C::kTile); };
-  auto g_tile = [&](int buf) { return q_tile(buf) + 32 * C::kS; };
-  // the next tile at or behind `tile` in which a row sees a key of this workgroup
-  auto next = [&](int tile) {
-    while (tile < nsum) {
-      RangeSummary const s = sums[tile];
-      if (s.lo_min < kv0 + 128 && s.hi_max > kv0) break;
-      tile++;
-    }
-    return tile;
+  auto g_tile = [&](int buf) { return q_tile(buf) + kT * C::kS; };
+  auto seen_by = [&](int tile) {
+    RangeSummary const s = sums[tile];
+    return s.lo_min < kv0 + 32 * KG && s.hi_max > kv0;
   };
-  using Regs = TileRegs<T, DP, 32>;
+  // the next step at or behind `step` in which a row sees a key of this workgroup
+  auto next = [&](int step) {
+    for (; step < nsteps; step++) {
+      bool any = false;
+#pragma unroll
+      for (int w = 0; w < KW; w++) any = any || (step * KW + w < nsum && seen_by(step * KW + w));
+      if (any) break;
+    }
+    return step;
+  };
+  using Regs = TileRegs<T, DP, kT>;
   Regs tq, tg;
   int2 seen[Regs::kN];  // the ranges of this thread's rows: one that sees none of the keys is a row of zeros in LDS
-  float st_lse2, st_delta, st_slope2;
+  float st_lse2, st_delta, st_slope;
   int st_lo, st_hi, st_position;
-  auto fetch = [&](int tile) {
+  auto fetch = [&](int step) {
 #pragma unroll
     for (int n = 0; n < Regs::kN; n++) {
-      int const r = tile * 32 + (t + n * 256) / Regs::kCPR;
+      int const r = step * kT + (t + n * 256) / Regs::kCPR;
       int i, g;
       row_of(p, min(r, p.R - 1), i, g);
       row_range(p, b, i, seen[n].x, seen[n].y);
@@ -284,59 +294,59 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
     }
     auto offset = [&](int r, int64_t seq_stride, int D) {
       int i, g;
-      row_of(p, min(tile * 32 + r, p.R - 1), i, g);
+      row_of(p, min(step * kT + r, p.R - 1), i, g);
       return (int64_t)i * seq_stride + (int64_t)(kh * p.G + g) * D;
     };
     tq.load([&](int r) { return qp + offset(r, p.q_ss, p.Dq); }, p.Dq, t);
     tg.load([&](int r) { return gp + offset(r, p.o_ss, p.Dv); }, p.Dv, t);
-    if (t < 32) {
-      int const r = tile * 32 + t;
+    if (t < kT) {
+      int const r = min(step * kT + t, p.R - 1);
       int i, g;
-      row_of(p, min(r, p.R - 1), i, g);
-      int const head = kh * p.G + g;
+      row_of(p, r, i, g);
       row_range(p, b, i, st_lo, st_hi);
-      if (r >= p.R) st_hi = 0;
+      if (step * kT + t >= p.R) st_hi = 0;
       float const *rows = p.rows + (int64_t)hb * kRowFields * p.padded_rows + r;
       st_lse2 = rows[kRowLse2 * (int64_t)p.padded_rows];
       st_delta = rows[kRowDelta * (int64_t)p.padded_rows];
-      st_slope2 = kBias ? p.slopes[head] * kLog2e : 0.0f;
+      st_slope = kBias ? p.slopes[kh * p.G + g] * p.slope_unit : 0.0f;
       st_position = p.q_offset + i;
     }
   };
   auto stash = [&](int buf) {
 #pragma unroll
     for (int n = 0; n < Regs::kN; n++) {
-      if (!(seen[n].x < kv0 + 128 && seen[n].y > kv0)) {
+      if (!(seen[n].x < kv0 + 32 * KG && seen[n].y > kv0)) {
         tq.r[n] = u32x4{0u, 0u, 0u, 0u};
         tg.r[n] = u32x4{0u, 0u, 0u, 0u};
       }
     }
     tq.store(q_tile(buf), C::kS, t);
     tg.store(g_tile(buf), C::kS, t);
-    if (t < 32) {
+    if (t < kT) {
       stats[buf].lse2[t] = st_lse2;
       stats[buf].delta[t] = st_delta;
-      stats[buf].slope2[t] = st_slope2;
+      stats[buf].slope[t] = st_slope;
       stats[buf].lo[t] = st_lo;
       stats[buf].hi[t] = st_hi;
       stats[buf].position[t] = st_position;
     }
   };
   int const roff = lane_k_off(C::kS, lane), toff = turn_off<T>(C::kS, lane);
-  int tile = next(0);
-  if (tile < nsum) {
-    fetch(tile);
+  int step = next(0);
+  if (step < nsteps) {
+    fetch(step);
     stash(0);
   }
   __syncthreads();
   int cur = 0;
-  while (tile < nsum) {
-    int const after = next(tile + 1);
-    if (after < nsum) fetch(after);
-    RangeSummary const sum = sums[tile];
+  while (step < nsteps) {
+    int const after = next(step + 1);
+    if (after < nsteps) fetch(after);
+    int const tile = step * KW + kw;
+    RangeSummary const sum = tile < nsum ? sums[tile] : RangeSummary{1 << 30, 0, 0, 0};
     if (wkv0 < p.Skv && sum.lo_min < wkv0 + 32 && sum.hi_max > wkv0) {
-      T const *qt = q_tile(cur), *gt = g_tile(cur);
-      RowStats const &rs = stats[cur];
+      T const *qt = q_tile(cur) + kw * 32 * C::kS, *gt = g_tile(cur) + kw * 32 * C::kS;
+      RowStats<kT> const &rs = stats[cur];
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; r++) {
@@ -352,16 +362,15 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
       bool const whole = wkv0 >= sum.lo_max && wkv0 + 32 <= sum.hi_min;
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        int const at = 8 * (r >> 2) + 4 * h32 + (r & 3);
-        float x = s[r] * p.scale_log2, slope = p.scale;
-        if constexpr (kCap) {
-          float const tanh = cap_tanh<T>(p, s[r]);
-          x = p.cap_out * tanh;
-          slope *= 1.0f - tanh * tanh;
+        int const at = kw * 32 + 8 * (r >> 2) + 4 * h32 + (r & 3);
+        float const y = capped<T, kCap>(p, s[r]);
+        float x = y;
+        if constexpr (kBias) x = __builtin_fmaf(-rs.slope[at], (float)abs(rs.position[at] - kv), x);
+        pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -rs.lse2[at]));
+        if constexpr (kDk) {
+          ds[r] = pv[r] * (dp[r] - rs.delta[at]);
+          if constexpr (kCap) ds[r] *= capped_slope<T>(y);
         }
-        if constexpr (kBias) x = __builtin_fmaf(-rs.slope2[at], (float)abs(rs.position[at] - kv), x);
-        pv[r] = __builtin_amdgcn_exp2f(x - rs.lse2[at]);
-        if constexpr (kDk) ds[r] = pv[r] * (dp[r] - rs.delta[at]) * slope;
         if (!whole && (kv < rs.lo[at] || kv >= rs.hi[at])) {
           pv[r] = 0.0f;
           if constexpr (kDk) ds[r] = 0.0f;
@@ -381,26 +390,54 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
         }
       }
     }
-    if (after < nsum) stash(cur ^ 1);
-    __syncthreads();
-    cur ^= 1;
-    tile = after;
+    if constexpr (C::kBuffers == 2) {
+      if (after < nsteps) stash(cur ^ 1);
+      __syncthreads();
+      cur ^= 1;
+    } else {
+      __syncthreads();
+      if (after < nsteps) stash(0);
+      __syncthreads();
+    }
+    step = after;
   }
-  if (kv >= p.Skv) return;
+
+  // the sums of the waves of a group, added up by its first, and written out: a lane owns a key
+  auto finish = [&](f32x16 (&acc)[DP / 32], float factor, T *out, int D) {
+    if constexpr (KW > 1) {
+      float *const area = reinterpret_cast<float *>(pool);
+      __syncthreads();
+      if (kw > 0) {
+        float *to = area + ((kw - 1) * KG + kg) * DP * 32;
 #pragma unroll
-  for (int i = 0; i < DP / 32; i++)
+        for (int i = 0; i < DP / 32; i++)
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-      int const d = i * 32 + 8 * g + 4 * h32;
-      if constexpr (kDk) {
-        T *out = static_cast<T *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kv * p.k_ss + (int64_t)kh * p.Dq;
-        if (d < p.Dq) store4(out + d, dk[i][4 * g], dk[i][4 * g + 1], dk[i][4 * g + 2], dk[i][4 * g + 3]);
+          for (int r = 0; r < 16; r++) to[(i * 16 + r) * 64 + lane] = acc[i][r];
       }
-      if constexpr (kDv) {
-        T *out = static_cast<T *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kv * p.v_ss + (int64_t)kh * p.Dv;
-        if (d < p.Dv) store4(out + d, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
+      __syncthreads();
+      if (kw == 0) {
+#pragma unroll
+        for (int w = 0; w < KW - 1; w++) {
+          float const *from = area + (w * KG + kg) * DP * 32;
+#pragma unroll
+          for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[i][r] += from[(i * 16 + r) * 64 + lane];
+        }
       }
     }
+    if (kw == 0 && kv < p.Skv) {
+#pragma unroll
+      for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          int const d = i * 32 + 8 * g + 4 * h32;
+          if (d < D) store4(out + d, acc[i][4 * g] * factor, acc[i][4 * g + 1] * factor, acc[i][4 * g + 2] * factor, acc[i][4 * g + 3] * factor);
+        }
+    }
+  };
+  if constexpr (kDk) finish(dk, p.grad_scale, static_cast<T *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kv * p.k_ss + (int64_t)kh * p.Dq, p.Dq);
+  if constexpr (kDv) finish(dv, 1.0f, static_cast<T *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kv * p.v_ss + (int64_t)kh * p.Dv, p.Dv);
 }
 
 template <typename T, int DP, int RG, int EXTRA>
@@ -415,34 +452,34 @@ static hipError_t masked_dq_launch_as(hipStream_t st, MaskedAttnParams const &p)
   return hipGetLastError();
 }
 
-template <typename T, int DP, int WHAT, int EXTRA>
+template <typename T, int DP, int KG, int WHAT, int EXTRA>
 static hipError_t masked_dkdv_launch_as(hipStream_t st, MaskedAttnParams const &p) {
   static LdsOptIn opt_in;
-  using C = MaskedDkdv<T, DP>;
-  auto kernel = &masked_dkdv_kernel<T, DP, WHAT, EXTRA>;
+  using C = MaskedDkdv<T, DP, KG>;
+  auto kernel = &masked_dkdv_kernel<T, DP, KG, WHAT, EXTRA>;
   hipError_t e = opt_in.ensure(reinterpret_cast<void const *>(kernel), C::kBytes);
   if (e != hipSuccess) return e;
-  int64_t const grid = ceil_div(p.Skv, 128) * p.KH * p.B;
+  int64_t const grid = ceil_div(p.Skv, 32 * KG) * p.KH * p.B;
   kernel<<<dim3((unsigned)grid), 256, C::kBytes, st>>>(p);
   return hipGetLastError();
 }
 
 template <typename T, int DP, int RG>
 static hipError_t masked_dq_launch(hipStream_t st, MaskedAttnParams const &p) {
-  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
+  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
   return cap && bias ? masked_dq_launch_as<T, DP, RG, 3>(st, p)
          : cap       ? masked_dq_launch_as<T, DP, RG, 1>(st, p)
          : bias      ? masked_dq_launch_as<T, DP, RG, 2>(st, p)
                      : masked_dq_launch_as<T, DP, RG, 0>(st, p);
 }
 
-template <typename T, int DP, int WHAT>
+template <typename T, int DP, int KG, int WHAT>
 static hipError_t masked_dkdv_launch(hipStream_t st, MaskedAttnParams const &p) {
-  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
-  return cap && bias ? masked_dkdv_launch_as<T, DP, WHAT, 3>(st, p)
-         : cap       ? masked_dkdv_launch_as<T, DP, WHAT, 1>(st, p)
-         : bias      ? masked_dkdv_launch_as<T, DP, WHAT, 2>(st, p)
-                     : masked_dkdv_launch_as<T, DP, WHAT, 0>(st, p);
+  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
+  return cap && bias ? masked_dkdv_launch_as<T, DP, KG, WHAT, 3>(st, p)
+         : cap       ? masked_dkdv_launch_as<T, DP, KG, WHAT, 1>(st, p)
+         : bias      ? masked_dkdv_launch_as<T, DP, KG, WHAT, 2>(st, p)
+                     : masked_dkdv_launch_as<T, DP, KG, WHAT, 0>(st, p);
 }
 
 }  // namespace ffk

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
   T const *qp = static_cast<T const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * p.Dq;
   T const *kp = static_cast<T const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * p.Dq;
   T const *vp = static_cast<T const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * p.Dv;
-  float const slope2 = kBias ? p.slopes[head] * kLog2e : 0.0f;
+  float const slope = kBias ? p.slopes[head] * p.slope_unit : 0.0f;
   int const position = p.q_offset + qi;
 
   Frag<T> qf[DP / 16];
@@ -115,17 +115,14 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; kk++) mma(s[j], frag_lds(kt + j * 32 * C::kKS + kk * 16), qf[kk]);
       }
-      // scores in powers of two
+      float const distance = (float)(position - (kv0 + 4 * h32));
 #pragma unroll
-      for (int j = 0; j < J; j++) {
+      for (int j = 0; j < J; j++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          float x = s[j][r];
-          x = kCap ? p.cap_out * cap_tanh<T>(p, x) : x * p.scale_log2;
-          if constexpr (kBias) x = __builtin_fmaf(-slope2, (float)abs(position - (kv0 + j * 32 + 8 * (r >> 2) + 4 * h32 + (r & 3))), x);
-          s[j][r] = x;
+          s[j][r] = capped<T, kCap>(p, s[j][r]);
+          if constexpr (kBias) s[j][r] = __builtin_fmaf(-slope, fabsf(distance - (float)(j * 32 + 8 * (r >> 2) + (r & 3))), s[j][r]);
         }
-      }
       if (kv0 < w_lo_max || kv0 + 32 * J > w_hi_min) {
 #pragma unroll
         for (int j = 0; j < J; j++) {
@@ -141,7 +138,8 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
       for (int j = 0; j < J; j++)
 #pragma unroll
         for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[j][r]);
-      float const m_new = fmaxf(m_run, max_across_halves(mx));
+      // (score_scale is positive, so it commutes with the maximum)
+      float const m_new = fmaxf(m_run, max_across_halves(mx) * p.score_scale);
       float const m_use = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every exponential is 0
       float const alpha = __builtin_amdgcn_exp2f(m_run - m_use);
       float sum = 0.0f;
@@ -151,7 +149,7 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
         float pv[16];
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          pv[r] = __builtin_amdgcn_exp2f(s[j][r] - m_use);
+          pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], p.score_scale, -m_use));
           sum += pv[r];
         }
         pf[2 * j] = frag_acc(pv, vp);
@@ -250,7 +248,7 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
         store4(op + d, oacc[i][4 * g] * inv, oacc[i][4 * g + 1] * inv, oacc[i][4 * g + 2] * inv, oacc[i][4 * g + 3] * inv);
     }
   if (h32 == 0 && p.lse != nullptr)
-    p.lse[((int64_t)b * p.H + head) * p.Sq + qi] = l_run == 0.0f ? -INFINITY : (m_run + __log2f(l_run)) * kLn2;
+    p.lse[((int64_t)b * p.H + head) * p.Sq + qi] = l_run == 0.0f ? -INFINITY : (m_run + p.shift + __log2f(l_run)) * kLn2;
 }
 
 template <typename T, int DP, int RG, int EXTRA>
@@ -267,7 +265,7 @@ static hipError_t masked_fwd_launch_as(hipStream_t st, MaskedAttnParams const &p
 
 template <typename T, int DP, int RG>
 static hipError_t masked_fwd_launch(hipStream_t st, MaskedAttnParams const &p) {
-  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
+  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
   return cap && bias ? masked_fwd_launch_as<T, DP, RG, 3>(st, p)
          : cap       ? masked_fwd_launch_as<T, DP, RG, 1>(st, p)
          : bias      ? masked_fwd_launch_as<T, DP, RG, 2>(st, p)

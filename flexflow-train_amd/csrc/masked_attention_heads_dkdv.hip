@@ -17,7 +17,7 @@
 namespace ffk {
 
 template <int D>
-struct WideDkdv {
+struct HeadsDkdv {
   static constexpr int kKeys = 128, kRows = 64;
   static constexpr int kCPR = D / 8;                // 16-byte chunks of a row
   static constexpr int kLoads = kRows * kCPR / 256; // direct loads of a thread, per tensor and tile
@@ -31,8 +31,8 @@ struct WideDkdv {
 };
 
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void masked_dkdv_wide_kernel(MaskedAttnParams p) {
-  using C = WideDkdv<D>;
+__global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams p) {
+  using C = HeadsDkdv<D>;
   constexpr int NBUF = 3;
   __shared__ __attribute__((aligned(1024))) bf16 Qs[NBUF][C::kTile];
   __shared__ __attribute__((aligned(1024))) bf16 Gs[NBUF][C::kTile];
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void masked_dkdv_wide_kernel(MaskedAttnParams 
   unsigned const unused_addr = lds_address_of(&Unused[0]);
   i32x4 const rq = buffer_resource(qp), rg = buffer_resource(gp);
   i32x4 const rr = buffer_resource(rowp + (int64_t)wave * p.padded_rows);
-  i32x4 const rx = buffer_resource(rowp + (int64_t)(kRowSlope2 + (wave & 1)) * p.padded_rows);
+  i32x4 const rx = buffer_resource(rowp + (int64_t)(kRowSlope + (wave & 1)) * p.padded_rows);
   constexpr int kFields = BIAS ? 6 : 4;
   constexpr int kLoadsPerTile = 2 * C::kLoads + (BIAS ? 2 : 1);
   auto issue_tile = [&](int row0, int buf) {
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void masked_dkdv_wide_kernel(MaskedAttnParams 
     unsigned const at = (unsigned)(row0 + lane) * 4u;  // padded_rows is whole tiles
     lds_dma4(rr, at, 0u, rows_addr + (unsigned)(buf * kFields + wave) * 256u);
     if constexpr (BIAS)
-      lds_dma4(rx, at, 0u, wave >= 2 ? unused_addr : rows_addr + (unsigned)(buf * kFields + kRowSlope2 + wave) * 256u);
+      lds_dma4(rx, at, 0u, wave >= 2 ? unused_addr : rows_addr + (unsigned)(buf * kFields + kRowSlope + wave) * 256u);
   };
 
   // Per-lane LDS offsets (in elements) of the two ways a tile is read (32 rows from its first row on).
@@ -212,22 +212,17 @@ __global__ __launch_bounds__(256) void masked_dkdv_wide_kernel(MaskedAttnParams 
             lrow = *reinterpret_cast<f32x4 const *>(fields + kRowLse2 * 64 + at);
             drow = *reinterpret_cast<f32x4 const *>(fields + kRowDelta * 64 + at);
             if constexpr (BIAS) {
-              srow = *reinterpret_cast<f32x4 const *>(fields + kRowSlope2 * 64 + at);
+              srow = *reinterpret_cast<f32x4 const *>(fields + kRowSlope * 64 + at);
               prow = *reinterpret_cast<i32x4 const *>(fields + kRowPosition * 64 + at);
             }
           }
-          float x, slope = p.scale;
-          if constexpr (CAP) {
-            float const tanh = cap_tanh<bf16>(p, s[u]);
-            x = __builtin_fmaf(p.cap_out, tanh, -lrow[u & 3]);
-            slope = __builtin_fmaf(-tanh * p.scale, tanh, p.scale);
-          } else {
-            x = __builtin_fmaf(s[u], p.scale_log2, -lrow[u & 3]);
-          }
+          float const y = capped<bf16, CAP>(p, s[u]);
+          float x = y;
           if constexpr (BIAS) x = __builtin_fmaf(-srow[u & 3], (float)abs(prow[u & 3] - kvcol), x);
-          float const e = __builtin_amdgcn_exp2f(x);
+          float const e = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lrow[u & 3]));
           pv[h][u] = e;
-          dsv[h][u] = e * ((dp[u] - drow[u & 3]) * slope);
+          dsv[h][u] = e * (dp[u] - drow[u & 3]);
+          if constexpr (CAP) dsv[h][u] *= capped_slope<bf16>(y);
           pin_here(pv[h][u]);
           pin_here(dsv[h][u]);
         };
@@ -351,12 +346,12 @@ __global__ __launch_bounds__(256) void masked_dkdv_wide_kernel(MaskedAttnParams 
   __syncthreads();
   bf16 *const stage = (wave < 2 ? &Qs[0][0] : &Gs[0][0]) + (wave & 1) * 32 * D;
   static_assert(2 * 32 * D <= NBUF * C::kTile, "staging fits the tile buffers");
-  auto write_out = [&](f32x16 const (&acc)[D / 32], bf16 *out, int64_t row_stride) {
+  auto write_out = [&](f32x16 const (&acc)[D / 32], float factor, bf16 *out, int64_t row_stride) {
 #pragma unroll
     for (int i = 0; i < D / 32; i++)
 #pragma unroll
       for (int r = 0; r < 16; r++)
-        VecIO<bf16>::store1(stage + (8 * (r >> 2) + 4 * h32 + (r & 3)) * D + i * 32 + (lane & 31), acc[i][r]);
+        VecIO<bf16>::store1(stage + (8 * (r >> 2) + 4 * h32 + (r & 3)) * D + i * 32 + (lane & 31), acc[i][r] * factor);
     // LDS operations of one wave complete in order: the reads below see the writes above
 #pragma unroll
     for (int k = 0; k < 32 * (D / 8) / 64; k++) {
@@ -366,21 +361,21 @@ __global__ __launch_bounds__(256) void masked_dkdv_wide_kernel(MaskedAttnParams 
       if (wkv0 + row < p.Skv) *reinterpret_cast<u32x4 *>(out + (int64_t)(wkv0 + row) * row_stride + ch * 8) = v;
     }
   };
-  write_out(dk, static_cast<bf16 *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kh * D, p.k_ss);
-  write_out(dv, static_cast<bf16 *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kh * D, p.v_ss);
+  write_out(dk, p.grad_scale, static_cast<bf16 *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kh * D, p.k_ss);
+  write_out(dv, 1.0f, static_cast<bf16 *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kh * D, p.v_ss);
 }
 
 template <int D>
 static void launch(hipStream_t st, MaskedAttnParams const &p) {
   dim3 const grid((unsigned)(ceil_div(p.Skv, 128) * p.KH * p.B));
-  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
-  if (cap && bias) masked_dkdv_wide_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
-  else if (cap) masked_dkdv_wide_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
-  else if (bias) masked_dkdv_wide_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
-  else masked_dkdv_wide_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
+  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
+  if (cap && bias) masked_dkdv_heads_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
+  else if (cap) masked_dkdv_heads_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
+  else if (bias) masked_dkdv_heads_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
+  else masked_dkdv_heads_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
 }
 
-hipError_t masked_attention_dkdv_wide(hipStream_t st, MaskedAttnParams const &p) {
+hipError_t masked_attention_dkdv_heads(hipStream_t st, MaskedAttnParams const &p) {
   if (p.Dq == 64) launch<64>(st, p);
   else launch<128>(st, p);
   return hipGetLastError();

@@ -9,7 +9,7 @@
 namespace ffk {
 
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void masked_dq_wide_kernel(MaskedAttnParams p) {
+__global__ __launch_bounds__(256) void masked_dq_heads_kernel(MaskedAttnParams p) {
   constexpr int kT = 32, kStride = D + 40;  // serves 16-byte and transposing reads
   constexpr int kChunks = kT * D / 8 / 256;
   __shared__ __attribute__((aligned(16))) bf16 Ks[2][kT * kStride];
@@ -49,13 +49,13 @@ __global__ __launch_bounds__(256) void masked_dq_wide_kernel(MaskedAttnParams p)
     for (int e = 0; e < 8; e++) part += (float)of[e] * (float)gf[kk][e];
   }
   float const delta = part + __shfl_xor(part, 32, 64);
-  float const lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + qi] * kLog2e;
-  float slope2 = 0.0f;
-  if constexpr (BIAS) slope2 = p.slopes[head] * kLog2e;
+  float const lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + qi] * kLog2e - p.shift;
+  float slope = 0.0f;
+  if constexpr (BIAS) slope = p.slopes[head] * p.slope_unit;
   int const position = p.q_offset + qi;
 
   int const w_lo_min = wave_min_int(lo), w_hi_max = wave_max_int(hi), w_lo_max = wave_max_int(lo), w_hi_min = wave_min_int(hi);
-  if (h32 == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope2, position);
+  if (h32 == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope, position);
   if (lane == 0) {
     window[0][wave] = w_lo_min;
     window[1][wave] = w_hi_max;
@@ -122,19 +122,15 @@ __global__ __launch_bounds__(256) void masked_dq_wide_kernel(MaskedAttnParams p)
           s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_k(kk_, kStride, 0, kk * 16), qf[kk], s, 0, 0, 0);
           dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_k(vk_, kStride, 0, kk * 16), gf[kk], dp, 0, 0, 0);
         }
+        float const distance = (float)(position - (kt0 + 4 * h32));
         float ds[16];
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          float x, slope = p.scale;
-          if constexpr (CAP) {
-            float const tanh = cap_tanh<bf16>(p, s[r]);
-            x = __builtin_fmaf(p.cap_out, tanh, -lse2);
-            slope = __builtin_fmaf(-tanh * p.scale, tanh, p.scale);
-          } else {
-            x = __builtin_fmaf(s[r], p.scale_log2, -lse2);
-          }
-          if constexpr (BIAS) x = __builtin_fmaf(-slope2, (float)abs(position - (kt0 + 8 * (r >> 2) + 4 * h32 + (r & 3))), x);
-          ds[r] = __builtin_amdgcn_exp2f(x) * ((dp[r] - delta) * slope);
+          float const y = capped<bf16, CAP>(p, s[r]);
+          float x = y;
+          if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
+          ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
+          if constexpr (CAP) ds[r] *= capped_slope<bf16>(y);
         }
         if (kt0 < w_lo_max || kt0 + kT > w_hi_min) {
 #pragma unroll
@@ -168,21 +164,22 @@ __global__ __launch_bounds__(256) void masked_dq_wide_kernel(MaskedAttnParams p)
     for (int i = 0; i < D / 32; i++)
 #pragma unroll
       for (int g = 0; g < 4; g++)
-        store4(dqp + i * 32 + 8 * g + 4 * h32, dq[i][4 * g], dq[i][4 * g + 1], dq[i][4 * g + 2], dq[i][4 * g + 3]);
+        store4(dqp + i * 32 + 8 * g + 4 * h32, dq[i][4 * g] * p.grad_scale, dq[i][4 * g + 1] * p.grad_scale, dq[i][4 * g + 2] * p.grad_scale,
+               dq[i][4 * g + 3] * p.grad_scale);
   }
 }
 
 template <int D>
 static void launch(hipStream_t st, MaskedAttnParams const &p) {
   dim3 const grid((unsigned)(ceil_div(p.R, 128) * p.KH * p.B));
-  bool const cap = p.cap_out != 0.0f, bias = p.slopes != nullptr;
-  if (cap && bias) masked_dq_wide_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
-  else if (cap) masked_dq_wide_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
-  else if (bias) masked_dq_wide_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
-  else masked_dq_wide_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
+  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
+  if (cap && bias) masked_dq_heads_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
+  else if (cap) masked_dq_heads_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
+  else if (bias) masked_dq_heads_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
+  else masked_dq_heads_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
 }
 
-hipError_t masked_attention_dq_wide(hipStream_t st, MaskedAttnParams const &p) {
+hipError_t masked_attention_dq_heads(hipStream_t st, MaskedAttnParams const &p) {
   if (p.Dq == 64) launch<64>(st, p);
   else launch<128>(st, p);
   return hipGetLastError();
