@@ -4,7 +4,10 @@
 // whole kernel next to the accumulators; one wave runs on a SIMD.  It streams the rows of all query heads that read the key
 // head in tiles of 64, two halves of 32: Q, dO and what the dQ kernel left of the rows arrive by direct loads in three LDS
 // buffers, two tiles ahead.  Vector and matrix work overlap inside the wave: the exponentials and dS of one half are cut
-// into units that sit behind the MFMAs of the other half's products, fenced against the scheduler.
+// into units that sit behind the MFMAs of the other half's products, fenced against the scheduler, and every LDS fragment
+// is read a few MFMAs ahead of its use, through the ends of the phases too.  Every MFMA takes a new fragment of 1 KB, so
+// that four of them in 32 cycles ask for all that LDS gives.  The accumulators stay in accumulation registers (mma_kept);
+// everything else, 200 registers of operands, scores and fragments, has the ordinary ones.
 //   Which tiles: a list in LDS of those with a row that sees one of the 128 keys, from the summaries of ranges, made for
 // 512 tiles at a time.  A wave passes over a tile none of whose rows sees its 32 keys, and compares ranges element by
 // element only where not all rows see all of them.  Rows that see none of the 128 keys are cleared in LDS before use: what
@@ -29,6 +32,18 @@ struct HeadsDkdv {
     return D == 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
   }
 };
+
+// acc += a b on an accumulator that stays in accumulation registers: left to itself the compiler keeps some of a wave's
+// 400 values in the wrong kind of register and moves a hundred of them there and back in every tile.  It does not see that
+// results take time: mma_settled has to stand between the last of these and the first use of an accumulator.
+__device__ __forceinline__ void mma_kept(f32x16 &acc, bf16x8 a, bf16x8 b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+template <int N>
+__device__ __forceinline__ void mma_settled(f32x16 (&acc)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("s_nop 15\n\ts_nop 7" : "+a"(acc[i]));
+}
 
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams p) {
@@ -82,15 +97,35 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
   i32x4 const rx = buffer_resource(rowp + (int64_t)(kRowSlope + (wave & 1)) * p.padded_rows);
   constexpr int kFields = BIAS ? 6 : 4;
   constexpr int kLoadsPerTile = 2 * C::kLoads + (BIAS ? 2 : 1);
-  auto issue_tile = [&](int row0, int buf) {
+  // Where G divides 64, a tile's rows lie as its first row's does, and the lanes' offsets inside it never change.
+  bool const even = p.group.d <= 64 && 64 % p.group.d == 0;
+  unsigned q_off[C::kLoads], g_off[C::kLoads];
 #pragma unroll
-    for (int i = 0; i < C::kLoads; i++) {
-      int qi, g;
-      row_of(p, min(row0 + slot_row + i * C::kRowsPerLoad, p.R - 1), qi, g);
-      unsigned const dst = (unsigned)(buf * C::kTile * 2 + (i * 4 + wave) * 1024);
-      unsigned const in_row = (unsigned)(g * D + slot_lc * 8) * 2u;
-      lds_dma16(rq, (unsigned)qi * ((unsigned)p.q_ss * 2u) + in_row, 0u, qs_addr + dst);
-      lds_dma16(rg, (unsigned)qi * ((unsigned)p.o_ss * 2u) + in_row, 0u, gs_addr + dst);
+  for (int i = 0; i < C::kLoads; i++) {
+    int qi, g;
+    row_of(p, slot_row + i * C::kRowsPerLoad, qi, g);
+    q_off[i] = (unsigned)qi * ((unsigned)p.q_ss * 2u) + (unsigned)(g * D + slot_lc * 8) * 2u;
+    g_off[i] = (unsigned)qi * ((unsigned)p.o_ss * 2u) + (unsigned)(g * D + slot_lc * 8) * 2u;
+  }
+  auto issue_tile = [&](int row0, int buf) {
+    unsigned const dst = (unsigned)(buf * C::kTile * 2 + wave * 1024);
+    if (even && row0 + C::kRows <= p.R) {  // uniform
+      unsigned const first = __builtin_amdgcn_readfirstlane(p.group.div((uint32_t)row0));
+      unsigned const q_tile = first * ((unsigned)p.q_ss * 2u), g_tile = first * ((unsigned)p.o_ss * 2u);
+#pragma unroll
+      for (int i = 0; i < C::kLoads; i++) {
+        lds_dma16(rq, q_off[i], q_tile, qs_addr + dst + (unsigned)(i * 4096));
+        lds_dma16(rg, g_off[i], g_tile, gs_addr + dst + (unsigned)(i * 4096));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::kLoads; i++) {
+        int qi, g;
+        row_of(p, min(row0 + slot_row + i * C::kRowsPerLoad, p.R - 1), qi, g);
+        unsigned const in_row = (unsigned)(g * D + slot_lc * 8) * 2u;
+        lds_dma16(rq, (unsigned)qi * ((unsigned)p.q_ss * 2u) + in_row, 0u, qs_addr + dst + (unsigned)(i * 4096));
+        lds_dma16(rg, (unsigned)qi * ((unsigned)p.o_ss * 2u) + in_row, 0u, gs_addr + dst + (unsigned)(i * 4096));
+      }
     }
     unsigned const at = (unsigned)(row0 + lane) * 4u;  // padded_rows is whole tiles
     lds_dma4(rr, at, 0u, rows_addr + (unsigned)(buf * kFields + wave) * 256u);
@@ -121,6 +156,111 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
     u.h2[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tr_off[i][0] + 16 * s * D));
     u.h2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tr_off[i][1] + 16 * s * D));
     return u.v;
+  };
+
+  // One tile that this wave works on; edge (uniform): one whose rows do not all see all of the wave's keys.
+  auto tile_work = [&](bf16 const *qt, bf16 const *gt, float const *fields, bool edge) __attribute__((always_inline)) {
+    constexpr int NM = D / 8;     // MFMAs of a phase
+    constexpr int UPM = 16 / NM;  // units of vector work behind each
+    constexpr int kAhead = 4;     // an LDS fragment is read this many MFMAs ahead of its use
+    constexpr int NI = D / 32;
+    // Fragment n of the tile's 4 NM.  Phases 0 and 1: S = Q K^T and dP = dO V^T of half 0, then 1 (rows = its 32 rows, column =
+    // key): d step m / 2 of Q (m even) or of dO.  Phases 2 and 3: dV += P^T dO and dK += dS^T Q of half 0, then 1: step
+    // m / (2 NI), d block (m / 2) % NI of dO (m even) or of Q.
+    auto fragment = [&](auto nc) __attribute__((always_inline)) -> bf16x8 {
+      constexpr int n = decltype(nc)::value;
+      constexpr int phase = n / NM, m = n % NM, h = phase & 1;
+      if constexpr (phase < 2) return *reinterpret_cast<bf16x8 const *>(((m & 1) ? gt : qt) + h * 32 * D + row_off[m >> 1]);
+      else return turned(((m & 1) ? qt : gt) + h * 32 * D, m / (2 * NI), (m >> 1) % NI);
+    };
+    f32x16 s[2], dp[2];
+    union {
+      uint32_t u[4];
+      bf16x8 v;
+    } pa[2][2], da[2][2];  // P and dS of a half as operands: step s2 takes scores 8 s2 .. + 7
+    // The vector work of a half, 16 units of one score each.  Unit 4 g reads the fields of rows 8 g + 4 (l/32) .. + 3.
+    f32x4 lrow, drow, srow;
+    i32x4 prow;
+    float p_even, ds_even;
+    auto unit = [&](auto hc, auto uc) __attribute__((always_inline)) {
+      constexpr int h = decltype(hc)::value, u = decltype(uc)::value;
+      int const at = h * 32 + 2 * u + 4 * h32;
+      if constexpr ((u & 3) == 0) {
+        lrow = *reinterpret_cast<f32x4 const *>(fields + kRowLse2 * 64 + at);
+        drow = *reinterpret_cast<f32x4 const *>(fields + kRowDelta * 64 + at);
+        if constexpr (BIAS) {
+          srow = *reinterpret_cast<f32x4 const *>(fields + kRowSlope * 64 + at);
+          prow = *reinterpret_cast<i32x4 const *>(fields + kRowPosition * 64 + at);
+        }
+      }
+      float const y = capped<bf16, CAP>(p, s[h][u]);
+      float x = y;
+      if constexpr (BIAS) x = __builtin_fmaf(-srow[u & 3], (float)abs(prow[u & 3] - kvcol), x);
+      float const e = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lrow[u & 3]));
+      float ds = e * (dp[h][u] - drow[u & 3]);
+      if constexpr (CAP) ds *= capped_slope<bf16>(y);
+      if constexpr ((u & 1) == 0) {
+        p_even = e;
+        ds_even = ds;
+        pin_here(p_even);
+        pin_here(ds_even);
+      } else {
+        uint32_t pp = pack_bf16x2(p_even, e), dd = pack_bf16x2(ds_even, ds);
+        asm volatile("" : "+v"(pp), "+v"(dd));
+        pa[h][u >> 3].u[(u & 7) >> 1] = pp;
+        da[h][u >> 3].u[(u & 7) >> 1] = dd;
+      }
+    };
+    // What a row does not see becomes 0 in the finished operands of a half, by their bits: whatever it was.  (A second
+    // instance of the whole tile for the masked ones makes the compiler move the accumulators where the two meet.)
+    auto mask_half = [&](int h) __attribute__((always_inline)) {
+      int const *row_lo = reinterpret_cast<int const *>(fields + kRowLo * 64), *row_hi = reinterpret_cast<int const *>(fields + kRowHi * 64);
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        i32x4 const lo4 = *reinterpret_cast<i32x4 const *>(row_lo + h * 32 + 8 * g + 4 * h32);
+        i32x4 const hi4 = *reinterpret_cast<i32x4 const *>(row_hi + h * 32 + 8 * g + 4 * h32);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          uint32_t const keep = (kvcol < lo4[e] || kvcol >= hi4[e] ? 0u : 0xffffu) | (kvcol < lo4[e + 1] || kvcol >= hi4[e + 1] ? 0u : 0xffff0000u);
+          pa[h][g >> 1].u[2 * (g & 1) + e / 2] &= keep;
+          da[h][g >> 1].u[2 * (g & 1) + e / 2] &= keep;
+        }
+      }
+    };
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        s[h][r] = 0.0f;
+        dp[h][r] = 0.0f;
+      }
+    bf16x8 fr[2 * kAhead];
+    static_for<0, kAhead>([&](auto nc) { fr[decltype(nc)::value] = fragment(nc); });
+    static_for<0, 4 * NM>([&](auto nc) {
+      constexpr int n = decltype(nc)::value;
+      constexpr int phase = n / NM, m = n % NM, h = phase & 1;
+      bf16x8 const f = fr[n % (2 * kAhead)];
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (phase < 2) {
+        if constexpr (m % 2 == 0) s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, kf[m / 2], s[h], 0, 0, 0);
+        else dp[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, vf[m / 2], dp[h], 0, 0, 0);
+      } else {
+        constexpr int s2 = m / (2 * NI), i = (m / 2) % NI;
+        if constexpr (m % 2 == 0) mma_kept(dv[i], pa[h][s2].v, f);
+        else mma_kept(dk[i], da[h][s2].v, f);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (n + kAhead < 4 * NM) fr[(n + kAhead) % (2 * kAhead)] = fragment(std::integral_constant<int, n + kAhead>{});
+      if constexpr (phase == 1 || phase == 2)
+        static_for<0, UPM>([&](auto uc) { unit(std::integral_constant<int, phase - 1>{}, std::integral_constant<int, m * UPM + decltype(uc)::value>{}); });
+      if constexpr ((phase == 1 || phase == 2) && m == NM - 1) {
+        if (edge) {
+          mask_half(phase - 1);
+          asm volatile("s_nop 3");  // the wait states between a vector instruction and mma_kept
+        }
+      }
+    });
+    __builtin_amdgcn_sched_barrier(0);
   };
 
   int const nsum = (p.R + 31) / 32, ntiles = (p.R + 63) / 64;
@@ -162,6 +302,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
     issue_tile(row0_of(0), 0);
     issue_tile(row0_of(min(1, count - 1)), 1);
     int next_row0 = row0_of(min(2, count - 1));
+    int next_tile = list_tile[min(3, count - 1)];
+    RangeSummary sum = list_sum[0];
     // tiles 0 and 1 have landed, and so have the K and V fragments: told to the compiler
     wait_all_vmem_known_to_compiler();
     __syncthreads();
@@ -170,10 +312,12 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
       // buffer (it+2) % 3 was read during step it-1; every wave has passed the barrier that ended it.  Past the end the last
       // tile is fetched again into a buffer nobody reads: the count of loads in flight is the same at every wait.
       issue_tile(next_row0, cur == 0 ? 2 : cur - 1);
-      RangeSummary const sum = list_sum[it];
       int const lo_min = __builtin_amdgcn_readfirstlane(sum.lo_min), hi_max = __builtin_amdgcn_readfirstlane(sum.hi_max);
       int const lo_max = __builtin_amdgcn_readfirstlane(sum.lo_max), hi_min = __builtin_amdgcn_readfirstlane(sum.hi_min);
-      next_row0 = row0_of(min(it + 3, count - 1));
+      // the list's entries of the tiles to come, read a step ahead of their use
+      next_row0 = __builtin_amdgcn_readfirstlane(next_tile) * C::kRows;
+      next_tile = list_tile[min(it + 4, count - 1)];
+      sum = list_sum[min(it + 1, count - 1)];
       bf16 *qt = Qs[cur], *gt = Gs[cur];
       float const *fields = &Rows[cur][0][0];
       int const *row_lo = reinterpret_cast<int const *>(fields + kRowLo * 64), *row_hi = reinterpret_cast<int const *>(fields + kRowHi * 64);
@@ -189,154 +333,14 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
         __syncthreads();
       }
       if (lo_min < wkv0 + 32 && hi_max > wkv0) {
-        bool const edge = lo_max > wkv0 || hi_min < wkv0 + 32;
-        constexpr int NM = D / 8;     // MFMAs of a phase
-        constexpr int UPM = 16 / NM;  // units of vector work behind each
-        constexpr int kAhead = 3;     // an LDS fragment is read this many MFMAs ahead of its use
-        constexpr int NI = D / 32;
-        // S = Q K^T and dP = dO V^T of one half: rows = its 32 rows, column = key; MFMA m: d step m / 2, Q (even) or dO
-        auto sdp_frag = [&](int h, int m) __attribute__((always_inline)) {
-          return *reinterpret_cast<bf16x8 const *>(((m & 1) ? gt : qt) + h * 32 * D + row_off[m >> 1]);
-        };
-        // dV += P^T dO, dK += dS^T Q of one half; MFMA m: step m / (2 NI), d block (m / 2) % NI, dO (even) or Q
-        auto grad_frag = [&](int h, int m) __attribute__((always_inline)) {
-          return turned(((m & 1) ? qt : gt) + h * 32 * D, m / (2 * NI), (m >> 1) % NI);
-        };
-        // The vector work of a half, 16 units of one score each.  Unit 4 g reads the fields of rows 8 g + 4 (l/32) .. + 3.
-        float pv[2][16], dsv[2][16];
-        f32x4 lrow, drow, srow;
-        i32x4 prow;
-        auto unit = [&](int h, int u, f32x16 const &s, f32x16 const &dp) __attribute__((always_inline)) {
-          int const at = h * 32 + 2 * u + 4 * h32;
-          if ((u & 3) == 0) {
-            lrow = *reinterpret_cast<f32x4 const *>(fields + kRowLse2 * 64 + at);
-            drow = *reinterpret_cast<f32x4 const *>(fields + kRowDelta * 64 + at);
-            if constexpr (BIAS) {
-              srow = *reinterpret_cast<f32x4 const *>(fields + kRowSlope * 64 + at);
-              prow = *reinterpret_cast<i32x4 const *>(fields + kRowPosition * 64 + at);
-            }
-          }
-          float const y = capped<bf16, CAP>(p, s[u]);
-          float x = y;
-          if constexpr (BIAS) x = __builtin_fmaf(-srow[u & 3], (float)abs(prow[u & 3] - kvcol), x);
-          float const e = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lrow[u & 3]));
-          pv[h][u] = e;
-          dsv[h][u] = e * (dp[u] - drow[u & 3]);
-          if constexpr (CAP) dsv[h][u] *= capped_slope<bf16>(y);
-          pin_here(pv[h][u]);
-          pin_here(dsv[h][u]);
-        };
-        auto mask_half = [&](int h) {
-#pragma unroll
-          for (int g = 0; g < 4; g++) {
-            i32x4 const lo4 = *reinterpret_cast<i32x4 const *>(row_lo + h * 32 + 8 * g + 4 * h32);
-            i32x4 const hi4 = *reinterpret_cast<i32x4 const *>(row_hi + h * 32 + 8 * g + 4 * h32);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              bool const masked = kvcol < lo4[e] || kvcol >= hi4[e];
-              pv[h][4 * g + e] = masked ? 0.0f : pv[h][4 * g + e];
-              dsv[h][4 * g + e] = masked ? 0.0f : dsv[h][4 * g + e];
-            }
-          }
-        };
-        f32x16 s[2], dp[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            s[h][r] = 0.0f;
-            dp[h][r] = 0.0f;
-          }
-        bf16x8 fr[NM];
-
-        // ---- phase 1: S, dP of half 0 ----
-#pragma unroll
-        for (int m = 0; m < kAhead; m++) fr[m] = sdp_frag(0, m);
-        static_for<0, NM>([&](auto mc) {
-          constexpr int m = decltype(mc)::value;
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m % 2 == 0) {
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[m], kf[m / 2], s[0], 0, 0, 0);
-          } else {
-            dp[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[m], vf[m / 2], dp[0], 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m + kAhead < NM) fr[m + kAhead] = sdp_frag(0, m + kAhead);
-        });
-        __builtin_amdgcn_sched_barrier(0);
-
-        // ---- phase 2: S, dP of half 1 on the matrix pipe, P and dS of half 0 on the vector ALU ----
-        bf16x8 fr2[NM];
-#pragma unroll
-        for (int m = 0; m < kAhead; m++) fr2[m] = sdp_frag(1, m);
-        static_for<0, NM>([&](auto mc) {
-          constexpr int m = decltype(mc)::value;
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m % 2 == 0) {
-            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr2[m], kf[m / 2], s[1], 0, 0, 0);
-          } else {
-            dp[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr2[m], vf[m / 2], dp[1], 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m + kAhead < NM) fr2[m + kAhead] = sdp_frag(1, m + kAhead);
-          static_for<0, UPM>([&](auto uc) { unit(0, m * UPM + decltype(uc)::value, s[0], dp[0]); });
-        });
-        __builtin_amdgcn_sched_barrier(0);
-        if (edge) mask_half(0);
-        bf16x8 pa[2][2], da[2][2];
-#pragma unroll
-        for (int s2 = 0; s2 < 2; s2++) {
-          pa[0][s2] = pack8(pv[0] + 8 * s2);
-          da[0][s2] = pack8(dsv[0] + 8 * s2);
-        }
-
-        // ---- phase 3: dV, dK of half 0 on the matrix pipe, P and dS of half 1 on the vector ALU ----
-        bf16x8 fr3[NM];
-#pragma unroll
-        for (int m = 0; m < kAhead; m++) fr3[m] = grad_frag(0, m);
-        static_for<0, NM>([&](auto mc) {
-          constexpr int m = decltype(mc)::value;
-          constexpr int s2 = m / (2 * NI), i = (m / 2) % NI;
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m % 2 == 0) {
-            dv[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa[0][s2], fr3[m], dv[i], 0, 0, 0);
-          } else {
-            dk[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da[0][s2], fr3[m], dk[i], 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m + kAhead < NM) fr3[m + kAhead] = grad_frag(0, m + kAhead);
-          static_for<0, UPM>([&](auto uc) { unit(1, m * UPM + decltype(uc)::value, s[1], dp[1]); });
-        });
-        __builtin_amdgcn_sched_barrier(0);
-        if (edge) mask_half(1);
-#pragma unroll
-        for (int s2 = 0; s2 < 2; s2++) {
-          pa[1][s2] = pack8(pv[1] + 8 * s2);
-          da[1][s2] = pack8(dsv[1] + 8 * s2);
-        }
-
-        // ---- phase 4: dV, dK of half 1 ----
-        bf16x8 fr4[NM];
-#pragma unroll
-        for (int m = 0; m < kAhead; m++) fr4[m] = grad_frag(1, m);
-        static_for<0, NM>([&](auto mc) {
-          constexpr int m = decltype(mc)::value;
-          constexpr int s2 = m / (2 * NI), i = (m / 2) % NI;
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m % 2 == 0) {
-            dv[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa[1][s2], fr4[m], dv[i], 0, 0, 0);
-          } else {
-            dk[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da[1][s2], fr4[m], dk[i], 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (m + kAhead < NM) fr4[m + kAhead] = grad_frag(1, m + kAhead);
-        });
-        __builtin_amdgcn_sched_barrier(0);
+        tile_work(qt, gt, fields, lo_max > wkv0 || hi_min < wkv0 + 32);
       }
       wait_vmcnt<kLoadsPerTile>();  // this wave's part of the next tile has landed
       __syncthreads();
       cur = cur == 2 ? 0 : cur + 1;
     }
+    mma_settled(dk);
+    mma_settled(dv);
     wait_vmcnt<0>();
     __syncthreads();  // the buffers are free: no load is in flight, no wave reads a tile
   }
