@@ -230,6 +230,21 @@ __device__ __forceinline__ int wave_min_int(int v) {
 }
 __device__ __forceinline__ int wave_max_int(int v) { return -wave_min_int(-v); }
 
+// acc += a b on an accumulator that stays in accumulation registers: left to itself the compiler keeps some of a wave's
+// values in the wrong kind of register and moves them there and back in every tile.  It does not see that results take
+// time: mma_settled has to stand between the last of these and any other use of an accumulator, and four wait states
+// between a vector instruction that writes an operand or an accumulator and the next of these
+// (tests/test_masked_accumulators.py reads the built library for both).
+__device__ __forceinline__ void mma_kept(f32x16 &acc, bf16x8 a, bf16x8 b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+template <int N>
+__device__ __forceinline__ void mma_settled(f32x16 (&acc)[N]) {
+  asm volatile("s_nop 15\n\ts_nop 7" ::);
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+a"(acc[i]));
+}
+
 // Writes 4 consecutive elements.
 __device__ __forceinline__ void store4(bf16 *p, float a, float b, float c, float d) {
   *reinterpret_cast<u32x2 *>(p) = u32x2{pack_bf16x2(a, b), pack_bf16x2(c, d)};

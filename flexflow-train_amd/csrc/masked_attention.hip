@@ -105,11 +105,13 @@ static int padded_head(ffk_masked_attention_desc_t const *d) {
 }
 static int64_t rows_of(ffk_masked_attention_desc_t const *d) { return d->seq_q * (d->heads / d->kv_heads); }
 
+// (FFK_OPTION_ATTENTION_VARIANT other than 0 keeps the kernels for many rows and keys at every size.)
 // 32-row groups of a workgroup: 4, or 1 whose four waves share out the keys, where there are no more rows or workgroups
 // of 128 would leave half of the CUs idle.  (fp32 heads past 128 have no such kernel.)
 static int row_groups(ffk_masked_attention_desc_t const *d, int dtype) {
   if (dtype == FFK_FLOAT && padded_head(d) > 128) return 4;
   int64_t const rows = rows_of(d);
+  if (option(FFK_OPTION_ATTENTION_VARIANT) != 0) return 4;
   return rows <= 32 || (ceil_div(rows, 128) * d->kv_heads * d->batch < kNumCU / 2) ? 1 : 4;
 }
 // Parts of the keys, each a workgroup of its own: where fewer workgroups than CUs would run over long keys.
@@ -215,6 +217,7 @@ static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype) {
 // four waves share out the rows, where workgroups of 128 keys would leave half of the CUs idle.
 static int key_groups(ffk_masked_attention_desc_t const *d) {
   if (padded_head(d) > 128) return 4;  // (no registers left for the rows' tiles)
+  if (option(FFK_OPTION_ATTENTION_VARIANT) != 0) return 4;
   return rows_of(d) > 32 && ceil_div(d->seq_kv, 128) * d->kv_heads * d->batch < kNumCU / 2 ? 1 : 4;
 }
 

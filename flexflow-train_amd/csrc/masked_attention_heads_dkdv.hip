@@ -3,10 +3,10 @@
 // One workgroup owns 128 keys of one key head, 32 to a wave, whose K and V rows are MFMA operands in registers for the
 // whole kernel next to the accumulators; one wave runs on a SIMD.  It streams the rows of all query heads that read the key
 // head in tiles of 64, two halves of 32: Q, dO and what the dQ kernel left of the rows arrive by direct loads in three LDS
-// buffers, two tiles ahead.  Vector and matrix work overlap inside the wave: the exponentials and dS of one half are cut
-// into units that sit behind the MFMAs of the other half's products, fenced against the scheduler, and every LDS fragment
-// is read a few MFMAs ahead of its use, through the ends of the phases too.  Every MFMA takes a new fragment of 1 KB, so
-// that four of them in 32 cycles ask for all that LDS gives.  The accumulators stay in accumulation registers (mma_kept);
+// buffers, two tiles ahead.  Vector and matrix work overlap inside the wave: behind every MFMA sits one step each of a few
+// scores (fenced against the scheduler), and every LDS fragment is read a few MFMAs ahead of its use, through the ends of
+// the phases too.  A vector instruction that needs the one right in front of it waits: a lone wave issues one in 10 cycles
+// then, and one in 6 otherwise, which is why a score takes its steps in different slots.  The accumulators stay in accumulation registers (mma_kept);
 // everything else, 200 registers of operands, scores and fragments, has the ordinary ones.
 //   Which tiles: a list in LDS of those with a row that sees one of the 128 keys, from the summaries of ranges, made for
 // 512 tiles at a time.  A wave passes over a tile none of whose rows sees its 32 keys, and compares ranges element by
@@ -32,18 +32,6 @@ struct HeadsDkdv {
     return D == 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
   }
 };
-
-// acc += a b on an accumulator that stays in accumulation registers: left to itself the compiler keeps some of a wave's
-// 400 values in the wrong kind of register and moves a hundred of them there and back in every tile.  It does not see that
-// results take time: mma_settled has to stand between the last of these and the first use of an accumulator.
-__device__ __forceinline__ void mma_kept(f32x16 &acc, bf16x8 a, bf16x8 b) {
-  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-}
-template <int N>
-__device__ __forceinline__ void mma_settled(f32x16 (&acc)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i++) asm volatile("s_nop 15\n\ts_nop 7" : "+a"(acc[i]));
-}
 
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams p) {
@@ -164,13 +152,13 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
     constexpr int UPM = 16 / NM;  // units of vector work behind each
     constexpr int kAhead = 4;     // an LDS fragment is read this many MFMAs ahead of its use
     constexpr int NI = D / 32;
-    // Fragment n of the tile's 4 NM.  Phases 0 and 1: S = Q K^T and dP = dO V^T of half 0, then 1 (rows = its 32 rows, column =
-    // key): d step m / 2 of Q (m even) or of dO.  Phases 2 and 3: dV += P^T dO and dK += dS^T Q of half 0, then 1: step
-    // m / (2 NI), d block (m / 2) % NI of dO (m even) or of Q.
+    // Fragment n of the tile's 4 NM.  Phases 0 and 1: S = Q K^T, then dP = dO V^T, of half 0, then 1 (rows = its 32 rows,
+    // column = key): d step m of Q, or m - NM / 2 of dO.  Phases 2 and 3: dV += P^T dO and dK += dS^T Q of half 0, then 1:
+    // step m / (2 NI), d block (m / 2) % NI of dO (m even) or of Q.
     auto fragment = [&](auto nc) __attribute__((always_inline)) -> bf16x8 {
       constexpr int n = decltype(nc)::value;
       constexpr int phase = n / NM, m = n % NM, h = phase & 1;
-      if constexpr (phase < 2) return *reinterpret_cast<bf16x8 const *>(((m & 1) ? gt : qt) + h * 32 * D + row_off[m >> 1]);
+      if constexpr (phase < 2) return *reinterpret_cast<bf16x8 const *>((m >= NM / 2 ? gt : qt) + h * 32 * D + row_off[m % (NM / 2)]);
       else return turned(((m & 1) ? qt : gt) + h * 32 * D, m / (2 * NI), (m >> 1) % NI);
     };
     f32x16 s[2], dp[2];
@@ -178,54 +166,64 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
       uint32_t u[4];
       bf16x8 v;
     } pa[2][2], da[2][2];  // P and dS of a half as operands: step s2 takes scores 8 s2 .. + 7
-    // The vector work of a half, 16 units of one score each.  Unit 4 g reads the fields of rows 8 g + 4 (l/32) .. + 3.
-    f32x4 lrow, drow, srow;
-    i32x4 prow;
-    float p_even, ds_even;
-    auto unit = [&](auto hc, auto uc) __attribute__((always_inline)) {
-      constexpr int h = decltype(hc)::value, u = decltype(uc)::value;
-      int const at = h * 32 + 2 * u + 4 * h32;
-      if constexpr ((u & 3) == 0) {
-        lrow = *reinterpret_cast<f32x4 const *>(fields + kRowLse2 * 64 + at);
-        drow = *reinterpret_cast<f32x4 const *>(fields + kRowDelta * 64 + at);
-        if constexpr (BIAS) {
-          srow = *reinterpret_cast<f32x4 const *>(fields + kRowSlope * 64 + at);
-          prow = *reinterpret_cast<i32x4 const *>(fields + kRowPosition * 64 + at);
-        }
-      }
-      float const y = capped<bf16, CAP>(p, s[h][u]);
-      float x = y;
-      if constexpr (BIAS) x = __builtin_fmaf(-srow[u & 3], (float)abs(prow[u & 3] - kvcol), x);
-      float const e = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lrow[u & 3]));
-      float ds = e * (dp[h][u] - drow[u & 3]);
-      if constexpr (CAP) ds *= capped_slope<bf16>(y);
-      if constexpr ((u & 1) == 0) {
-        p_even = e;
-        ds_even = ds;
-        pin_here(p_even);
-        pin_here(ds_even);
-      } else {
-        uint32_t pp = pack_bf16x2(p_even, e), dd = pack_bf16x2(ds_even, ds);
-        asm volatile("" : "+v"(pp), "+v"(dd));
-        pa[h][u >> 3].u[(u & 7) >> 1] = pp;
-        da[h][u >> 3].u[(u & 7) >> 1] = dd;
+    // A score's steps, each of a vector instruction or two that do not need each other; s becomes P and dp becomes dS.
+    f32x4 lrow[2][4], drow[2][4], srow[2][4];
+    i32x4 prow[2][4];
+    float far[2][16], y[2][16];
+    constexpr int kBias = BIAS ? 1 : 0;
+    constexpr int kScore = CAP ? 4 : BIAS ? 2 : 0;  // the step in which a score's y is there
+    constexpr int kPack = D == 64 ? 0 : 1;  // a slot of its own (at two scores a slot there is none left)
+    constexpr int kSteps = kScore + kBias + 3 + kPack;
+    auto step = [&](auto hc, auto uc, auto kc) __attribute__((always_inline)) {
+      constexpr int h = decltype(hc)::value, u = decltype(uc)::value, k = decltype(kc)::value, g = u >> 2, e = u & 3;
+      // the distance beside the first steps
+      if constexpr (BIAS && k == 0) far[h][u] = __builtin_bit_cast(float, prow[h][g][e] - kvcol);
+      if constexpr (BIAS && k == 1) far[h][u] = (float)__builtin_bit_cast(int, far[h][u]);
+      if constexpr (CAP && k == 0) s[h][u] *= p.cap_in;
+      if constexpr (CAP && k == 1) s[h][u] = __builtin_amdgcn_exp2f(s[h][u]);
+      if constexpr (CAP && k == 2) s[h][u] += 1.0f;
+      if constexpr (CAP && k == 3) s[h][u] = -__builtin_amdgcn_rcpf(s[h][u]);  // capped<bf16, true>
+      if constexpr (k == kScore && CAP) y[h][u] = __builtin_fmaf(s[h][u], s[h][u], s[h][u]);  // capped_slope<bf16>
+      if constexpr (k == kScore && BIAS) s[h][u] = __builtin_fmaf(-srow[h][g][e], fabsf(far[h][u]), s[h][u]);
+      if constexpr (k == kScore + kBias) s[h][u] = __builtin_fmaf(s[h][u], p.score_scale, -lrow[h][g][e]);
+      if constexpr (k == kScore + kBias) dp[h][u] -= drow[h][g][e];
+      if constexpr (k == kScore + kBias + 1) s[h][u] = __builtin_amdgcn_exp2f(s[h][u]);
+      if constexpr (k == kScore + kBias + 1 && CAP) dp[h][u] *= y[h][u];
+      if constexpr (k == kScore + kBias + 2) dp[h][u] *= s[h][u];
+      if constexpr (k == kSteps - 1 && (u & 1) == 1) {
+        pa[h][u >> 3].u[(u & 7) >> 1] = pack_bf16x2(s[h][u - 1], s[h][u]);
+        da[h][u >> 3].u[(u & 7) >> 1] = pack_bf16x2(dp[h][u - 1], dp[h][u]);
       }
     };
-    // What a row does not see becomes 0 in the finished operands of a half, by their bits: whatever it was.  (A second
-    // instance of the whole tile for the masked ones makes the compiler move the accumulators where the two meet.)
-    auto mask_half = [&](int h) __attribute__((always_inline)) {
+    // What rows 8 g + 4 (l/32) .. + 3 of a half bring along, four scores' worth.
+    auto read_fields = [&](auto hc, auto gc) __attribute__((always_inline)) {
+      constexpr int h = decltype(hc)::value, g = decltype(gc)::value;
+      int const at = h * 32 + 8 * g + 4 * h32;
+      lrow[h][g] = *reinterpret_cast<f32x4 const *>(fields + kRowLse2 * 64 + at);
+      drow[h][g] = *reinterpret_cast<f32x4 const *>(fields + kRowDelta * 64 + at);
+      if constexpr (BIAS) {
+        srow[h][g] = *reinterpret_cast<f32x4 const *>(fields + kRowSlope * 64 + at);
+        prow[h][g] = *reinterpret_cast<i32x4 const *>(fields + kRowPosition * 64 + at);
+      }
+    };
+    // What a row does not see becomes 0 in the finished operands, by their bits: whatever it was.  (A second instance of the
+    // whole tile for the masked ones makes the compiler move the accumulators where the two meet.)
+    auto mask = [&](auto hc, auto sc) __attribute__((always_inline)) {
+      constexpr int h = decltype(hc)::value, s2 = decltype(sc)::value;
       int const *row_lo = reinterpret_cast<int const *>(fields + kRowLo * 64), *row_hi = reinterpret_cast<int const *>(fields + kRowHi * 64);
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
+      for (int g = 2 * s2; g < 2 * s2 + 2; g++) {
         i32x4 const lo4 = *reinterpret_cast<i32x4 const *>(row_lo + h * 32 + 8 * g + 4 * h32);
         i32x4 const hi4 = *reinterpret_cast<i32x4 const *>(row_hi + h * 32 + 8 * g + 4 * h32);
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           uint32_t const keep = (kvcol < lo4[e] || kvcol >= hi4[e] ? 0u : 0xffffu) | (kvcol < lo4[e + 1] || kvcol >= hi4[e + 1] ? 0u : 0xffff0000u);
-          pa[h][g >> 1].u[2 * (g & 1) + e / 2] &= keep;
-          da[h][g >> 1].u[2 * (g & 1) + e / 2] &= keep;
+          pa[h][s2].u[2 * (g & 1) + e / 2] &= keep;
+          da[h][s2].u[2 * (g & 1) + e / 2] &= keep;
         }
       }
+      // the wait states between a vector instruction and mma_kept
+      asm volatile("s_nop 3" : "+v"(pa[h][s2].v), "+v"(da[h][s2].v));
     };
 #pragma unroll
     for (int h = 0; h < 2; h++)
@@ -234,31 +232,44 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
         s[h][r] = 0.0f;
         dp[h][r] = 0.0f;
       }
-    bf16x8 fr[2 * kAhead];
+    bf16x8 fr[kAhead + 1];
     static_for<0, kAhead>([&](auto nc) { fr[decltype(nc)::value] = fragment(nc); });
     static_for<0, 4 * NM>([&](auto nc) {
       constexpr int n = decltype(nc)::value;
       constexpr int phase = n / NM, m = n % NM, h = phase & 1;
-      bf16x8 const f = fr[n % (2 * kAhead)];
+      // The scores of half h are in steps from slot kFirst + NM h on, UPM of them entering a slot: S is there since slot
+      // NM / 2 - 1 + NM h, and dP, which a score needs kScore + kBias steps on, since slot NM - 1 + NM h.  P and dS of a
+      // half's step s2 are needed from slot (2 + h) NM + s2 NM / 2 on.
+      constexpr int kNeedsDp = NM + 1 - kScore - kBias, kNeedsS = NM / 2 + NM / 8;
+      constexpr int kFirst = kNeedsDp > kNeedsS ? kNeedsDp : kNeedsS;
+      static_assert(kFirst + 15 / UPM + kSteps <= 2 * NM + NM / 2 && kFirst + 7 / UPM + kSteps <= 2 * NM, "operands are ready");
+      if constexpr (phase >= 2 && m % (NM / 2) == 0) {
+        if (edge) mask(std::integral_constant<int, h>{}, std::integral_constant<int, m / (NM / 2)>{});
+      }
+      bf16x8 const f = fr[n % (kAhead + 1)];
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (phase < 2) {
-        if constexpr (m % 2 == 0) s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, kf[m / 2], s[h], 0, 0, 0);
-        else dp[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, vf[m / 2], dp[h], 0, 0, 0);
+        if constexpr (m < NM / 2) s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, kf[m], s[h], 0, 0, 0);
+        else dp[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, vf[m - NM / 2], dp[h], 0, 0, 0);
       } else {
         constexpr int s2 = m / (2 * NI), i = (m / 2) % NI;
         if constexpr (m % 2 == 0) mma_kept(dv[i], pa[h][s2].v, f);
         else mma_kept(dk[i], da[h][s2].v, f);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (n + kAhead < 4 * NM) fr[(n + kAhead) % (2 * kAhead)] = fragment(std::integral_constant<int, n + kAhead>{});
-      if constexpr (phase == 1 || phase == 2)
-        static_for<0, UPM>([&](auto uc) { unit(std::integral_constant<int, phase - 1>{}, std::integral_constant<int, m * UPM + decltype(uc)::value>{}); });
-      if constexpr ((phase == 1 || phase == 2) && m == NM - 1) {
-        if (edge) {
-          mask_half(phase - 1);
-          asm volatile("s_nop 3");  // the wait states between a vector instruction and mma_kept
-        }
-      }
+      if constexpr (n + kAhead < 4 * NM) fr[(n + kAhead) % (kAhead + 1)] = fragment(std::integral_constant<int, n + kAhead>{});
+      static_for<0, 2>([&](auto hc) {
+        // this slot's place in the half's sequence, and the fields of the scores that enter three slots on
+        constexpr int at = n - kFirst - NM * decltype(hc)::value;
+        if constexpr (at + 3 >= 0 && (at + 3) * UPM < 16 && (at + 3) * UPM % 4 == 0)
+          read_fields(hc, std::integral_constant<int, (at + 3) * UPM / 4>{});
+        // the last steps of the oldest scores first
+        static_for<0, kSteps>([&](auto rc) {
+          constexpr int k = kSteps - 1 - decltype(rc)::value;
+          if constexpr (at - k >= 0 && (at - k) * UPM < 16)
+            static_for<0, UPM>([&](auto vc) { step(hc, std::integral_constant<int, (at - k) * UPM + decltype(vc)::value>{}, std::integral_constant<int, k>{}); });
+        });
+      });
     });
     __builtin_amdgcn_sched_barrier(0);
   };

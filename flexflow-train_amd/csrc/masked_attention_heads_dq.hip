@@ -2,18 +2,33 @@
 //
 // One workgroup owns 128 rows of one key head, 32 to a wave, whose Q and dO rows are MFMA operands in registers; two
 // workgroups run on a CU, so that the vector work of one covers the matrix work of the other.  Keys and values come in
-// tiles of 32, through registers into two LDS buffers, two tiles ahead.  Like the general kernel it leaves delta, the
-// log-sum-exp and the ranges of its rows in memory for the dK/dV kernel, and summaries of the ranges.
+// tiles of 64, two halves of 32, by direct loads one tile ahead, and lie in LDS as in memory but for a permutation of the
+// 16-byte chunks of a row that keeps both ways of reading them free of bank conflicts (that of the dK/dV kernel).  Like
+// the general kernel it leaves delta, the log-sum-exp and the ranges of its rows in memory for the dK/dV kernel, and
+// summaries of the ranges.
 #include "masked_attention.h"
+#include "lds_dma.h"
 
 namespace ffk {
 
+template <int D>
+struct HeadsDq {
+  static constexpr int kKeys = 64;
+  static constexpr int kCPR = D / 8;
+  static constexpr int kLoads = kKeys * kCPR / 256;
+  static constexpr int kRowsPerLoad = 256 / kCPR;
+  static constexpr int kTile = kKeys * D;
+  __device__ static int swz(int row) {
+    return D == 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+  }
+  static_assert(D == 64 || D == 128, "permutations are written for these two");
+};
+
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void masked_dq_heads_kernel(MaskedAttnParams p) {
-  constexpr int kT = 32, kStride = D + 40;  // serves 16-byte and transposing reads
-  constexpr int kChunks = kT * D / 8 / 256;
-  __shared__ __attribute__((aligned(16))) bf16 Ks[2][kT * kStride];
-  __shared__ __attribute__((aligned(16))) bf16 Vs[2][kT * kStride];
+__global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParams p) {
+  using C = HeadsDq<D>;
+  __shared__ __attribute__((aligned(1024))) bf16 Ks[2][C::kTile];
+  __shared__ __attribute__((aligned(1024))) bf16 Vs[2][C::kTile];
   __shared__ int window[2][4];
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -36,8 +51,8 @@ __global__ __launch_bounds__(256) void masked_dq_heads_kernel(MaskedAttnParams p
   int64_t const o_at = (int64_t)b * p.o_bs + (int64_t)qi * p.o_ss + (int64_t)head * D;
   bf16 const *qp = static_cast<bf16 const *>(p.q) + q_at, *gp = static_cast<bf16 const *>(p.d_o) + o_at;
   bf16 const *op = static_cast<bf16 const *>(p.o) + o_at;
-  bf16 const *kp = static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * D;
-  bf16 const *vp = static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * D;
+  bf16 const *kp = uniform_pointer(static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * D);
+  bf16 const *vp = uniform_pointer(static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * D);
   bf16x8 qf[D / 16], gf[D / 16];
   float part = 0.0f;
 #pragma unroll
@@ -65,7 +80,7 @@ __global__ __launch_bounds__(256) void masked_dq_heads_kernel(MaskedAttnParams p
   __syncthreads();
   int const lo_all = __builtin_amdgcn_readfirstlane(min(min(window[0][0], window[0][1]), min(window[0][2], window[0][3])));
   int const hi_all = __builtin_amdgcn_readfirstlane(max(max(window[1][0], window[1][1]), max(window[1][2], window[1][3])));
-  int const ntiles = hi_all > lo_all ? (hi_all - lo_all + kT - 1) / kT : 0;
+  int const ntiles = hi_all > lo_all ? (hi_all - lo_all + C::kKeys - 1) / C::kKeys : 0;
 
   f32x16 dq[D / 32];
 #pragma unroll
@@ -73,91 +88,122 @@ __global__ __launch_bounds__(256) void masked_dq_heads_kernel(MaskedAttnParams p
 #pragma unroll
     for (int r = 0; r < 16; r++) dq[i][r] = 0.0f;
 
-  if (ntiles > 0) {
-    u32x4 rk[2][kChunks], rv[2][kChunks];
-    auto gload = [&](int kt0, auto set_tag) {
-      constexpr int R = decltype(set_tag)::value;
+  // Direct loads: thread slot c (of 256 a load) writes LDS chunk c of the load's 4 KB and fetches the chunk that the
+  // permutation puts there.
+  int const slot_row = t / C::kCPR, slot_lc = (t % C::kCPR) ^ C::swz(t / C::kCPR);
+  unsigned const ks_addr = lds_address_of(&Ks[0][0]), vs_addr = lds_address_of(&Vs[0][0]);
+  unsigned k_voff[C::kLoads], v_voff[C::kLoads];  // of a tile that lies wholly below hi_all
 #pragma unroll
-      for (int i = 0; i < kChunks; i++) {
-        int const c = t + i * 256;
-        int const r = c / (D / 8), ch = c % (D / 8);
-        int const gr = min(kt0 + r, hi_all - 1);  // what no row of the workgroup sees is not read
-        rk[R][i] = *reinterpret_cast<u32x4 const *>(kp + (int64_t)gr * p.k_ss + ch * 8);
-        rv[R][i] = *reinterpret_cast<u32x4 const *>(vp + (int64_t)gr * p.v_ss + ch * 8);
-      }
-    };
-    auto lstore = [&](auto set_tag) {
-      constexpr int R = decltype(set_tag)::value;
-#pragma unroll
-      for (int i = 0; i < kChunks; i++) {
-        int const c = t + i * 256;
-        int const r = c / (D / 8), ch = c % (D / 8);
-        *reinterpret_cast<u32x4 *>(&Ks[R][r * kStride + ch * 8]) = rk[R][i];
-        *reinterpret_cast<u32x4 *>(&Vs[R][r * kStride + ch * 8]) = rv[R][i];
-      }
-    };
-    using Set0 = std::integral_constant<int, 0>;
-    using Set1 = std::integral_constant<int, 1>;
-    int const koff = lane_k_off(kStride, lane);
-    int const toff = lane_tr_off(kStride, lane);
-    gload(lo_all, Set0{});
-    lstore(Set0{});
-    gload(lo_all + kT, Set1{});  // unconditional, like every load ahead below: the loop's waits are exact then
-    __syncthreads();
-    auto step = [&](int it, auto parity) {
-      constexpr int cur = decltype(parity)::value;  // == it % 2
-      int const kt0 = lo_all + it * kT;
-      gload(kt0 + 2 * kT, parity);
-      if (it < ntiles && kt0 < w_hi_max && kt0 + kT > w_lo_min) {
-        bf16 const *kk_ = Ks[cur] + koff, *vk_ = Vs[cur] + koff, *ktr = Ks[cur] + toff;
-        // S^T = K Q^T, dP^T = V dO^T: rows = keys of the tile, column = row
-        f32x16 s, dp;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          s[r] = 0.0f;
-          dp[r] = 0.0f;
-        }
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk++) {
-          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_k(kk_, kStride, 0, kk * 16), qf[kk], s, 0, 0, 0);
-          dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_k(vk_, kStride, 0, kk * 16), gf[kk], dp, 0, 0, 0);
-        }
-        float const distance = (float)(position - (kt0 + 4 * h32));
-        float ds[16];
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          float const y = capped<bf16, CAP>(p, s[r]);
-          float x = y;
-          if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
-          ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
-          if constexpr (CAP) ds[r] *= capped_slope<bf16>(y);
-        }
-        if (kt0 < w_lo_max || kt0 + kT > w_hi_min) {
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            int const kv = kt0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
-            ds[r] = kv < lo || kv >= hi ? 0.0f : ds[r];
-          }
-        }
-        // dQ^T += K^T dS^T : A = K^T (rows d) by transposing loads, B = dS^T
-#pragma unroll
-        for (int s2 = 0; s2 < 2; s2++) {
-          bf16x8 const db = pack8(ds + 8 * s2);
-#pragma unroll
-          for (int i = 0; i < D / 32; i++)
-            dq[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_acc(ktr, kStride, 0, s2, i * 32), db, dq[i], 0, 0, 0);
-        }
-      }
-      if (it + 1 < ntiles) lstore(std::integral_constant<int, cur ^ 1>{});
-      __syncthreads();
-    };
-    // in pairs (an odd count runs one idle step)
-    for (int it = 0; it < ntiles; it += 2) {
-      step(it, Set0{});
-      step(it + 1, Set1{});
-    }
+  for (int i = 0; i < C::kLoads; i++) {
+    k_voff[i] = (unsigned)((slot_row + i * C::kRowsPerLoad) * p.k_ss + slot_lc * 8) * 2u;
+    v_voff[i] = (unsigned)((slot_row + i * C::kRowsPerLoad) * p.v_ss + slot_lc * 8) * 2u;
   }
-
+  auto issue_tile = [&](int kv0, int buf) {
+    i32x4 const k_rsrc = buffer_resource(kp + (int64_t)kv0 * p.k_ss);
+    i32x4 const v_rsrc = buffer_resource(vp + (int64_t)kv0 * p.v_ss);
+    unsigned const k_dst = ks_addr + (unsigned)(buf * C::kTile * 2 + wave * 1024);
+    unsigned const v_dst = vs_addr + (unsigned)(buf * C::kTile * 2 + wave * 1024);
+    if (kv0 + C::kKeys > hi_all) {  // uniform
+      // keys past the last one that is seen repeat it: what lies there is not read
+#pragma unroll
+      for (int i = 0; i < C::kLoads; i++) {
+        int const r = min(slot_row + i * C::kRowsPerLoad, hi_all - 1 - kv0);
+        lds_dma16(k_rsrc, (unsigned)(r * p.k_ss + slot_lc * 8) * 2u, 0u, k_dst + (unsigned)(i * 4096));
+        lds_dma16(v_rsrc, (unsigned)(r * p.v_ss + slot_lc * 8) * 2u, 0u, v_dst + (unsigned)(i * 4096));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::kLoads; i++) {
+        lds_dma16(k_rsrc, k_voff[i], 0u, k_dst + (unsigned)(i * 4096));
+        lds_dma16(v_rsrc, v_voff[i], 0u, v_dst + (unsigned)(i * 4096));
+      }
+    }
+  };
+  // Per-lane LDS offsets (in elements) of the two ways a tile is read (32 rows from its first row on).
+  int row_off[D / 16], tr_off[D / 32][2];
+  {
+    int const r = lane & 31;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; kk++) row_off[kk] = r * D + (((2 * kk + h32) ^ C::swz(r)) << 3);
+    int const i16 = lane & 15, q = i16 >> 2, bb = (lane >> 4) & 1, c = i16 & 3;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+#pragma unroll
+      for (int sec = 0; sec < 2; sec++) {
+        int const r2 = 8 * sec + 4 * h32 + q, chunk = 4 * i + 2 * bb + (c >> 1);
+        tr_off[i][sec] = r2 * D + ((chunk ^ C::swz(r2)) << 3) + 4 * (c & 1);
+      }
+  }
+  auto rows = [&](bf16 const *tile, int kk) -> bf16x8 { return *reinterpret_cast<bf16x8 const *>(tile + row_off[kk]); };
+  auto turned = [&](bf16 const *tile, int s, int i) -> bf16x8 {
+    union {
+      s16x4 h2[2];
+      bf16x8 v;
+    } u;
+    u.h2[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tr_off[i][0] + 16 * s * D));
+    u.h2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tr_off[i][1] + 16 * s * D));
+    return u.v;
+  };
+  if (ntiles > 0) issue_tile(lo_all, 0);
+  wait_all_vmem_known_to_compiler();
+  __syncthreads();
+  // 32 keys: S^T = K Q^T, dP^T = V dO^T (rows = keys, column = row), dS, dQ^T += K^T dS^T
+  auto half_work = [&](int kv0, bf16 const *kt, bf16 const *vt) __attribute__((always_inline)) {
+    f32x16 s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      s[r] = 0.0f;
+      dp[r] = 0.0f;
+    }
+#pragma unroll
+    for (int kk = 0; kk < D / 16; kk++) {
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows(kt, kk), qf[kk], s, 0, 0, 0);
+      dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows(vt, kk), gf[kk], dp, 0, 0, 0);
+    }
+    int const kv_first = kv0 + 4 * h32;
+    float const distance = (float)(position - kv_first);
+    float ds[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      float const y = capped<bf16, CAP>(p, s[r]);
+      float x = y;
+      if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
+      ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
+      if constexpr (CAP) ds[r] *= capped_slope<bf16>(y);
+    }
+    if (kv0 < w_lo_max || kv0 + 32 > w_hi_min) {
+      int const from = lo - kv_first, to = hi - kv_first;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        int const kv = 8 * (r >> 2) + (r & 3);
+        ds[r] = kv < from || kv >= to ? 0.0f : ds[r];
+      }
+    }
+    bf16x8 db[2] = {pack8(ds), pack8(ds + 8)};
+    bf16x8 tf[4];  // a fragment is read three MFMAs ahead of its use
+#pragma unroll
+    for (int n = 0; n < 3; n++) tf[n] = turned(kt, n / (D / 32), n % (D / 32));
+#pragma unroll
+    for (int n = 0; n < D / 16; n++) {
+      if (n + 3 < D / 16) tf[(n + 3) % 4] = turned(kt, (n + 3) / (D / 32), (n + 3) % (D / 32));
+      dq[n % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tf[n % 4], db[n / (D / 32)], dq[n % (D / 32)], 0, 0, 0);
+    }
+  };
+  auto tile_step = [&](int it, auto buffer_tag) __attribute__((always_inline)) {
+    constexpr int cur = decltype(buffer_tag)::value;
+    int const kv0 = lo_all + it * C::kKeys;
+    if (it + 1 < ntiles) issue_tile(kv0 + C::kKeys, cur ^ 1);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if (kv0 + 32 * h < w_hi_max && kv0 + 32 * h + 32 > w_lo_min) half_work(kv0 + 32 * h, Ks[cur] + h * 32 * D, Vs[cur] + h * 32 * D);
+    }
+    wait_vmcnt<0>();  // this wave's part of the next tile has landed
+    __syncthreads();
+  };
+  for (int it = 0; it < ntiles; it += 2) {
+    tile_step(it, std::integral_constant<int, 0>{});
+    if (it + 1 < ntiles) tile_step(it + 1, std::integral_constant<int, 1>{});
+  }
   if (row < p.R) {
     bf16 *dqp = static_cast<bf16 *>(p.dq) + q_at;
 #pragma unroll

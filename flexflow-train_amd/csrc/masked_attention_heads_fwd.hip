@@ -139,9 +139,8 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
   if (ntiles > 0) issue_tile(lo_all, 0);
   wait_all_vmem_known_to_compiler();  // the Q fragments too: no wait for them inside the loop
   __syncthreads();
-  // One tile that this wave works on; EDGE: one that is not seen whole by all of its rows.
-  auto tile_work = [&](int kv0, bf16 const *kt, bf16 const *vt, auto edge_tag) __attribute__((always_inline)) {
-    constexpr bool EDGE = decltype(edge_tag)::value;
+  // One tile that this wave works on; edge (uniform): one that is not seen whole by all of its rows.
+  auto tile_work = [&](int kv0, bf16 const *kt, bf16 const *vt, bool edge) __attribute__((always_inline)) {
     f32x16 s[2];
 #pragma unroll
     for (int j = 0; j < 2; j++)
@@ -152,19 +151,29 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
 #pragma unroll
       for (int j = 0; j < 2; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kt, j, kk), qf[kk], s[j], 0, 0, 0);
     int const kv_first = kv0 + 4 * h32;
-    float const distance = (float)(position - kv_first);
-    float mx = -INFINITY;
+    if constexpr (CAP || BIAS) {
+      float const distance = (float)(position - kv_first);
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+      for (int j = 0; j < 2; j++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        int const kv = j * 32 + 8 * (r >> 2) + (r & 3);
-        float y = capped<bf16, CAP>(p, s[j][r]);
-        if constexpr (BIAS) y = __builtin_fmaf(-slope, fabsf(distance - (float)kv), y);
-        if constexpr (EDGE) y = kv < lo - kv_first || kv >= hi - kv_first ? -INFINITY : y;
-        s[j][r] = y;
-        mx = fmaxf(mx, y);
-      }
+        for (int r = 0; r < 16; r++) {
+          s[j][r] = capped<bf16, CAP>(p, s[j][r]);
+          if constexpr (BIAS) s[j][r] = __builtin_fmaf(-slope, fabsf(distance - (float)(j * 32 + 8 * (r >> 2) + (r & 3))), s[j][r]);
+        }
+    }
+    if (edge) {
+      int const from = lo - kv_first, to = hi - kv_first;
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          int const kv = j * 32 + 8 * (r >> 2) + (r & 3);
+          s[j][r] = kv < from || kv >= to ? -INFINITY : s[j][r];
+        }
+    }
+    float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int r = 1; r < 16; r++) mx = fmaxf(fmaxf(mx, s[0][r]), s[1][r]);
     // (score_scale is positive, so it commutes with the maximum.)  The reference point of the exponentials moves only
     // when the maximum has grown by more than kLazy (in powers of two): until then probabilities may exceed 1, by at most
     // 2^kLazy, harmless in 32-bit sums and in bf16's range, and nearly no tile rescales the accumulators.
@@ -175,10 +184,13 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
     if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
       float const alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_use);
       l_part *= alpha;
+      mma_settled(oacc);
 #pragma unroll
       for (int i = 0; i < D / 32; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) oacc[i][r] *= alpha;
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) asm volatile("" : "+a"(oacc[i]));
       m_run = m_new;
     }
     bf16x8 pf[4];
@@ -195,19 +207,22 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
       pf[2 * j + 1] = pack8(pv + 8);
     }
     l_part += sum;
+    bf16x8 vf[4];  // a fragment is read three MFMAs ahead of its use
 #pragma unroll
-    for (int js = 0; js < 4; js++)
+    for (int n = 0; n < 3; n++) vf[n] = v_frag(vt, n / (D / 32), n % (D / 32));
+    asm volatile("s_nop 3" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pf[2]), "+v"(pf[3]));
 #pragma unroll
-      for (int i = 0; i < D / 32; i++)
-        oacc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(vt, js, i), pf[js], oacc[i], 0, 0, 0);
+    for (int n = 0; n < D / 8; n++) {
+      if (n + 3 < D / 8) vf[(n + 3) % 4] = v_frag(vt, (n + 3) / (D / 32), (n + 3) % (D / 32));
+      mma_kept(oacc[n % (D / 32)], vf[n % 4], pf[n / (D / 32)]);
+    }
   };
   auto tile_step = [&](int it, auto buffer_tag) __attribute__((always_inline)) {
     constexpr int cur = decltype(buffer_tag)::value;
     int const kv0 = lo_all + it * C::kKeys;
     if (it + 1 < ntiles) issue_tile(kv0 + C::kKeys, cur ^ 1);
     if (kv0 < w_hi_max && kv0 + C::kKeys > w_lo_min) {
-      if (kv0 < w_lo_max || kv0 + C::kKeys > w_hi_min) tile_work(kv0, Ks[cur], Vs[cur], std::true_type{});
-      else tile_work(kv0, Ks[cur], Vs[cur], std::false_type{});
+      tile_work(kv0, Ks[cur], Vs[cur], kv0 < w_lo_max || kv0 + C::kKeys > w_hi_min);
     }
     wait_vmcnt<0>();  // this wave's part of the next tile has landed
     __syncthreads();
@@ -217,6 +232,7 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
     if (it + 1 < ntiles) tile_step(it + 1, std::integral_constant<int, 1>{});
   }
 
+  mma_settled(oacc);
   float const l = l_part + __shfl_xor(l_part, 32, 64);
   if (row < p.R) {
     float const inv = l == 0.0f ? 0.0f : 1.0f / l;

@@ -144,8 +144,8 @@ int ffk_probe_mfma_bf16(ffk_stream_t stream, int iterations, uint32_t seed,
  *     one kernel per operator.  No other call changes with it.
  *   FFK_OPTION_ATTENTION_VARIANT: which of the two tuned bf16 forward
  *     kernels runs: 0 = 64 query rows per wavefront from 1024 keys on, 32
- *     below; 1 = 32 rows at every size; 2 = 64 rows at every size.  The same
- *     choice for masked attention.                                           */
+ *     below; 1 = 32 rows at every size; 2 = 64 rows at every size.  Either
+ *     also keeps masked attention on its kernels for many rows and keys.     */
 enum {
   FFK_OPTION_GEMM_VARIANT = 0,
   FFK_OPTION_LAYER_UNFUSED = 1,

@@ -106,7 +106,7 @@ def attention(q, k, v, scale, causal=False, cap=0.0, ranges=None, slopes=None, o
     return out
 
 
-def check(got, want, name):
+def check(got, want, name, what=""):
     """`got` within the bound of want[name] everywhere, infinities where they belong."""
     got, ref, tol = got.detach().cpu().double(), want[name], want[name + "_tol"]
     assert got.shape == ref.shape, (name, got.shape, ref.shape)
@@ -117,5 +117,5 @@ def check(got, want, name):
     bad = whole & ~(off <= tol + 1e-30)
     if bad.any():
         at = torch.nonzero(bad)[0].tolist()
-        raise AssertionError("%s: %d of %d values out of bounds, first at %s: %r, wanted %r within %r"
-                             % (name, int(bad.sum()), bad.numel(), at, got[tuple(at)].item(), ref[tuple(at)].item(), tol[tuple(at)].item()))
+        raise AssertionError("%s%s: %d of %d values out of bounds, first at %s: %r, wanted %r within %r"
+                             % (what, name, int(bad.sum()), bad.numel(), at, got[tuple(at)].item(), ref[tuple(at)].item(), tol[tuple(at)].item()))

@@ -34,11 +34,17 @@ def run(ffk, q, k, v, d_o, scale, **how):
 
 
 def compare(ffk, q, k, v, d_o, causal=False, cap=0.0, ranges=None, slopes=None, offset=0):
+    """By the kernels that the size asks for, and by those for many rows and keys."""
     scale = q.shape[3] ** -0.5
-    got = run(ffk, q, k, v, d_o, scale, causal=causal, score_cap=cap, key_ranges=ranges, distance_slopes=slopes, query_offset=offset)
     want = attention(q, k, v, scale, causal, cap, ranges, slopes, offset, d_o, UNIT[q.dtype])
-    for name in ("o", "lse", "dq", "dk", "dv"):
-        check(got[name], want, name)
+    for variant in (1, 0):
+        ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, variant)
+        try:
+            got = run(ffk, q, k, v, d_o, scale, causal=causal, score_cap=cap, key_ranges=ranges, distance_slopes=slopes, query_offset=offset)
+        finally:
+            ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, 0)
+        for name in ("o", "lse", "dq", "dk", "dv"):
+            check(got[name], want, name, "variant %d, " % variant)
     return got
 
 
@@ -149,33 +155,29 @@ def test_given_ranges(ffk, kind, D, dtype):
         assert all(not got[n].any() for n in ("o", "dq", "dk", "dv"))
 
 
-@pytest.mark.parametrize("variant", [1, 2])
 @pytest.mark.parametrize("kind", sorted(RANGES) + ["causal"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("cap,bias", [(0.0, False), (20.0, False), (0.0, True), (5.0, True)])
-def test_both_forward_kernels(ffk, kind, D, cap, bias, variant):
-    """32 and 64 rows to a wave (the size decides otherwise), over every kind of range, with heads that share keys."""
-    say("masked attention, forward variant", variant, kind, D, cap, bias)
+def test_every_kind_of_score(ffk, kind, D, cap, bias):
+    """The kernels of heads of 64 and 128 over every kind of range, with heads that share keys."""
+    say("masked attention", kind, D, cap, bias)
     B, Sq, Skv, H, KH = 2, 210, 290, 6, 2
-    q, k, v, _ = make(D + 2, B, Sq, Skv, H, KH, D, D, BF, 3.0 if cap else 1.0)
+    q, k, v, d_o = make(D + 2, B, Sq, Skv, H, KH, D, D, BF, 3.0 if cap else 1.0)
     ranges = None
     if kind != "causal":
         rows = RANGES[kind](B, Sq, Skv)
         ranges = torch.tensor([rows, rows[::-1]], dtype=torch.int32).cuda()
-    slopes = slopes_of(H) if bias else None
-    ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, variant)
-    try:
-        o, lse = ffk.masked_attention_forward(q, k, v, D ** -0.5, causal=kind == "causal", score_cap=cap, key_ranges=ranges, distance_slopes=slopes)
-        torch.cuda.synchronize()
-    finally:
-        ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, 0)
-    want = attention(q, k, v, D ** -0.5, kind == "causal", cap, ranges, slopes, unit=2.0 ** -8)
-    check(o, want, "o")
-    check(lse, want, "lse")
+    compare(ffk, q, k, v, d_o, causal=kind == "causal", cap=cap, ranges=ranges, slopes=slopes_of(H) if bias else None)
 
 
-def test_forward_kernel_that_the_size_asks_for(ffk):
-    """256 workgroups of 256 rows over more than a thousand keys: 64 rows to a wave by itself."""
+@pytest.mark.parametrize("G", [1, 3, 8])
+def test_heads_that_share_keys(ffk, G):
+    """Row tiles that begin inside a query row's heads (G does not divide 64), and those that do not."""
+    compare(ffk, *make(50 + G, 1, 90, 150, 2 * G, 2, 64, 64, BF), causal=True)
+
+
+def test_kernels_that_the_size_asks_for(ffk):
+    """Workgroups for every CU, so that the kernels for many rows and keys run by themselves."""
     compare(ffk, *make(40, 4, 70, 1030, 64, 64, 64, 64, BF), causal=False, cap=20.0)
 
 
