@@ -136,7 +136,9 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
     u.h2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(q + 8 * D));
     return u.v;
   };
-  if (ntiles > 0) issue_tile(lo_all, 0);
+  // From the last tile to the first: under a causal mask with a bias the largest scores come first then, and the reference
+  // point stays where it is (the other way round it moves in every tile: 8192 tokens, 16 heads of 128, 395 us and 330).
+  if (ntiles > 0) issue_tile(lo_all + (ntiles - 1) * C::kKeys, 0);
   wait_all_vmem_known_to_compiler();  // the Q fragments too: no wait for them inside the loop
   __syncthreads();
   // One tile that this wave works on; edge (uniform): one that is not seen whole by all of its rows.
@@ -219,8 +221,8 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
   };
   auto tile_step = [&](int it, auto buffer_tag) __attribute__((always_inline)) {
     constexpr int cur = decltype(buffer_tag)::value;
-    int const kv0 = lo_all + it * C::kKeys;
-    if (it + 1 < ntiles) issue_tile(kv0 + C::kKeys, cur ^ 1);
+    int const kv0 = lo_all + (ntiles - 1 - it) * C::kKeys;
+    if (it + 1 < ntiles) issue_tile(kv0 - C::kKeys, cur ^ 1);
     if (kv0 < w_hi_max && kv0 + C::kKeys > w_lo_min) {
       tile_work(kv0, Ks[cur], Vs[cur], kv0 < w_lo_max || kv0 + C::kKeys > w_hi_min);
     }
