@@ -12,6 +12,7 @@ The directory name contains a hyphen, so load it with
 (see ``tests/conftest.py``).
 """
 import ctypes
+import functools
 import importlib.util
 import os
 
@@ -785,40 +786,73 @@ def attention_key_ranges(batch, seq_q, seq_kv, causal=False, document_starts=Non
 
 def masked_attention_desc(q, k, v, scale, causal=False, score_cap=0.0, query_offset=0):
     """Descriptor for dense q [B, Sq, H, D], k [B, Skv, KH, D], v [B, Skv, KH, Dv] tensors."""
-    B, Sq, H, D = q.shape
-    _, Skv, KH, _ = k.shape
-    Dv = v.shape[3]
-    if k.shape[0] != B or k.shape[3] != D or tuple(v.shape[:3]) != (B, Skv, KH):
-        raise ValueError("masked attention: q %s, k %s and v %s do not fit each other" % (list(q.shape), list(k.shape), list(v.shape)))
+    return _masked_attention_desc.__wrapped__(q.shape, k.shape, v.shape, scale, causal, score_cap, query_offset)
+
+
+@functools.lru_cache(maxsize=128)  # (the wrappers below share one, and change nothing in it)
+def _masked_attention_desc(q, k, v, scale, causal, score_cap, query_offset):
+    B, Sq, H, D = q
+    _, Skv, KH, _ = k
+    Dv = v[3]
+    if k[0] != B or k[3] != D or tuple(v[:3]) != (B, Skv, KH):
+        raise ValueError("masked attention: q %s, k %s and v %s do not fit each other" % (list(q), list(k), list(v)))
     return MaskedAttentionDesc(B, H, KH, Sq, Skv, D, Dv, Sq * H * D, H * D, Skv * KH * D, KH * D, Skv * KH * Dv, KH * Dv,
                                Sq * H * Dv, H * Dv, query_offset, scale, score_cap, int(causal))
 
 
-def _masked_attention_args(q, k, v, desc, key_ranges, distance_slopes):
+def _reaches(what, t, batch, batch_stride, seq, seq_stride, row):
+    if (batch - 1) * batch_stride + (seq - 1) * seq_stride + row > t.numel():
+        raise ValueError("%s: %d elements do not hold what the descriptor says" % (what, t.numel()))
+
+
+def _masked_attention_reach(desc, q, k, v, outs):
+    """The tensors hold what the descriptor's strides reach."""
+    d, dv = desc, desc.v_head_dim or desc.head_dim
+    for t in q:
+        _reaches("masked attention: q", t, d.batch, d.q_batch_stride, d.seq_q, d.q_seq_stride, d.heads * d.head_dim)
+    for t in k:
+        _reaches("masked attention: k", t, d.batch, d.k_batch_stride, d.seq_kv, d.k_seq_stride, d.kv_heads * d.head_dim)
+    for t in v:
+        _reaches("masked attention: v", t, d.batch, d.v_batch_stride, d.seq_kv, d.v_seq_stride, d.kv_heads * dv)
+    for t in outs:
+        _reaches("masked attention: o", t, d.batch, d.o_batch_stride, d.seq_q, d.o_seq_stride, d.heads * dv)
+
+
+def _masked_attention_args(q, k, v, scale, causal, score_cap, query_offset, desc, key_ranges, distance_slopes):
     torch = _torch()
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("masked attention: q, k and v have one data type")
-    _int32(key_ranges, (desc.batch, desc.seq_q, 2), "key_ranges")
+    if desc is None:
+        desc = _masked_attention_desc(q.shape, k.shape, v.shape, float(scale), bool(causal), float(score_cap), int(query_offset))
+    else:
+        _masked_attention_reach(desc, (q,), (k,), (v,), ())
+    if key_ranges is not None:
+        _int32(key_ranges, (desc.batch, desc.seq_q, 2), "key_ranges")
     if distance_slopes is not None and (distance_slopes.dtype != torch.float32 or distance_slopes.numel() != desc.heads):
         raise ValueError("distance_slopes: float32 [%d] expected" % desc.heads)
+    return desc
 
 
 def masked_attention_forward(q, k, v, scale, causal=False, score_cap=0.0, key_ranges=None, distance_slopes=None,
                              query_offset=0, desc=None, out=None, lse=None, workspace=None):
     """(o, lse).  desc: strides of its own (q, k, v are then the tensors it points into, out the one for o)."""
     torch = _torch()
-    desc = desc or masked_attention_desc(q, k, v, scale, causal, score_cap, query_offset)
-    _masked_attention_args(q, k, v, desc, key_ranges, distance_slopes)
+    d = _masked_attention_args(q, k, v, scale, causal, score_cap, query_offset, desc, key_ranges, distance_slopes)
     if out is None:
-        out = torch.empty((desc.batch, desc.seq_q, desc.heads, desc.v_head_dim or desc.head_dim), dtype=q.dtype, device=q.device)
+        out = torch.empty((d.batch, d.seq_q, d.heads, d.v_head_dim or d.head_dim), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype:
+        raise ValueError("masked attention: out has the data type of q")
     if lse is None:
-        lse = torch.empty((desc.batch, desc.heads, desc.seq_q), dtype=torch.float32, device=q.device)
+        lse = torch.empty((d.batch, d.heads, d.seq_q), dtype=torch.float32, device=q.device)
+    elif lse.dtype != torch.float32 or lse.numel() < d.batch * d.heads * d.seq_q:
+        raise ValueError("masked attention: lse is float32 [%d, %d, %d]" % (d.batch, d.heads, d.seq_q))
+    _masked_attention_reach(d, (), (), (), (out,))
     dtype = dtype_of(q)
     if workspace is None:
-        need = _call.ffk_masked_attention_forward_workspace_bytes(desc, dtype)
+        need = _call.ffk_masked_attention_forward_workspace_bytes(d, dtype)
         if need:
             workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
-    _call.ffk_masked_attention_forward(dtype, desc, q, k, v, key_ranges, distance_slopes, out, lse, workspace,
+    _call.ffk_masked_attention_forward(dtype, d, q, k, v, key_ranges, distance_slopes, out, lse, workspace,
                                        0 if workspace is None else workspace.numel())
     return out, lse
 
@@ -827,26 +861,38 @@ def masked_attention_backward(q, k, v, o, d_o, lse, scale, causal=False, score_c
                               query_offset=0, desc=None, grads=None, workspace=None):
     """(dq, dk, dv), each with the strides of its tensor."""
     torch = _torch()
-    desc = desc or masked_attention_desc(q, k, v, scale, causal, score_cap, query_offset)
-    _masked_attention_args(q, k, v, desc, key_ranges, distance_slopes)
+    d = _masked_attention_args(q, k, v, scale, causal, score_cap, query_offset, desc, key_ranges, distance_slopes)
     if o.dtype != q.dtype or d_o.dtype != q.dtype or lse.dtype != torch.float32:
         raise ValueError("masked attention: o and d_o have the data type of q, lse is float32")
-    dq, dk, dv = grads if grads is not None else (torch.empty_like(q), torch.empty_like(k), torch.empty_like(v))
+    if lse.numel() < d.batch * d.heads * d.seq_q:
+        raise ValueError("masked attention: lse is float32 [%d, %d, %d]" % (d.batch, d.heads, d.seq_q))
+    if grads is None:
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        _masked_attention_reach(d, (), (), (), (o, d_o))
+    else:
+        dq, dk, dv = grads
+        if dq.dtype != q.dtype or dk.dtype != q.dtype or dv.dtype != q.dtype:
+            raise ValueError("masked attention: the gradients have the data type of q")
+        _masked_attention_reach(d, (dq,), (dk,), (dv,), (o, d_o))
     dtype = dtype_of(q)
     if workspace is None:
-        workspace = torch.empty((_call.ffk_masked_attention_backward_workspace_bytes(desc, dtype),), dtype=torch.uint8, device=q.device)
-    _call.ffk_masked_attention_backward(dtype, desc, q, k, v, key_ranges, distance_slopes, o, d_o, lse, dq, dk, dv, workspace,
+        workspace = torch.empty((_call.ffk_masked_attention_backward_workspace_bytes(d, dtype),), dtype=torch.uint8, device=q.device)
+    _call.ffk_masked_attention_backward(dtype, d, q, k, v, key_ranges, distance_slopes, o, d_o, lse, dq, dk, dv, workspace,
                                         workspace.numel())
     return dq, dk, dv
 
 
 def rotary_desc(q, k, sections, interleaved=False):
     """Descriptor for dense q [B, S, H, D], k [B, S, KH, D] (or None) and outputs laid out the same."""
-    B, S, H, D = q.shape
-    KH = 0 if k is None else k.shape[2]
-    if k is not None and (tuple(k.shape[:2]) != (B, S) or k.shape[3] != D):
-        raise ValueError("rotary: q %s and k %s do not fit each other" % (list(q.shape), list(k.shape)))
-    sections = [int(s) for s in sections]
+    return _rotary_desc.__wrapped__(q.shape, None if k is None else k.shape, tuple(int(s) for s in sections), interleaved)
+
+
+@functools.lru_cache(maxsize=128)  # (shared, and changed by none)
+def _rotary_desc(q, k, sections, interleaved):
+    B, S, H, D = q
+    KH = 0 if k is None else k[2]
+    if k is not None and (tuple(k[:2]) != (B, S) or k[3] != D):
+        raise ValueError("rotary: q %s and k %s do not fit each other" % (list(q), list(k)))
     if not 1 <= len(sections) <= 4:
         raise ValueError("rotary: one to four axes, not %d" % len(sections))
     return RotaryDesc(B, S, H, KH, D, S * H * D, H * D, S * KH * D, KH * D, S * H * D, H * D, S * KH * D, KH * D, len(sections),
@@ -855,7 +901,11 @@ def rotary_desc(q, k, sections, interleaved=False):
 
 def _rotary(entry, q, k, positions, frequencies, sections, interleaved, desc, q_out, k_out):
     torch = _torch()
-    desc = desc or rotary_desc(q, k, sections, interleaved)
+    if any(t is not None and t.dtype != q.dtype for t in (k, q_out, k_out)):
+        raise ValueError("rotary: all tensors have one data type")
+    own = q_out is not None or k_out is not None or desc is not None
+    if desc is None:
+        desc = _rotary_desc(q.shape, None if k is None else k.shape, tuple(map(int, sections)), interleaved)
     _int32(positions, (desc.num_axes, desc.batch, desc.seq), "positions")
     if frequencies.dtype != torch.float32 or frequencies.numel() != sum(desc.sections[:desc.num_axes]):
         raise ValueError("frequencies: float32 [%d] expected" % sum(desc.sections[:desc.num_axes]))
@@ -863,8 +913,13 @@ def _rotary(entry, q, k, positions, frequencies, sections, interleaved, desc, q_
         q_out = torch.empty_like(q)
     if k_out is None and k is not None:
         k_out = torch.empty_like(k)
-    if any(t is not None and t.dtype != q.dtype for t in (k, q_out, k_out)):
-        raise ValueError("rotary: all tensors have one data type")
+    if own:
+        d = desc
+        _reaches("rotary: q", q, d.batch, d.q_batch_stride, d.seq, d.q_seq_stride, d.q_heads * d.head_dim)
+        _reaches("rotary: q_out", q_out, d.batch, d.q_out_batch_stride, d.seq, d.q_out_seq_stride, d.q_heads * d.head_dim)
+        if k is not None:
+            _reaches("rotary: k", k, d.batch, d.k_batch_stride, d.seq, d.k_seq_stride, d.k_heads * d.head_dim)
+            _reaches("rotary: k_out", k_out, d.batch, d.k_out_batch_stride, d.seq, d.k_out_seq_stride, d.k_heads * d.head_dim)
     entry(dtype_of(q), desc, q, k, positions, frequencies, q_out, k_out)
     return q_out, k_out
 

@@ -54,6 +54,7 @@ EXTRA_FLAGS = {
     "masked_attention_dkdv_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "masked_attention_dkdv_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "masked_attention_heads_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
+    "masked_attention_heads_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
     "masked_attention_heads_dq.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "masked_attention_heads_dkdv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "optimizer.hip": ["-ffp-contract=off"],

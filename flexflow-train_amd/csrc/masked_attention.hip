@@ -14,6 +14,7 @@ hipError_t masked_attention_dkdv_bf16(hipStream_t st, MaskedAttnParams const &p,
 hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
 // bf16, head sizes 64 and 128: masked_attention_heads_{fwd,dq,dkdv}.hip
 hipError_t masked_attention_fwd_heads(hipStream_t st, MaskedAttnParams const &p);
+hipError_t masked_attention_fwd_rows(hipStream_t st, MaskedAttnParams const &p);  // few rows
 hipError_t masked_attention_dq_heads(hipStream_t st, MaskedAttnParams const &p);
 hipError_t masked_attention_dkdv_heads(hipStream_t st, MaskedAttnParams const &p);
 
@@ -60,33 +61,47 @@ __global__ __launch_bounds__(kRangeThreads) void key_ranges_kernel(int2 *out, in
 // --------------------------------------------------------------------------
 // the parts of the keys, added up
 // --------------------------------------------------------------------------
-// One wave a row: a lane owns up to 4 columns (head sizes to 256), all parts read once.
+// One wave a row.  First the lanes are parts, 64 at a time, for the reference point; then they are columns, up to 4 each
+// (head sizes to 256), and take the parts' rows eight at a time, so that their loads are in flight together.
 template <typename T>
-__global__ __launch_bounds__(256) void masked_merge_kernel(MaskedAttnParams p) {
-  int const lane = threadIdx.x & 63;
-  int64_t const rows = (int64_t)p.B * p.KH * p.R;
-  int64_t const at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= rows) return;
+__global__ __launch_bounds__(64) void masked_merge_kernel(MaskedAttnParams p) {
+  int const lane = threadIdx.x;
+  int64_t const rows = (int64_t)p.B * p.KH * p.R, at = blockIdx.x;
   int const row = (int)(at % p.R), hb = (int)(at / p.R);
   int const kh = hb % p.KH, b = hb / p.KH;
   int i, g;
   row_of(p, row, i, g);
   int const head = kh * p.G + g;
   float m = -INFINITY;
-  for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part_ml[2 * (s * rows + at)]);
+  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_ml[2 * (s * rows + at)]);
+  m = wave_max(m);
   float const m_use = m == -INFINITY ? 0.0f : m;
   int const d = lane * 4;
   float l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.splits; s++) {
-    float const f = __builtin_amdgcn_exp2f(p.part_ml[2 * (s * rows + at)] - m_use);
-    l += p.part_ml[2 * (s * rows + at) + 1] * f;
-    if (d < p.Dv) {
-      f32x4 const x = *reinterpret_cast<f32x4 const *>(p.part_o + (s * rows + at) * p.Dv + d);
+  for (int s0 = 0; s0 < p.splits; s0 += 64) {
+    float f = 0.0f;
+    if (s0 + lane < p.splits) {
+      float const *ml = p.part_ml + 2 * ((s0 + lane) * rows + at);
+      f = __builtin_amdgcn_exp2f(ml[0] - m_use);
+      l += ml[1] * f;
+    }
+    int const n = min(64, p.splits - s0);
+    float const *po = p.part_o + (s0 * rows + at) * p.Dv + (d < p.Dv ? d : 0);
+    for (int s = 0; s < n; s += 8) {
+      f32x4 x[8];
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] += x[e] * f;
+      for (int u = 0; u < 8; u++) x[u] = *reinterpret_cast<f32x4 const *>(po + min(s + u, n - 1) * rows * p.Dv);
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        // past the last part the last is there again, times 0 (its values are finite, or the row's are not)
+        float const fu = s + u < n ? __shfl(f, s + u, 64) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += x[u][e] * fu;
+      }
     }
   }
+  l = wave_sum(l);
   float const inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (d < p.Dv)
     store4(static_cast<T *>(p.o) + (int64_t)b * p.o_bs + (int64_t)i * p.o_ss + (int64_t)head * p.Dv + d, o[0] * inv, o[1] * inv, o[2] * inv,
@@ -114,12 +129,19 @@ static int row_groups(ffk_masked_attention_desc_t const *d, int dtype) {
   if (option(FFK_OPTION_ATTENTION_VARIANT) != 0) return 4;
   return rows <= 32 || (ceil_div(rows, 128) * d->kv_heads * d->batch < kNumCU / 2) ? 1 : 4;
 }
-// Parts of the keys, each a workgroup of its own: where fewer workgroups than CUs would run over long keys.
+static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype);
+// Parts of the keys, each a workgroup of its own, where few workgroups would run over long keys.  In the kernel of one
+// wave a workgroup (masked_attention_heads_rows.hip) ten waves for every CU, each with 256 keys at least: twice what runs at
+// a time, so that sequences of several lengths even out (16 of 4096 to 8192 keys, 8 key heads of 128: 86 us, with five 90);
+// in the general one two workgroups for every CU, each with 512.
 static int key_splits(ffk_masked_attention_desc_t const *d, int dtype) {
-  int64_t const workgroups = ceil_div(rows_of(d), 32 * row_groups(d, dtype)) * d->kv_heads * d->batch;
-  int64_t const most = d->seq_kv / 512;
-  if (workgroups >= kNumCU || most <= 1) return 1;
-  int64_t const want = ceil_div(2 * kNumCU, workgroups);
+  int const groups = row_groups(d, dtype);
+  bool const rows_kernel = groups == 1 && heads_kernels(d, dtype);
+  if (groups == 4 && heads_kernels(d, dtype)) return 1;  // (masked_attention_heads_fwd.hip takes its keys whole)
+  int64_t const workgroups = ceil_div(rows_of(d), 32 * groups) * d->kv_heads * d->batch;
+  int64_t const most = d->seq_kv / (rows_kernel ? 256 : 512), enough = rows_kernel ? 10 * kNumCU : 2 * kNumCU;
+  if (2 * workgroups > enough || most <= 1) return 1;
+  int64_t const want = enough / workgroups;
   return (int)(want < most ? want : most);
 }
 static size_t split_bytes(ffk_masked_attention_desc_t const *d, int splits) {
@@ -206,12 +228,12 @@ static size_t backward_bytes(ffk_masked_attention_desc_t const *d) {
   return row_bytes(d) + (size_t)d->batch * ceil_div(rows_of(d), 32) * sizeof(RangeSummary);
 }
 
-// The kernels of masked_attention_heads_*.hip: bf16, one head size of 64 or 128, rows that 32-bit byte offsets reach (of
-// all rows of an entry in the dK/dV kernel, of a tile in the others).
+// The kernels of masked_attention_heads_*.hip: bf16, head sizes up to 128 (64 and 128 themselves, others made longer with
+// zeros), rows that byte offsets below 2^31 reach (of all rows of an entry in the dK/dV kernel, of a tile in the others).
 static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype) {
-  int64_t const lim = (int64_t)1 << 32;
-  return dtype == FFK_BF16 && (d->head_dim == 64 || d->head_dim == 128) && (d->v_head_dim == 0 || d->v_head_dim == d->head_dim) &&
-         d->k_seq_stride < (1 << 24) && d->v_seq_stride < (1 << 24) && d->seq_q * d->q_seq_stride * 2 < lim && d->seq_q * d->o_seq_stride * 2 < lim;
+  int64_t const lim = (int64_t)1 << 31;
+  return dtype == FFK_BF16 && padded_head(d) <= 128 && d->k_seq_stride < (1 << 24) && d->v_seq_stride < (1 << 24) &&
+         d->seq_q * d->q_seq_stride * 2 < lim && d->seq_q * d->o_seq_stride * 2 < lim;
 }
 // 32-key groups of a workgroup of the general dK/dV kernel, and whether it is to run in place of the one above: 4, or 1 whose
 // four waves share out the rows, where workgroups of 128 keys would leave half of the CUs idle.
@@ -269,16 +291,15 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = p.part_o + (int64_t)splits * p.B * p.KH * p.R * p.Dv;
   }
-  if (row_groups(d, dtype) == 4 && heads_kernels(d, dtype)) {
-    FFK_HIP(masked_attention_fwd_heads(st, p));
-    return FFK_OK;
-  }
-  auto const launch = dtype == FFK_BF16 ? masked_attention_fwd_bf16 : masked_attention_fwd_f32;
-  FFK_HIP(launch(st, p, padded_head(d), row_groups(d, dtype)));
+  int const groups = row_groups(d, dtype);
+  auto const general = dtype == FFK_BF16 ? masked_attention_fwd_bf16 : masked_attention_fwd_f32;
+  if (!heads_kernels(d, dtype)) FFK_HIP(general(st, p, padded_head(d), groups));
+  else if (groups == 4) FFK_HIP(masked_attention_fwd_heads(st, p));
+  else FFK_HIP(masked_attention_fwd_rows(st, p));
   if (p.splits > 1) {
-    dim3 const grid((unsigned)ceil_div((int64_t)p.B * p.KH * p.R, 4));
-    if (dtype == FFK_BF16) masked_merge_kernel<bf16><<<grid, 256, 0, st>>>(p);
-    else masked_merge_kernel<float><<<grid, 256, 0, st>>>(p);
+    dim3 const grid((unsigned)((int64_t)p.B * p.KH * p.R));
+    if (dtype == FFK_BF16) masked_merge_kernel<bf16><<<grid, 64, 0, st>>>(p);
+    else masked_merge_kernel<float><<<grid, 64, 0, st>>>(p);
     FFK_CHECK_LAUNCH();
   }
   return FFK_OK;

@@ -14,8 +14,7 @@
 // lies in them must not meet the zeros of the masked probabilities.
 //   A tile lies in LDS as in memory, [64 rows][D], the 16-byte chunks of a row permuted on the fetching side such that
 // both ways it is read (16 bytes a lane by rows, and turned) are free of bank conflicts.
-#include "masked_attention.h"
-#include "lds_dma.h"
+#include "masked_attention_heads.h"
 
 namespace ffk {
 
@@ -33,7 +32,7 @@ struct HeadsDkdv {
   }
 };
 
-template <int D, bool CAP, bool BIAS>
+template <int D, bool PAD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams p) {
   using C = HeadsDkdv<D>;
   constexpr int NBUF = 3;
@@ -44,16 +43,17 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
   __shared__ int list_tile[C::kList];
   __shared__ RangeSummary list_sum[C::kList];
   __shared__ int wave_count[4];
+  int const dim_qk = PAD ? p.Dq : D, dim_v = PAD ? p.Dv : D;  // the heads themselves
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const hb = blockIdx.x % (p.KH * p.B);
   int const kh = hb % p.KH, b = hb / p.KH;
   int const kv0 = (int)(blockIdx.x / (p.KH * p.B)) * C::kKeys;  // under a causal mask the first keys are seen by most rows
   int const wkv0 = kv0 + wave * 32, kvcol = wkv0 + (lane & 31);
-  bf16 const *qp = static_cast<bf16 const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)kh * p.G * D;
-  bf16 const *gp = static_cast<bf16 const *>(p.d_o) + (int64_t)b * p.o_bs + (int64_t)kh * p.G * D;
-  bf16 const *kp = static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * D;
-  bf16 const *vp = static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * D;
+  bf16 const *qp = static_cast<bf16 const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)kh * p.G * dim_qk;
+  bf16 const *gp = static_cast<bf16 const *>(p.d_o) + (int64_t)b * p.o_bs + (int64_t)kh * p.G * dim_v;
+  bf16 const *kp = static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * dim_qk;
+  bf16 const *vp = static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * dim_v;
   float const *rowp = p.rows + (int64_t)hb * kRowFields * p.padded_rows;
 
   bf16x8 kf[D / 16], vf[D / 16];
@@ -61,8 +61,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
     int const r = min(kvcol, p.Skv - 1);
 #pragma unroll
     for (int kk = 0; kk < D / 16; kk++) {
-      kf[kk] = *reinterpret_cast<bf16x8 const *>(kp + (int64_t)r * p.k_ss + kk * 16 + h32 * 8);
-      vf[kk] = *reinterpret_cast<bf16x8 const *>(vp + (int64_t)r * p.v_ss + kk * 16 + h32 * 8);
+      kf[kk] = head_chunk<PAD>(kp + (int64_t)r * p.k_ss, kk * 16 + h32 * 8, dim_qk);
+      vf[kk] = head_chunk<PAD>(vp + (int64_t)r * p.v_ss, kk * 16 + h32 * 8, dim_v);
     }
   }
   f32x16 dk[D / 32], dv[D / 32];
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
   int const slot_row = t / C::kCPR, slot_lc = (t % C::kCPR) ^ C::swz(t / C::kCPR);
   unsigned const qs_addr = lds_address_of(&Qs[0][0]), gs_addr = lds_address_of(&Gs[0][0]), rows_addr = lds_address_of(&Rows[0][0][0]);
   unsigned const unused_addr = lds_address_of(&Unused[0]);
-  i32x4 const rq = buffer_resource(qp), rg = buffer_resource(gp);
+  i32x4 const rq = tile_resource<PAD>(qp), rg = tile_resource<PAD>(gp);
   i32x4 const rr = buffer_resource(rowp + (int64_t)wave * p.padded_rows);
   i32x4 const rx = buffer_resource(rowp + (int64_t)(kRowSlope + (wave & 1)) * p.padded_rows);
   constexpr int kFields = BIAS ? 6 : 4;
@@ -92,8 +92,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
   for (int i = 0; i < C::kLoads; i++) {
     int qi, g;
     row_of(p, slot_row + i * C::kRowsPerLoad, qi, g);
-    q_off[i] = (unsigned)qi * ((unsigned)p.q_ss * 2u) + (unsigned)(g * D + slot_lc * 8) * 2u;
-    g_off[i] = (unsigned)qi * ((unsigned)p.o_ss * 2u) + (unsigned)(g * D + slot_lc * 8) * 2u;
+    q_off[i] = row_offset<PAD>((unsigned)qi * ((unsigned)p.q_ss * 2u), g, slot_lc * 8, dim_qk);
+    g_off[i] = row_offset<PAD>((unsigned)qi * ((unsigned)p.o_ss * 2u), g, slot_lc * 8, dim_v);
   }
   auto issue_tile = [&](int row0, int buf) {
     unsigned const dst = (unsigned)(buf * C::kTile * 2 + wave * 1024);
@@ -110,9 +110,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
       for (int i = 0; i < C::kLoads; i++) {
         int qi, g;
         row_of(p, min(row0 + slot_row + i * C::kRowsPerLoad, p.R - 1), qi, g);
-        unsigned const in_row = (unsigned)(g * D + slot_lc * 8) * 2u;
-        lds_dma16(rq, (unsigned)qi * ((unsigned)p.q_ss * 2u) + in_row, 0u, qs_addr + dst + (unsigned)(i * 4096));
-        lds_dma16(rg, (unsigned)qi * ((unsigned)p.o_ss * 2u) + in_row, 0u, gs_addr + dst + (unsigned)(i * 4096));
+        lds_dma16(rq, row_offset<PAD>((unsigned)qi * ((unsigned)p.q_ss * 2u), g, slot_lc * 8, dim_qk), 0u, qs_addr + dst + (unsigned)(i * 4096));
+        lds_dma16(rg, row_offset<PAD>((unsigned)qi * ((unsigned)p.o_ss * 2u), g, slot_lc * 8, dim_v), 0u, gs_addr + dst + (unsigned)(i * 4096));
       }
     }
     unsigned const at = (unsigned)(row0 + lane) * 4u;  // padded_rows is whole tiles
@@ -361,7 +360,7 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
   __syncthreads();
   bf16 *const stage = (wave < 2 ? &Qs[0][0] : &Gs[0][0]) + (wave & 1) * 32 * D;
   static_assert(2 * 32 * D <= NBUF * C::kTile, "staging fits the tile buffers");
-  auto write_out = [&](f32x16 const (&acc)[D / 32], float factor, bf16 *out, int64_t row_stride) {
+  auto write_out = [&](f32x16 const (&acc)[D / 32], float factor, bf16 *out, int64_t row_stride, int dim) {
 #pragma unroll
     for (int i = 0; i < D / 32; i++)
 #pragma unroll
@@ -373,26 +372,28 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
       int const c = lane + k * 64;
       int const row = c / (D / 8), ch = c % (D / 8);
       u32x4 const v = *reinterpret_cast<u32x4 const *>(stage + row * D + ch * 8);
-      if (wkv0 + row < p.Skv) *reinterpret_cast<u32x4 *>(out + (int64_t)(wkv0 + row) * row_stride + ch * 8) = v;
+      if (wkv0 + row < p.Skv && (!PAD || ch * 8 < dim)) *reinterpret_cast<u32x4 *>(out + (int64_t)(wkv0 + row) * row_stride + ch * 8) = v;
     }
   };
-  write_out(dk, p.grad_scale, static_cast<bf16 *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kh * D, p.k_ss);
-  write_out(dv, 1.0f, static_cast<bf16 *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kh * D, p.v_ss);
+  write_out(dk, p.grad_scale, static_cast<bf16 *>(p.dk) + (int64_t)b * p.k_bs + (int64_t)kh * dim_qk, p.k_ss, dim_qk);
+  write_out(dv, 1.0f, static_cast<bf16 *>(p.dv) + (int64_t)b * p.v_bs + (int64_t)kh * dim_v, p.v_ss, dim_v);
 }
 
-template <int D>
+template <int D, bool PAD>
 static void launch(hipStream_t st, MaskedAttnParams const &p) {
   dim3 const grid((unsigned)(ceil_div(p.Skv, 128) * p.KH * p.B));
   bool const cap = p.capped != 0, bias = p.slopes != nullptr;
-  if (cap && bias) masked_dkdv_heads_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
-  else if (cap) masked_dkdv_heads_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
-  else if (bias) masked_dkdv_heads_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
-  else masked_dkdv_heads_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
+  if (cap && bias) masked_dkdv_heads_kernel<D, PAD, true, true><<<grid, 256, 0, st>>>(p);
+  else if (cap) masked_dkdv_heads_kernel<D, PAD, true, false><<<grid, 256, 0, st>>>(p);
+  else if (bias) masked_dkdv_heads_kernel<D, PAD, false, true><<<grid, 256, 0, st>>>(p);
+  else masked_dkdv_heads_kernel<D, PAD, false, false><<<grid, 256, 0, st>>>(p);
 }
 
 hipError_t masked_attention_dkdv_heads(hipStream_t st, MaskedAttnParams const &p) {
-  if (p.Dq == 64) launch<64>(st, p);
-  else launch<128>(st, p);
+  if (p.Dq == p.Dv && p.Dq == 64) launch<64, false>(st, p);
+  else if (p.Dq == p.Dv && p.Dq == 128) launch<128, false>(st, p);
+  else if (p.Dq <= 64 && p.Dv <= 64) launch<64, true>(st, p);
+  else launch<128, true>(st, p);
   return hipGetLastError();
 }
 

@@ -6,8 +6,7 @@
 // 16-byte chunks of a row that keeps both ways of reading them free of bank conflicts (that of the dK/dV kernel).  Like
 // the general kernel it leaves delta, the log-sum-exp and the ranges of its rows in memory for the dK/dV kernel, and
 // summaries of the ranges.
-#include "masked_attention.h"
-#include "lds_dma.h"
+#include "masked_attention_heads.h"
 
 namespace ffk {
 
@@ -24,12 +23,13 @@ struct HeadsDq {
   static_assert(D == 64 || D == 128, "permutations are written for these two");
 };
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int U, bool PAD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParams p) {
   using C = HeadsDq<D>;
   __shared__ __attribute__((aligned(1024))) bf16 Ks[2][C::kTile];
   __shared__ __attribute__((aligned(1024))) bf16 Vs[2][C::kTile];
   __shared__ int window[2][4];
+  int const dim_qk = PAD ? p.Dq : D, dim_v = PAD ? p.Dv : D;  // the heads themselves
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const nrb = (p.R + 127) / 128;
@@ -47,19 +47,19 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
     lo = 1 << 30;
     hi = 0;
   }
-  int64_t const q_at = (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * D;
-  int64_t const o_at = (int64_t)b * p.o_bs + (int64_t)qi * p.o_ss + (int64_t)head * D;
+  int64_t const q_at = (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * dim_qk;
+  int64_t const o_at = (int64_t)b * p.o_bs + (int64_t)qi * p.o_ss + (int64_t)head * dim_v;
   bf16 const *qp = static_cast<bf16 const *>(p.q) + q_at, *gp = static_cast<bf16 const *>(p.d_o) + o_at;
   bf16 const *op = static_cast<bf16 const *>(p.o) + o_at;
-  bf16 const *kp = uniform_pointer(static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * D);
-  bf16 const *vp = uniform_pointer(static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * D);
-  bf16x8 qf[D / 16], gf[D / 16];
+  bf16 const *kp = uniform_pointer(static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * dim_qk);
+  bf16 const *vp = uniform_pointer(static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * dim_v);
+  bf16x8 qf[U / 16], gf[U / 16];
   float part = 0.0f;
 #pragma unroll
-  for (int kk = 0; kk < D / 16; kk++) {
-    qf[kk] = *reinterpret_cast<bf16x8 const *>(qp + kk * 16 + h32 * 8);
-    gf[kk] = *reinterpret_cast<bf16x8 const *>(gp + kk * 16 + h32 * 8);
-    bf16x8 const of = *reinterpret_cast<bf16x8 const *>(op + kk * 16 + h32 * 8);
+  for (int kk = 0; kk < U / 16; kk++) {
+    qf[kk] = head_chunk<PAD>(qp, kk * 16 + h32 * 8, dim_qk);
+    gf[kk] = head_chunk<PAD>(gp, kk * 16 + h32 * 8, dim_v);
+    bf16x8 const of = head_chunk<PAD>(op, kk * 16 + h32 * 8, dim_v);
 #pragma unroll
     for (int e = 0; e < 8; e++) part += (float)of[e] * (float)gf[kk][e];
   }
@@ -82,9 +82,9 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
   int const hi_all = __builtin_amdgcn_readfirstlane(max(max(window[1][0], window[1][1]), max(window[1][2], window[1][3])));
   int const ntiles = hi_all > lo_all ? (hi_all - lo_all + C::kKeys - 1) / C::kKeys : 0;
 
-  f32x16 dq[D / 32];
+  f32x16 dq[U / 32];
 #pragma unroll
-  for (int i = 0; i < D / 32; i++)
+  for (int i = 0; i < U / 32; i++)
 #pragma unroll
     for (int r = 0; r < 16; r++) dq[i][r] = 0.0f;
 
@@ -95,12 +95,12 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
   unsigned k_voff[C::kLoads], v_voff[C::kLoads];  // of a tile that lies wholly below hi_all
 #pragma unroll
   for (int i = 0; i < C::kLoads; i++) {
-    k_voff[i] = (unsigned)((slot_row + i * C::kRowsPerLoad) * p.k_ss + slot_lc * 8) * 2u;
-    v_voff[i] = (unsigned)((slot_row + i * C::kRowsPerLoad) * p.v_ss + slot_lc * 8) * 2u;
+    k_voff[i] = tile_offset<PAD>((slot_row + i * C::kRowsPerLoad) * p.k_ss, slot_lc * 8, dim_qk);
+    v_voff[i] = tile_offset<PAD>((slot_row + i * C::kRowsPerLoad) * p.v_ss, slot_lc * 8, dim_v);
   }
   auto issue_tile = [&](int kv0, int buf) {
-    i32x4 const k_rsrc = buffer_resource(kp + (int64_t)kv0 * p.k_ss);
-    i32x4 const v_rsrc = buffer_resource(vp + (int64_t)kv0 * p.v_ss);
+    i32x4 const k_rsrc = tile_resource<PAD>(kp + (int64_t)kv0 * p.k_ss);
+    i32x4 const v_rsrc = tile_resource<PAD>(vp + (int64_t)kv0 * p.v_ss);
     unsigned const k_dst = ks_addr + (unsigned)(buf * C::kTile * 2 + wave * 1024);
     unsigned const v_dst = vs_addr + (unsigned)(buf * C::kTile * 2 + wave * 1024);
     if (kv0 + C::kKeys > hi_all) {  // uniform
@@ -108,8 +108,8 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
 #pragma unroll
       for (int i = 0; i < C::kLoads; i++) {
         int const r = min(slot_row + i * C::kRowsPerLoad, hi_all - 1 - kv0);
-        lds_dma16(k_rsrc, (unsigned)(r * p.k_ss + slot_lc * 8) * 2u, 0u, k_dst + (unsigned)(i * 4096));
-        lds_dma16(v_rsrc, (unsigned)(r * p.v_ss + slot_lc * 8) * 2u, 0u, v_dst + (unsigned)(i * 4096));
+        lds_dma16(k_rsrc, tile_offset<PAD>(r * p.k_ss, slot_lc * 8, dim_qk), 0u, k_dst + (unsigned)(i * 4096));
+        lds_dma16(v_rsrc, tile_offset<PAD>(r * p.v_ss, slot_lc * 8, dim_v), 0u, v_dst + (unsigned)(i * 4096));
       }
     } else {
 #pragma unroll
@@ -120,14 +120,14 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
     }
   };
   // Per-lane LDS offsets (in elements) of the two ways a tile is read (32 rows from its first row on).
-  int row_off[D / 16], tr_off[D / 32][2];
+  int row_off[U / 16], tr_off[U / 32][2];
   {
     int const r = lane & 31;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; kk++) row_off[kk] = r * D + (((2 * kk + h32) ^ C::swz(r)) << 3);
+    for (int kk = 0; kk < U / 16; kk++) row_off[kk] = r * D + (((2 * kk + h32) ^ C::swz(r)) << 3);
     int const i16 = lane & 15, q = i16 >> 2, bb = (lane >> 4) & 1, c = i16 & 3;
 #pragma unroll
-    for (int i = 0; i < D / 32; i++)
+    for (int i = 0; i < U / 32; i++)
 #pragma unroll
       for (int sec = 0; sec < 2; sec++) {
         int const r2 = 8 * sec + 4 * h32 + q, chunk = 4 * i + 2 * bb + (c >> 1);
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
       dp[r] = 0.0f;
     }
 #pragma unroll
-    for (int kk = 0; kk < D / 16; kk++) {
+    for (int kk = 0; kk < U / 16; kk++) {
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows(kt, kk), qf[kk], s, 0, 0, 0);
       dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows(vt, kk), gf[kk], dp, 0, 0, 0);
     }
@@ -182,11 +182,11 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
     bf16x8 db[2] = {pack8(ds), pack8(ds + 8)};
     bf16x8 tf[4];  // a fragment is read three MFMAs ahead of its use
 #pragma unroll
-    for (int n = 0; n < 3; n++) tf[n] = turned(kt, n / (D / 32), n % (D / 32));
+    for (int n = 0; n < 3; n++) tf[n] = turned(kt, n / (U / 32), n % (U / 32));
 #pragma unroll
-    for (int n = 0; n < D / 16; n++) {
-      if (n + 3 < D / 16) tf[(n + 3) % 4] = turned(kt, (n + 3) / (D / 32), (n + 3) % (D / 32));
-      dq[n % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tf[n % 4], db[n / (D / 32)], dq[n % (D / 32)], 0, 0, 0);
+    for (int n = 0; n < U / 16; n++) {
+      if (n + 3 < U / 16) tf[(n + 3) % 4] = turned(kt, (n + 3) / (U / 32), (n + 3) % (U / 32));
+      dq[n % (U / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tf[n % 4], db[n / (U / 32)], dq[n % (U / 32)], 0, 0, 0);
     }
   };
   auto tile_step = [&](int it, auto buffer_tag) __attribute__((always_inline)) {
@@ -207,27 +207,32 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
   if (row < p.R) {
     bf16 *dqp = static_cast<bf16 *>(p.dq) + q_at;
 #pragma unroll
-    for (int i = 0; i < D / 32; i++)
+    for (int i = 0; i < U / 32; i++)
 #pragma unroll
       for (int g = 0; g < 4; g++)
-        store4(dqp + i * 32 + 8 * g + 4 * h32, dq[i][4 * g] * p.grad_scale, dq[i][4 * g + 1] * p.grad_scale, dq[i][4 * g + 2] * p.grad_scale,
-               dq[i][4 * g + 3] * p.grad_scale);
+        if (!PAD || i * 32 + 8 * g + 4 * h32 < dim_qk)
+          store4(dqp + i * 32 + 8 * g + 4 * h32, dq[i][4 * g] * p.grad_scale, dq[i][4 * g + 1] * p.grad_scale, dq[i][4 * g + 2] * p.grad_scale,
+                 dq[i][4 * g + 3] * p.grad_scale);
   }
 }
 
-template <int D>
+template <int D, int U, bool PAD>
 static void launch(hipStream_t st, MaskedAttnParams const &p) {
   dim3 const grid((unsigned)(ceil_div(p.R, 128) * p.KH * p.B));
   bool const cap = p.capped != 0, bias = p.slopes != nullptr;
-  if (cap && bias) masked_dq_heads_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
-  else if (cap) masked_dq_heads_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
-  else if (bias) masked_dq_heads_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
-  else masked_dq_heads_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
+  if (cap && bias) masked_dq_heads_kernel<D, U, PAD, true, true><<<grid, 256, 0, st>>>(p);
+  else if (cap) masked_dq_heads_kernel<D, U, PAD, true, false><<<grid, 256, 0, st>>>(p);
+  else if (bias) masked_dq_heads_kernel<D, U, PAD, false, true><<<grid, 256, 0, st>>>(p);
+  else masked_dq_heads_kernel<D, U, PAD, false, false><<<grid, 256, 0, st>>>(p);
 }
 
 hipError_t masked_attention_dq_heads(hipStream_t st, MaskedAttnParams const &p) {
-  if (p.Dq == 64) launch<64>(st, p);
-  else launch<128>(st, p);
+  int const most = p.Dq > p.Dv ? p.Dq : p.Dv;
+  if (p.Dq == p.Dv && p.Dq == 64) launch<64, 64, false>(st, p);
+  else if (p.Dq == p.Dv && p.Dq == 128) launch<128, 128, false>(st, p);
+  else if (most <= 64) launch<64, 64, true>(st, p);
+  else if (most <= 96) launch<128, 96, true>(st, p);
+  else launch<128, 128, true>(st, p);
   return hipGetLastError();
 }
 

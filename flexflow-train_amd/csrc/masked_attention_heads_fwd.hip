@@ -6,8 +6,7 @@
 // chunks of a row on the fetching side, which keeps both ways of reading them free of bank conflicts.
 //   The loop runs over the union of the rows' ranges.  A wave passes over a tile that none of its rows sees, and ranges
 // are compared element by element only where a tile is not seen whole by all of its rows.
-#include "masked_attention.h"
-#include "lds_dma.h"
+#include "masked_attention_heads.h"
 
 namespace ffk {
 
@@ -23,12 +22,13 @@ struct HeadsFwd {
   static_assert(D == 64 || D == 128, "permutations are written for these two");
 };
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int U, bool PAD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnParams p) {
   using C = HeadsFwd<D>;
   __shared__ __attribute__((aligned(1024))) bf16 Ks[2][C::kTile];
   __shared__ __attribute__((aligned(1024))) bf16 Vs[2][C::kTile];
   __shared__ int window[2][4];
+  int const dim_qk = PAD ? p.Dq : D, dim_v = PAD ? p.Dv : D;  // the heads themselves
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const nrb = (p.R + C::kRows - 1) / C::kRows;
@@ -58,15 +58,15 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
   int const lo_all = __builtin_amdgcn_readfirstlane(min(min(window[0][0], window[0][1]), min(window[0][2], window[0][3])));
   int const hi_all = __builtin_amdgcn_readfirstlane(max(max(window[1][0], window[1][1]), max(window[1][2], window[1][3])));
   int const ntiles = hi_all > lo_all ? (hi_all - lo_all + C::kKeys - 1) / C::kKeys : 0;
-  bf16 const *kp = uniform_pointer(static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * D);
-  bf16 const *vp = uniform_pointer(static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * D);
+  bf16 const *kp = uniform_pointer(static_cast<bf16 const *>(p.k) + (int64_t)b * p.k_bs + (int64_t)kh * dim_qk);
+  bf16 const *vp = uniform_pointer(static_cast<bf16 const *>(p.v) + (int64_t)b * p.v_bs + (int64_t)kh * dim_v);
 
   // Q as the B operand of S^T = K Q^T: column = row, k = d
-  bf16x8 qf[D / 16];
+  bf16x8 qf[U / 16];
   {
-    bf16 const *qp = static_cast<bf16 const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * D;
+    bf16 const *qp = static_cast<bf16 const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * dim_qk;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; kk++) qf[kk] = *reinterpret_cast<bf16x8 const *>(qp + kk * 16 + h32 * 8);
+    for (int kk = 0; kk < U / 16; kk++) qf[kk] = head_chunk<PAD>(qp, kk * 16 + h32 * 8, dim_qk);
   }
 
   // Direct loads: thread slot c (of 256 a load) writes LDS chunk c of the load's 4 KB and fetches the chunk that the
@@ -78,12 +78,12 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
   unsigned k_voff[C::kLoads], v_voff[C::kLoads];  // of a tile that lies wholly below hi_all
 #pragma unroll
   for (int i = 0; i < C::kLoads; i++) {
-    k_voff[i] = (unsigned)((slot_row + i * C::kRowsPerLoad) * p.k_ss + k_lc * 8) * 2u;
-    v_voff[i] = (unsigned)((slot_row + i * C::kRowsPerLoad) * p.v_ss + v_lc * 8) * 2u;
+    k_voff[i] = tile_offset<PAD>((slot_row + i * C::kRowsPerLoad) * p.k_ss, k_lc * 8, dim_qk);
+    v_voff[i] = tile_offset<PAD>((slot_row + i * C::kRowsPerLoad) * p.v_ss, v_lc * 8, dim_v);
   }
   auto issue_tile = [&](int kv0, int buf) {
-    i32x4 const k_rsrc = buffer_resource(kp + (int64_t)kv0 * p.k_ss);
-    i32x4 const v_rsrc = buffer_resource(vp + (int64_t)kv0 * p.v_ss);
+    i32x4 const k_rsrc = tile_resource<PAD>(kp + (int64_t)kv0 * p.k_ss);
+    i32x4 const v_rsrc = tile_resource<PAD>(vp + (int64_t)kv0 * p.v_ss);
     unsigned const k_dst = ks_addr + (unsigned)(buf * C::kTile * 2 + wave * 1024);
     unsigned const v_dst = vs_addr + (unsigned)(buf * C::kTile * 2 + wave * 1024);
     if (kv0 + C::kKeys > hi_all) {  // uniform
@@ -91,12 +91,12 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
 #pragma unroll
       for (int i = 0; i < C::kLoads; i++) {
         int const r = min(slot_row + i * C::kRowsPerLoad, hi_all - 1 - kv0);
-        lds_dma16(k_rsrc, (unsigned)(r * p.k_ss + k_lc * 8) * 2u, 0u, k_dst + (unsigned)(i * 4096));
+        lds_dma16(k_rsrc, tile_offset<PAD>(r * p.k_ss, k_lc * 8, dim_qk), 0u, k_dst + (unsigned)(i * 4096));
       }
 #pragma unroll
       for (int i = 0; i < C::kLoads; i++) {
         int const r = min(slot_row + i * C::kRowsPerLoad, hi_all - 1 - kv0);
-        lds_dma16(v_rsrc, (unsigned)(r * p.v_ss + v_lc * 8) * 2u, 0u, v_dst + (unsigned)(i * 4096));
+        lds_dma16(v_rsrc, tile_offset<PAD>(r * p.v_ss, v_lc * 8, dim_v), 0u, v_dst + (unsigned)(i * 4096));
       }
     } else {
 #pragma unroll
@@ -106,24 +106,24 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
     }
   };
 
-  f32x16 oacc[D / 32];
+  f32x16 oacc[U / 32];
 #pragma unroll
-  for (int i = 0; i < D / 32; i++)
+  for (int i = 0; i < U / 32; i++)
 #pragma unroll
     for (int r = 0; r < 16; r++) oacc[i][r] = 0.0f;
   float m_run = -INFINITY;
   float l_part = 0.0f;  // this lane's 16 of every 32 keys; the two lane halves meet at the end
 
   // K fragment (key block j, d step kk): row j*32 + l%32, chunk (2 kk + l/32) ^ kswz(row)
-  int k_off[D / 16];
+  int k_off[U / 16];
 #pragma unroll
-  for (int kk = 0; kk < D / 16; kk++) k_off[kk] = (lane & 31) * D + (((2 * kk + h32) ^ C::kswz(lane & 31)) << 3);
+  for (int kk = 0; kk < U / 16; kk++) k_off[kk] = (lane & 31) * D + (((2 * kk + h32) ^ C::kswz(lane & 31)) << 3);
   // V fragment (d block i): rows 4 (l/32) + (l%16)/4 (+ 8) of a 16-row step, 4 columns at 16 ((l/16)%2) + 4 (l%4)
-  int v_off[D / 32];
+  int v_off[U / 32];
   {
     int const i16 = lane & 15, lr = 4 * h32 + (i16 >> 2);
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) v_off[i] = lr * D + ((i ^ C::vswz(lr)) << 5) + ((lane >> 4) & 1) * 16 + (i16 & 3) * 4;
+    for (int i = 0; i < U / 32; i++) v_off[i] = lr * D + ((i ^ C::vswz(lr)) << 5) + ((lane >> 4) & 1) * 16 + (i16 & 3) * 4;
   }
   auto k_frag = [&](bf16 const *tile, int j, int kk) -> bf16x8 { return *reinterpret_cast<bf16x8 const *>(tile + k_off[kk] + j * 32 * D); };
   auto v_frag = [&](bf16 const *tile, int js, int i) -> bf16x8 {
@@ -136,9 +136,12 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
     u.h2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(q + 8 * D));
     return u.v;
   };
-  // From the last tile to the first: under a causal mask with a bias the largest scores come first then, and the reference
+  // With a bias from the last tile to the first: under a causal mask the largest scores come first then, and the reference
   // point stays where it is (the other way round it moves in every tile: 8192 tokens, 16 heads of 128, 395 us and 330).
-  if (ntiles > 0) issue_tile(lo_all + (ntiles - 1) * C::kKeys, 0);
+  // Without one from the first: the workgroups of a head read the same keys at about the same time (4 sequences of 4096 in
+  // 3 documents each, 32 heads on 8 of 128, a cap: 374 us, the other way round 396).
+  auto tile_at = [&](int it) { return lo_all + (BIAS ? ntiles - 1 - it : it) * C::kKeys; };
+  if (ntiles > 0) issue_tile(tile_at(0), 0);
   wait_all_vmem_known_to_compiler();  // the Q fragments too: no wait for them inside the loop
   __syncthreads();
   // One tile that this wave works on; edge (uniform): one that is not seen whole by all of its rows.
@@ -149,7 +152,7 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
 #pragma unroll
       for (int r = 0; r < 16; r++) s[j][r] = 0.0f;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; kk++)
+    for (int kk = 0; kk < U / 16; kk++)
 #pragma unroll
       for (int j = 0; j < 2; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kt, j, kk), qf[kk], s[j], 0, 0, 0);
     int const kv_first = kv0 + 4 * h32;
@@ -188,11 +191,11 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
       l_part *= alpha;
       mma_settled(oacc);
 #pragma unroll
-      for (int i = 0; i < D / 32; i++)
+      for (int i = 0; i < U / 32; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) oacc[i][r] *= alpha;
 #pragma unroll
-      for (int i = 0; i < D / 32; i++) asm volatile("" : "+a"(oacc[i]));
+      for (int i = 0; i < U / 32; i++) asm volatile("" : "+a"(oacc[i]));
       m_run = m_new;
     }
     bf16x8 pf[4];
@@ -211,18 +214,18 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
     l_part += sum;
     bf16x8 vf[4];  // a fragment is read three MFMAs ahead of its use
 #pragma unroll
-    for (int n = 0; n < 3; n++) vf[n] = v_frag(vt, n / (D / 32), n % (D / 32));
+    for (int n = 0; n < 3; n++) vf[n] = v_frag(vt, n / (U / 32), n % (U / 32));
     asm volatile("s_nop 3" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pf[2]), "+v"(pf[3]));
 #pragma unroll
-    for (int n = 0; n < D / 8; n++) {
-      if (n + 3 < D / 8) vf[(n + 3) % 4] = v_frag(vt, (n + 3) / (D / 32), (n + 3) % (D / 32));
-      mma_kept(oacc[n % (D / 32)], vf[n % 4], pf[n / (D / 32)]);
+    for (int n = 0; n < U / 8; n++) {
+      if (n + 3 < U / 8) vf[(n + 3) % 4] = v_frag(vt, (n + 3) / (U / 32), (n + 3) % (U / 32));
+      mma_kept(oacc[n % (U / 32)], vf[n % 4], pf[n / (U / 32)]);
     }
   };
   auto tile_step = [&](int it, auto buffer_tag) __attribute__((always_inline)) {
     constexpr int cur = decltype(buffer_tag)::value;
-    int const kv0 = lo_all + (ntiles - 1 - it) * C::kKeys;
-    if (it + 1 < ntiles) issue_tile(kv0 - C::kKeys, cur ^ 1);
+    int const kv0 = tile_at(it);
+    if (it + 1 < ntiles) issue_tile(tile_at(it + 1), cur ^ 1);
     if (kv0 < w_hi_max && kv0 + C::kKeys > w_lo_min) {
       tile_work(kv0, Ks[cur], Vs[cur], kv0 < w_lo_max || kv0 + C::kKeys > w_hi_min);
     }
@@ -238,30 +241,36 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
   float const l = l_part + __shfl_xor(l_part, 32, 64);
   if (row < p.R) {
     float const inv = l == 0.0f ? 0.0f : 1.0f / l;
-    bf16 *op = static_cast<bf16 *>(p.o) + (int64_t)b * p.o_bs + (int64_t)qi * p.o_ss + (int64_t)head * D;
+    bf16 *op = static_cast<bf16 *>(p.o) + (int64_t)b * p.o_bs + (int64_t)qi * p.o_ss + (int64_t)head * dim_v;
 #pragma unroll
-    for (int i = 0; i < D / 32; i++)
+    for (int i = 0; i < U / 32; i++)
 #pragma unroll
       for (int g = 0; g < 4; g++)
-        store4(op + i * 32 + 8 * g + 4 * h32, oacc[i][4 * g] * inv, oacc[i][4 * g + 1] * inv, oacc[i][4 * g + 2] * inv, oacc[i][4 * g + 3] * inv);
+        if (!PAD || i * 32 + 8 * g + 4 * h32 < dim_v)
+          store4(op + i * 32 + 8 * g + 4 * h32, oacc[i][4 * g] * inv, oacc[i][4 * g + 1] * inv, oacc[i][4 * g + 2] * inv,
+                 oacc[i][4 * g + 3] * inv);
     if (h32 == 0 && p.lse != nullptr)
       p.lse[((int64_t)b * p.H + head) * p.Sq + qi] = l == 0.0f ? -INFINITY : (m_run + p.shift + __log2f(l)) * kLn2;
   }
 }
 
-template <int D>
+template <int D, int U, bool PAD>
 static void launch(hipStream_t st, MaskedAttnParams const &p) {
   dim3 const grid((unsigned)(ceil_div(p.R, HeadsFwd<D>::kRows) * p.KH * p.B));
   bool const cap = p.capped != 0, bias = p.slopes != nullptr;
-  if (cap && bias) masked_fwd_heads_kernel<D, true, true><<<grid, 256, 0, st>>>(p);
-  else if (cap) masked_fwd_heads_kernel<D, true, false><<<grid, 256, 0, st>>>(p);
-  else if (bias) masked_fwd_heads_kernel<D, false, true><<<grid, 256, 0, st>>>(p);
-  else masked_fwd_heads_kernel<D, false, false><<<grid, 256, 0, st>>>(p);
+  if (cap && bias) masked_fwd_heads_kernel<D, U, PAD, true, true><<<grid, 256, 0, st>>>(p);
+  else if (cap) masked_fwd_heads_kernel<D, U, PAD, true, false><<<grid, 256, 0, st>>>(p);
+  else if (bias) masked_fwd_heads_kernel<D, U, PAD, false, true><<<grid, 256, 0, st>>>(p);
+  else masked_fwd_heads_kernel<D, U, PAD, false, false><<<grid, 256, 0, st>>>(p);
 }
 
 hipError_t masked_attention_fwd_heads(hipStream_t st, MaskedAttnParams const &p) {
-  if (p.Dq == 64) launch<64>(st, p);
-  else launch<128>(st, p);
+  int const most = p.Dq > p.Dv ? p.Dq : p.Dv;
+  if (p.Dq == p.Dv && p.Dq == 64) launch<64, 64, false>(st, p);
+  else if (p.Dq == p.Dv && p.Dq == 128) launch<128, 128, false>(st, p);
+  else if (most <= 64) launch<64, 64, true>(st, p);
+  else if (most <= 96) launch<128, 96, true>(st, p);
+  else launch<128, 128, true>(st, p);
   return hipGetLastError();
 }
 

@@ -191,6 +191,43 @@ def test_many_tiles_of_rows(ffk, D, cap, bias):
     compare(ffk, q, k, v, d_o, ranges=ranges, cap=cap, slopes=slopes_of(H) if bias else None)
 
 
+@pytest.mark.parametrize("D,Dv", [(8, 8), (40, 40), (72, 72), (88, 96), (96, 64), (104, 104), (120, 16), (16, 128)])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (5.0, True)])
+def test_heads_of_other_sizes(ffk, D, Dv, cap, bias):
+    """Heads that the kernels make longer with zeros: nothing of the next head, or of what lies behind a row's heads, enters."""
+    H, KH, B, Sq, Skv = 4, 2, 2, 150, 170
+    for rows in (Sq, 3):
+        tensors = make(D + Dv, B, rows, Skv, H, KH, D, Dv, BF)
+        wide = []
+        for x in tensors:  # the second key head's, and behind every row, are NaN
+            half = x.shape[2] * x.shape[3] // 2
+            w = torch.full((B, x.shape[1], 2 * half + 8), float("nan"), dtype=BF, device="cuda")
+            w[:, :, :half] = x.flatten(2)[:, :, :half]
+            wide.append(w)
+        q, k, v, d_o = wide
+        slopes = slopes_of(H) if bias else None
+        scale, offset = D ** -0.5, Skv - rows
+        strides = [n for x in wide for n in x.stride()[:2]]
+        desc = ffk.MaskedAttentionDesc(B, H, KH, rows, Skv, D, Dv, *strides, offset, scale, cap, 1)
+        first = [x[:, :, :x.shape[2] // 2].contiguous() for x in tensors]
+        want = attention(*first[:3], scale, True, cap, None, slopes[:H // 2] if bias else None, offset, first[3], UNIT[BF])
+        for variant in (1, 0):
+            say("heads", D, Dv, rows, variant)
+            ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, variant)
+            try:
+                o, grads = torch.full_like(d_o, 7.0), [torch.full_like(x, 7.0) for x in (q, k, v)]
+                _, lse = ffk.masked_attention_forward(q, k, v, scale, distance_slopes=slopes, desc=desc, out=o)
+                ffk.masked_attention_backward(q, k, v, o, d_o, lse, scale, distance_slopes=slopes, desc=desc, grads=grads)
+                torch.cuda.synchronize()
+            finally:
+                ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, 0)
+            for name, w in zip(("o", "dq", "dk", "dv"), [o] + grads):
+                assert bool((w[:, :, -8:] == 7.0).all()), name
+                n = want[name].shape[2]
+                check(w[:, :, :(w.shape[2] - 8) // 2].unflatten(2, (n, -1)), want, name, "variant %d, " % variant)
+            check(lse[:, :H // 2].contiguous(), want, "lse")
+
+
 def test_ranges_and_causal_both_apply(ffk):
     q, k, v, d_o = make(4, 1, 200, 200, 2, 2, 64, 64, BF)
     ranges = torch.tensor([[[i // 2, 200] for i in range(200)]], dtype=torch.int32).cuda()
