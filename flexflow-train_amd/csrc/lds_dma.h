@@ -51,6 +51,14 @@ __device__ __forceinline__ void lds_dma16(i32x4 rsrc, unsigned lane_byte_off, un
                              // direct loads (tests/test_gpu_linear.py: GEMM variants)
                              // and by the attention kernels' tests against the oracle.
 }
+// The same for data that is read once: nothing of it is kept in the caches.
+__device__ __forceinline__ void lds_dma16_once(i32x4 rsrc, unsigned lane_byte_off, unsigned uniform_byte_off,
+                                               unsigned lds_byte_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+               :
+               : "s"(lds_byte_addr), "v"(lane_byte_off), "s"(rsrc), "s"(uniform_byte_off)
+               : "memory");
+}
 // The same for 4 bytes per lane: lane l's dword lands at lds_base + 4 l.
 __device__ __forceinline__ void lds_dma4(i32x4 rsrc, unsigned lane_byte_off, unsigned uniform_byte_off,
                                          unsigned lds_byte_addr) {

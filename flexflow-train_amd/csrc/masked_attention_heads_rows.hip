@@ -79,14 +79,14 @@ __global__ __launch_bounds__(64) void masked_fwd_rows_kernel(MaskedAttnParams p)
 #pragma unroll
       for (int i = 0; i < C::kLoads; i++) {
         int const slot = slot_row + i * C::kRowsPerLoad, r = min(slot, hi_all - 1 - kv0);
-        lds_dma16(k_rsrc, tile_offset<PAD>(r * p.k_ss, (slot_pc ^ C::kswz(slot)) * 8, dim_qk), 0u, k_dst + (unsigned)(i * 1024));
-        lds_dma16(v_rsrc, tile_offset<PAD>(r * p.v_ss, v_lc * 8, dim_v), 0u, v_dst + (unsigned)(i * 1024));
+        lds_dma16_once(k_rsrc, tile_offset<PAD>(r * p.k_ss, (slot_pc ^ C::kswz(slot)) * 8, dim_qk), 0u, k_dst + (unsigned)(i * 1024));
+        lds_dma16_once(v_rsrc, tile_offset<PAD>(r * p.v_ss, v_lc * 8, dim_v), 0u, v_dst + (unsigned)(i * 1024));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < C::kLoads; i++) {
-        lds_dma16(k_rsrc, k_voff[i], 0u, k_dst + (unsigned)(i * 1024));
-        lds_dma16(v_rsrc, v_voff, (unsigned)(i * C::kRowsPerLoad) * (unsigned)p.v_ss * 2u, v_dst + (unsigned)(i * 1024));
+        lds_dma16_once(k_rsrc, k_voff[i], 0u, k_dst + (unsigned)(i * 1024));
+        lds_dma16_once(v_rsrc, v_voff, (unsigned)(i * C::kRowsPerLoad) * (unsigned)p.v_ss * 2u, v_dst + (unsigned)(i * 1024));
       }
     }
   };
