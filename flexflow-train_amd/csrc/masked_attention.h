@@ -173,8 +173,9 @@ struct TileStride {
   static constexpr int both = sizeof(T) == 2 ? (DP % 64 == 0 ? DP + 40 : DP + 8) : DP + 4;
 };
 
-// A tile of N rows on its way from memory to LDS.  Columns past the head size are zeros, rows outside [first, last]
-// repeat a row inside: whatever lies in memory that no row of the workgroup sees is not read.
+// A tile of N rows on its way from memory to LDS.  Columns past the head size become zeros on the way into LDS (a lane
+// there fetches the row's first columns again: no branch around a load), rows outside of the tensors are the caller's to
+// replace by others: whatever lies in memory that no row of the workgroup sees is not read.
 template <typename T, int DP, int N>
 struct TileRegs {
   static constexpr int kE = 16 / (int)sizeof(T);  // elements of a 16-byte chunk
@@ -186,17 +187,21 @@ struct TileRegs {
 #pragma unroll
     for (int n = 0; n < kN; n++) {
       int const c = t + n * 256, row = c / kCPR, ch = c % kCPR;
-      r[n] = u32x4{0u, 0u, 0u, 0u};
-      if ((N * kCPR % 256 == 0 || c < N * kCPR) && ch * kE < D)
-        r[n] = *reinterpret_cast<u32x4 const *>(row_pointer(row) + ch * kE);
+      r[n] = *reinterpret_cast<u32x4 const *>(row_pointer(row) + (ch * kE < D ? ch * kE : 0));
     }
   }
-  __device__ __forceinline__ void store(T *tile, int stride, int t) const {
+  // `keep(n)`: whether the row of chunk n is wanted, or zeros in its place
+  template <typename KEEP>
+  __device__ __forceinline__ void store(T *tile, int stride, int D, int t, KEEP keep) const {
 #pragma unroll
     for (int n = 0; n < kN; n++) {
       int const c = t + n * 256, row = c / kCPR, ch = c % kCPR;
-      if (N * kCPR % 256 == 0 || c < N * kCPR) *reinterpret_cast<u32x4 *>(tile + row * stride + ch * kE) = r[n];
+      u32x4 const v = ch * kE < D && keep(n) ? r[n] : u32x4{0u, 0u, 0u, 0u};
+      if (N * kCPR % 256 == 0 || c < N * kCPR) *reinterpret_cast<u32x4 *>(tile + row * stride + ch * kE) = v;
     }
+  }
+  __device__ __forceinline__ void store(T *tile, int stride, int D, int t) const {
+    store(tile, stride, D, t, [](int) { return true; });
   }
 };
 

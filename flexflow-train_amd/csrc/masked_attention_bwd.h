@@ -106,8 +106,8 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
     tv.load([&](int r) { return vp + (int64_t)min(kv0 + r, hi_all - 1) * p.v_ss; }, p.Dv, t);
   };
   auto stash = [&](int buf) {
-    tk.store(k_tile(buf), C::kKS, t);
-    tv.store(v_tile(buf), C::kVS, t);
+    tk.store(k_tile(buf), C::kKS, p.Dq, t);
+    tv.store(v_tile(buf), C::kVS, p.Dv, t);
   };
   int const koff = lane_k_off(C::kKS, lane), voff = lane_k_off(C::kVS, lane), toff = turn_off<T>(C::kKS, lane);
   if (ntiles > 0) {
@@ -203,11 +203,6 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
 }
 
 // What a row brings along into LDS: its range, statistics, slope and position.
-template <int N>
-struct RowStats {
-  float lse2[N], delta[N], slope[N];
-  int lo[N], hi[N], position[N];
-};
 
 template <typename T, int DP, int KG>
 struct MaskedDkdv {
@@ -231,7 +226,7 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
   constexpr bool kDv = (WHAT & 1) != 0, kDk = (WHAT & 2) != 0;
   constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
-  __shared__ RowStats<kT> stats[C::kBuffers];
+  __shared__ __attribute__((aligned(16))) float stats[C::kBuffers][kRowFields][kT];  // integers by their bits
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const kg = wave / KW, kw = wave % KW;
@@ -264,33 +259,42 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
 
   auto q_tile = [&](int buf) { return reinterpret_cast<T *>(pool + buf * C::kTile); };
   auto g_tile = [&](int buf) { return q_tile(buf) + kT * C::kS; };
-  auto seen_by = [&](int tile) {
-    RangeSummary const s = sums[tile];
-    return s.lo_min < kv0 + 32 * KG && s.hi_max > kv0;
-  };
-  // the next step at or behind `step` in which a row sees a key of this workgroup
-  auto next = [&](int step) {
-    for (; step < nsteps; step++) {
-      bool any = false;
-#pragma unroll
-      for (int w = 0; w < KW; w++) any = any || (step * KW + w < nsum && seen_by(step * KW + w));
-      if (any) break;
+  // Which tiles: a lane holds the summary of one of 64, read before they are needed, so that no step waits for memory to
+  // know its tile (a load behind those of the next tile's rows would wait for them too).
+  RangeSummary mine;
+  uint64_t wanted = 0;  // tiles with a row that sees a key of this workgroup
+  int group = -1;
+  auto next = [&](int step) {  // the first step at or behind `step` that has such a tile
+    int tile = step * KW;
+    while (tile < nsum) {
+      if (tile >> 6 != group) {
+        group = tile >> 6;
+        int const at = group * 64 + lane;
+        mine = at < nsum ? sums[at] : RangeSummary{1 << 30, 0, 1 << 30, 0};
+        wanted = __builtin_amdgcn_ballot_w64(mine.lo_min < kv0 + 32 * KG && mine.hi_max > kv0);
+      }
+      uint64_t const left = wanted >> (tile & 63);
+      if (left != 0) return (tile + __builtin_ctzll(left)) / KW;
+      tile = (tile & ~63) + 64;
     }
-    return step;
+    return nsteps;
+  };
+  auto summary_of = [&](int tile) {  // of the tiles that `next` looked at last
+    int const at = tile & 63;
+    return RangeSummary{__builtin_amdgcn_readlane(mine.lo_min, at), __builtin_amdgcn_readlane(mine.hi_max, at),
+                        __builtin_amdgcn_readlane(mine.lo_max, at), __builtin_amdgcn_readlane(mine.hi_min, at)};
   };
   using Regs = TileRegs<T, DP, kT>;
   Regs tq, tg;
-  int2 seen[Regs::kN];  // the ranges of this thread's rows: one that sees none of the keys is a row of zeros in LDS
-  float st_lse2, st_delta, st_slope;
-  int st_lo, st_hi, st_position;
+  int seen_lo[Regs::kN], seen_hi[Regs::kN];  // of this thread's rows: one that sees none of the keys is a row of zeros in LDS
+  float field[kRowFields];                   // of row t of the step
+  float const *rows = p.rows + (int64_t)hb * kRowFields * p.padded_rows;
   auto fetch = [&](int step) {
 #pragma unroll
     for (int n = 0; n < Regs::kN; n++) {
-      int const r = step * kT + (t + n * 256) / Regs::kCPR;
-      int i, g;
-      row_of(p, min(r, p.R - 1), i, g);
-      row_range(p, b, i, seen[n].x, seen[n].y);
-      if (r >= p.R) seen[n].y = 0;
+      int const r = min(step * kT + (t + n * 256) / Regs::kCPR, p.padded_rows - 1);
+      seen_lo[n] = __float_as_int(rows[kRowLo * (int64_t)p.padded_rows + r]);
+      seen_hi[n] = __float_as_int(rows[kRowHi * (int64_t)p.padded_rows + r]);
     }
     auto offset = [&](int r, int64_t seq_stride, int D) {
       int i, g;
@@ -299,54 +303,39 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
     };
     tq.load([&](int r) { return qp + offset(r, p.q_ss, p.Dq); }, p.Dq, t);
     tg.load([&](int r) { return gp + offset(r, p.o_ss, p.Dv); }, p.Dv, t);
-    if (t < kT) {
-      int const r = min(step * kT + t, p.R - 1);
-      int i, g;
-      row_of(p, r, i, g);
-      row_range(p, b, i, st_lo, st_hi);
-      if (step * kT + t >= p.R) st_hi = 0;
-      float const *rows = p.rows + (int64_t)hb * kRowFields * p.padded_rows + r;
-      st_lse2 = rows[kRowLse2 * (int64_t)p.padded_rows];
-      st_delta = rows[kRowDelta * (int64_t)p.padded_rows];
-      st_slope = kBias ? p.slopes[kh * p.G + g] * p.slope_unit : 0.0f;
-      st_position = p.q_offset + i;
-    }
-  };
-  auto stash = [&](int buf) {
+    int const r = min(step * kT + min(t, kT - 1), p.padded_rows - 1);
 #pragma unroll
-    for (int n = 0; n < Regs::kN; n++) {
-      if (!(seen[n].x < kv0 + 32 * KG && seen[n].y > kv0)) {
-        tq.r[n] = u32x4{0u, 0u, 0u, 0u};
-        tg.r[n] = u32x4{0u, 0u, 0u, 0u};
-      }
-    }
-    tq.store(q_tile(buf), C::kS, t);
-    tg.store(g_tile(buf), C::kS, t);
+    for (int f = 0; f < (kBias ? kRowFields : kRowSlope); f++) field[f] = rows[f * (int64_t)p.padded_rows + r];
+  };
+  auto stash = [&](int buf, int step) {
+    auto keep = [&](int n) {
+      int const r = step * kT + (t + n * 256) / Regs::kCPR;
+      return r < p.R && seen_lo[n] < kv0 + 32 * KG && seen_hi[n] > kv0;
+    };
+    tq.store(q_tile(buf), C::kS, p.Dq, t, keep);
+    tg.store(g_tile(buf), C::kS, p.Dv, t, keep);
     if (t < kT) {
-      stats[buf].lse2[t] = st_lse2;
-      stats[buf].delta[t] = st_delta;
-      stats[buf].slope[t] = st_slope;
-      stats[buf].lo[t] = st_lo;
-      stats[buf].hi[t] = st_hi;
-      stats[buf].position[t] = st_position;
+#pragma unroll
+      for (int f = 0; f < (kBias ? kRowFields : kRowSlope); f++)
+        stats[buf][f][t] = f == kRowHi && step * kT + t >= p.R ? __int_as_float(0) : field[f];
     }
   };
   int const roff = lane_k_off(C::kS, lane), toff = turn_off<T>(C::kS, lane);
-  int step = next(0);
+  int step = __builtin_amdgcn_readfirstlane(next(0));
   if (step < nsteps) {
     fetch(step);
-    stash(0);
+    stash(0, step);
   }
   __syncthreads();
   int cur = 0;
   while (step < nsteps) {
-    int const after = next(step + 1);
+    RangeSummary const sum = summary_of(step * KW + kw);
+    int const after = __builtin_amdgcn_readfirstlane(next(step + 1));
     if (after < nsteps) fetch(after);
-    int const tile = step * KW + kw;
-    RangeSummary const sum = tile < nsum ? sums[tile] : RangeSummary{1 << 30, 0, 0, 0};
     if (wkv0 < p.Skv && sum.lo_min < wkv0 + 32 && sum.hi_max > wkv0) {
       T const *qt = q_tile(cur) + kw * 32 * C::kS, *gt = g_tile(cur) + kw * 32 * C::kS;
-      RowStats<kT> const &rs = stats[cur];
+      // a field of the rows of scores 4 g .. + 3
+      auto rows4 = [&](int f, int g) { return *reinterpret_cast<f32x4 const *>(&stats[cur][f][kw * 32 + 8 * g + 4 * h32]); };
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; r++) {
@@ -361,19 +350,38 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
       float pv[16], ds[16];
       bool const whole = wkv0 >= sum.lo_max && wkv0 + 32 <= sum.hi_min;
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        int const at = kw * 32 + 8 * (r >> 2) + 4 * h32 + (r & 3);
-        float const y = capped<T, kCap>(p, s[r]);
-        float x = y;
-        if constexpr (kBias) x = __builtin_fmaf(-rs.slope[at], (float)abs(rs.position[at] - kv), x);
-        pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -rs.lse2[at]));
-        if constexpr (kDk) {
-          ds[r] = pv[r] * (dp[r] - rs.delta[at]);
-          if constexpr (kCap) ds[r] *= capped_slope<T>(y);
+      for (int g = 0; g < 4; g++) {
+        f32x4 const lse4 = rows4(kRowLse2, g);
+        f32x4 delta4, slope4, position4;
+        if constexpr (kDk) delta4 = rows4(kRowDelta, g);
+        if constexpr (kBias) {
+          slope4 = rows4(kRowSlope, g);
+          position4 = rows4(kRowPosition, g);
         }
-        if (!whole && (kv < rs.lo[at] || kv >= rs.hi[at])) {
-          pv[r] = 0.0f;
-          if constexpr (kDk) ds[r] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          int const r = 4 * g + e;
+          float const y = capped<T, kCap>(p, s[r]);
+          float x = y;
+          if constexpr (kBias) x = __builtin_fmaf(-slope4[e], (float)abs(__float_as_int(position4[e]) - kv), x);
+          pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse4[e]));
+          if constexpr (kDk) {
+            ds[r] = pv[r] * (dp[r] - delta4[e]);
+            if constexpr (kCap) ds[r] *= capped_slope<T>(y);
+          }
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          f32x4 const lo4 = rows4(kRowLo, g), hi4 = rows4(kRowHi, g);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (kv < __float_as_int(lo4[e]) || kv >= __float_as_int(hi4[e])) {
+              pv[4 * g + e] = 0.0f;
+              if constexpr (kDk) ds[4 * g + e] = 0.0f;
+            }
+          }
         }
       }
 #pragma unroll
@@ -391,12 +399,12 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
       }
     }
     if constexpr (C::kBuffers == 2) {
-      if (after < nsteps) stash(cur ^ 1);
+      if (after < nsteps) stash(cur ^ 1, after);
       __syncthreads();
       cur ^= 1;
     } else {
       __syncthreads();
-      if (after < nsteps) stash(0);
+      if (after < nsteps) stash(0, after);
       __syncthreads();
     }
     step = after;

@@ -90,8 +90,8 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
     tv.load([&](int r) { return vp + (int64_t)min(kv0 + r, hi_all - 1) * p.v_ss; }, p.Dv, t);
   };
   auto stash = [&](int buf) {
-    tk.store(k_tile(buf), C::kKS, t);
-    tv.store(v_tile(buf), C::kVS, t);
+    tk.store(k_tile(buf), C::kKS, p.Dq, t);
+    tv.store(v_tile(buf), C::kVS, p.Dv, t);
   };
   int const koff = lane_k_off(C::kKS, lane), toff = turn_off<T>(C::kVS, lane);
   if (ntiles > 0) {
