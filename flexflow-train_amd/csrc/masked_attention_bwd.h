@@ -224,6 +224,9 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
   using C = MaskedDkdv<T, DP, KG>;
   constexpr int KW = C::kKW, kT = C::kT;
   constexpr bool kDv = (WHAT & 1) != 0, kDk = (WHAT & 2) != 0;
+  // bf16 past 128 columns: the accumulators, half of a lane's registers, stay in accumulation registers, so that the other
+  // half holds operands read ahead
+  constexpr bool kKept = sizeof(T) == 2 && DP > 128;
   constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ __attribute__((aligned(16))) float stats[C::kBuffers][kRowFields][kT];  // integers by their bits
@@ -256,6 +259,13 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
       if constexpr (kDk) dk[i][r] = 0.0f;
       if constexpr (kDv) dv[i][r] = 0.0f;
     }
+  if constexpr (kKept) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; i++) {
+      if constexpr (kDk) asm volatile("" : "+a"(dk[i]));
+      if constexpr (kDv) asm volatile("" : "+a"(dv[i]));
+    }
+  }
 
   auto q_tile = [&](int buf) { return reinterpret_cast<T *>(pool + buf * C::kTile); };
   auto g_tile = [&](int buf) { return q_tile(buf) + kT * C::kS; };
@@ -342,10 +352,25 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
         s[r] = 0.0f;
         dp[r] = 0.0f;
       }
+      if constexpr (kKept) {
+        constexpr int W = kDk ? 2 : 1, N = W * DP / 16, kAhead = 4;
+        Frag<T> fr[kAhead + 1];
+        auto fragment = [&](int n) { return frag_lds((n % W == 0 ? qt : gt) + roff + n / W * 16); };
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; kk++) {
-        mma(s, frag_lds(qt + roff + kk * 16), kf[kk]);
-        if constexpr (kDk) mma(dp, frag_lds(gt + roff + kk * 16), vf[kk]);
+        for (int n = 0; n < kAhead; n++) fr[n] = fragment(n);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+          if (n + kAhead < N) fr[(n + kAhead) % (kAhead + 1)] = fragment(n + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+          if (n % W == 0) mma(s, fr[n % (kAhead + 1)], kf[n / W]);
+          else mma(dp, fr[n % (kAhead + 1)], vf[n / W]);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; kk++) {
+          mma(s, frag_lds(qt + roff + kk * 16), kf[kk]);
+          if constexpr (kDk) mma(dp, frag_lds(gt + roff + kk * 16), vf[kk]);
+        }
       }
       float pv[16], ds[16];
       bool const whole = wkv0 >= sum.lo_max && wkv0 + 32 <= sum.hi_min;
@@ -384,17 +409,34 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
           }
         }
       }
+      if constexpr (kKept) {
+        // (one of the two products: WHAT is 1 or 2 past 128 columns)
+        bf16x8 of[2] = {pack8(kDv ? pv : ds), pack8((kDv ? pv : ds) + 8)};
+        bf16 const *from = (kDv ? gt : qt) + toff;
+        constexpr int N = DP / 16, kAhead = 4;
+        bf16x8 fr[kAhead + 1];
 #pragma unroll
-      for (int s2 = 0; s2 < 2; s2++) {
-        if constexpr (kDv) {
-          Frag<T> const pf = frag_acc(pv + 8 * s2, kp);
+        for (int n = 0; n < kAhead; n++) fr[n] = frag_turned(from, C::kS, n / (DP / 32), n % (DP / 32) * 32).v;
+        asm volatile("s_nop 3" : "+v"(of[0]), "+v"(of[1]));  // the wait states between a vector instruction and mma_kept
 #pragma unroll
-          for (int i = 0; i < DP / 32; i++) mma(dv[i], frag_turned(gt + toff, C::kS, s2, i * 32), pf);
+        for (int n = 0; n < N; n++) {
+          if (n + kAhead < N) fr[(n + kAhead) % (kAhead + 1)] = frag_turned(from, C::kS, (n + kAhead) / (DP / 32), (n + kAhead) % (DP / 32) * 32).v;
+          if constexpr (kDv) mma_kept(dv[n % (DP / 32)], fr[n % (kAhead + 1)], of[n / (DP / 32)]);
+          else mma_kept(dk[n % (DP / 32)], fr[n % (kAhead + 1)], of[n / (DP / 32)]);
         }
-        if constexpr (kDk) {
-          Frag<T> const df = frag_acc(ds + 8 * s2, kp);
+      } else {
 #pragma unroll
-          for (int i = 0; i < DP / 32; i++) mma(dk[i], frag_turned(qt + toff, C::kS, s2, i * 32), df);
+        for (int s2 = 0; s2 < 2; s2++) {
+          if constexpr (kDv) {
+            Frag<T> const pf = frag_acc(pv + 8 * s2, kp);
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) mma(dv[i], frag_turned(gt + toff, C::kS, s2, i * 32), pf);
+          }
+          if constexpr (kDk) {
+            Frag<T> const df = frag_acc(ds + 8 * s2, kp);
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) mma(dk[i], frag_turned(qt + toff, C::kS, s2, i * 32), df);
+          }
         }
       }
     }
@@ -410,6 +452,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
     step = after;
   }
 
+  if constexpr (kKept && kDv) mma_settled(dv);
+  if constexpr (kKept && kDk) mma_settled(dk);
   // the sums of the waves of a group, added up by its first, and written out: a lane owns a key
   auto finish = [&](f32x16 (&acc)[DP / 32], float factor, T *out, int D) {
     if constexpr (KW > 1) {
