@@ -51,7 +51,7 @@ struct MaskedAttnParams {
   float score_scale, shift, slope_unit, grad_scale;
   float cap_in;
   int capped, causal;
-  FastDiv group;
+  FastDiv group, heads_div, places_div;  // by G, KH and KH B
   // forward, split over the keys: partial O (unnormalised), maximum and sum of each part
   int splits;
   float *part_o, *part_ml;
@@ -62,6 +62,16 @@ __device__ __forceinline__ void row_of(MaskedAttnParams const &p, int r, int &i,
   p.group.divmod((uint32_t)r, a, b);
   i = (int)a;
   g = (int)b;
+}
+// The key head that this workgroup works on, its batch entry and their place among all; returns the workgroup's number there.
+__device__ __forceinline__ int place_of(MaskedAttnParams const &p, int &kh, int &b, int &hb) {
+  uint32_t rest, place, entry, head;
+  p.places_div.divmod(blockIdx.x, rest, place);
+  p.heads_div.divmod(place, entry, head);
+  kh = (int)head;
+  b = (int)entry;
+  hb = (int)place;
+  return (int)rest;
 }
 // The keys that row i of batch b sees, within [0, Skv]; nothing is (INT_MAX / 2, 0), which widens no window.
 __device__ __forceinline__ void row_range(MaskedAttnParams const &p, int b, int i, int &lo, int &hi) {
@@ -229,9 +239,8 @@ __device__ __forceinline__ float capped_slope(float y) {
 
 // A wave's smallest and largest of an integer, scalar.
 __device__ __forceinline__ int wave_min_int(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64));
-  return __builtin_amdgcn_readfirstlane(v);
+  float const r = wave_reduce(__int_as_float(v), [](float a, float b) { return __int_as_float(min(__float_as_int(a), __float_as_int(b))); });
+  return __builtin_amdgcn_readfirstlane(__float_as_int(r));
 }
 __device__ __forceinline__ int wave_max_int(int v) { return -wave_min_int(-v); }
 

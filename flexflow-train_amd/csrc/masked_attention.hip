@@ -216,6 +216,8 @@ static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, int dtyp
   p.causal = d->causal != 0;
   p.padded_rows = (p.R + 63) / 64 * 64;
   p.group = make_fast_div((uint32_t)p.G);
+  p.heads_div = make_fast_div((uint32_t)p.KH);
+  p.places_div = make_fast_div((uint32_t)(p.KH * p.B));
   p.splits = 1;
   return p;
 }

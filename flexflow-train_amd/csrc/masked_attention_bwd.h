@@ -33,9 +33,8 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const qw = wave / KW, kw = wave % KW;
   int const nrb = (p.R + 32 * RG - 1) / (32 * RG);
-  int const hb = blockIdx.x % (p.KH * p.B);
-  int const rb = nrb - 1 - blockIdx.x / (p.KH * p.B);
-  int const kh = hb % p.KH, b = hb / p.KH;
+  int kh, b, hb;
+  int const rb = nrb - 1 - place_of(p, kh, b, hb);
   int const row0 = rb * 32 * RG + qw * 32;
   int const row = row0 + (lane & 31);
   int qi, qg;
@@ -233,9 +232,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const kg = wave / KW, kw = wave % KW;
-  int const hb = blockIdx.x % (p.KH * p.B);
-  int const kh = hb % p.KH, b = hb / p.KH;
-  int const kv0 = (int)(blockIdx.x / (p.KH * p.B)) * 32 * KG;  // under a causal mask the first keys are seen by most rows
+  int kh, b, hb;
+  int const kv0 = place_of(p, kh, b, hb) * 32 * KG;  // under a causal mask the first keys are seen by most rows
   int const wkv0 = kv0 + kg * 32, kv = wkv0 + (lane & 31);
   int const nsum = (p.R + 31) / 32, nsteps = (nsum + KW - 1) / KW;
   RangeSummary const *sums = p.summary + (int64_t)b * nsum;

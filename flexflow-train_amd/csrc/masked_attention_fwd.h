@@ -34,11 +34,10 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const qw = wave / KW, kw = wave % KW;
   int const nrb = (p.R + 32 * RG - 1) / (32 * RG);
-  int const hb = blockIdx.x % (p.KH * p.B);
-  int const rest = blockIdx.x / (p.KH * p.B);
+  int kh, b, hb;
+  int const rest = place_of(p, kh, b, hb);
   int const split = rest % p.splits;
   int const rb = nrb - 1 - rest / p.splits;  // under a causal mask the heaviest rows go first
-  int const kh = hb % p.KH, b = hb / p.KH;
   int const row0 = rb * 32 * RG + qw * 32;
   int const row = row0 + (lane & 31);
   int qi, qg;

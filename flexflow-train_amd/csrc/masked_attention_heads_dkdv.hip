@@ -46,9 +46,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
   int const dim_qk = PAD ? p.Dq : D, dim_v = PAD ? p.Dv : D;  // the heads themselves
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  int const hb = blockIdx.x % (p.KH * p.B);
-  int const kh = hb % p.KH, b = hb / p.KH;
-  int const kv0 = (int)(blockIdx.x / (p.KH * p.B)) * C::kKeys;  // under a causal mask the first keys are seen by most rows
+  int kh, b, hb;
+  int const kv0 = place_of(p, kh, b, hb) * C::kKeys;  // under a causal mask the first keys are seen by most rows
   int const wkv0 = kv0 + wave * 32, kvcol = wkv0 + (lane & 31);
   bf16 const *qp = static_cast<bf16 const *>(p.q) + (int64_t)b * p.q_bs + (int64_t)kh * p.G * dim_qk;
   bf16 const *gp = static_cast<bf16 const *>(p.d_o) + (int64_t)b * p.o_bs + (int64_t)kh * p.G * dim_v;

@@ -33,9 +33,8 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const nrb = (p.R + 127) / 128;
-  int const hb = blockIdx.x % (p.KH * p.B);
-  int const rb = nrb - 1 - blockIdx.x / (p.KH * p.B);
-  int const kh = hb % p.KH, b = hb / p.KH;
+  int kh, b, hb;
+  int const rb = nrb - 1 - place_of(p, kh, b, hb);
   int const row0 = rb * 128 + wave * 32;
   int const row = row0 + (lane & 31);
   int qi, qg;

@@ -32,9 +32,8 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const nrb = (p.R + C::kRows - 1) / C::kRows;
-  int const hb = blockIdx.x % (p.KH * p.B);
-  int const rb = nrb - 1 - blockIdx.x / (p.KH * p.B);  // under a causal mask the heaviest rows go first
-  int const kh = hb % p.KH, b = hb / p.KH;
+  int kh, b, hb;
+  int const rb = nrb - 1 - place_of(p, kh, b, hb);  // under a causal mask the heaviest rows go first
   int const row = rb * C::kRows + wave * 32 + (lane & 31);
   int qi, qg;
   row_of(p, min(row, p.R - 1), qi, qg);

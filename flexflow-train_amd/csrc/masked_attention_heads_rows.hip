@@ -30,10 +30,9 @@ __global__ __launch_bounds__(64) void masked_fwd_rows_kernel(MaskedAttnParams p)
   __shared__ __attribute__((aligned(1024))) bf16 Vs[2][C::kBlock];
   int const dim_qk = PAD ? p.Dq : D, dim_v = PAD ? p.Dv : D;  // the heads themselves
   int const lane = threadIdx.x, h32 = lane >> 5;
-  int const hb = blockIdx.x % (p.KH * p.B);
-  int const rest = blockIdx.x / (p.KH * p.B);
+  int kh, b, hb;
+  int const rest = place_of(p, kh, b, hb);
   int const split = rest % p.splits, rb = rest / p.splits;
-  int const kh = hb % p.KH, b = hb / p.KH;
   int const row = rb * 32 + (lane & 31);
   int qi, qg;
   row_of(p, min(row, p.R - 1), qi, qg);
