@@ -762,7 +762,7 @@ def attention_backward(q, k, v, o, d_o, lse, scale, causal, desc=None):
 
 def _int32(t, shape, what):
     torch = _torch()
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape):
+    if t is not None and (t.dtype != torch.int32 or t.shape != shape):
         raise ValueError("%s: int32 %s expected, %s %s given" % (what, list(shape), t.dtype, list(t.shape)))
     return t
 
@@ -771,15 +771,19 @@ def attention_key_ranges(batch, seq_q, seq_kv, causal=False, document_starts=Non
                          out=None, device="cuda"):
     """int32 [batch, seq_q, 2]: the keys lo <= j < hi that each query row sees (ffk_attention_key_ranges)."""
     torch = _torch()
-    docs = 1
+    docs, like = 1, document_starts
     if document_starts is not None:
         docs = document_starts.shape[-1] - 1
         _int32(document_starts, (batch, docs + 1), "document_starts")
-    _int32(prefix_lengths, (batch, docs), "prefix_lengths")
-    if out is None:
-        like = document_starts if document_starts is not None else prefix_lengths
-        out = torch.empty((batch, seq_q, 2), dtype=torch.int32, device=device if like is None else like.device)
-    _int32(out, (batch, seq_q, 2), "out")
+    if prefix_lengths is not None:
+        _int32(prefix_lengths, (batch, docs), "prefix_lengths")
+        like = prefix_lengths
+    if out is not None:
+        _int32(out, (batch, seq_q, 2), "out")
+    elif like is not None:
+        out = like.new_empty((batch, seq_q, 2))
+    else:
+        out = torch.empty((batch, seq_q, 2), dtype=torch.int32, device=device)
     _call.ffk_attention_key_ranges(batch, seq_q, seq_kv, query_offset, int(causal), document_starts, docs, prefix_lengths, out)
     return out
 
@@ -901,19 +905,22 @@ def _rotary_desc(q, k, sections, interleaved):
 
 def _rotary(entry, q, k, positions, frequencies, sections, interleaved, desc, q_out, k_out):
     torch = _torch()
-    if any(t is not None and t.dtype != q.dtype for t in (k, q_out, k_out)):
+    dtype, plain = q.dtype, desc is None and q_out is None and k_out is None
+    if k is not None and k.dtype != dtype or not plain and any(t is not None and t.dtype != dtype for t in (q_out, k_out)):
         raise ValueError("rotary: all tensors have one data type")
-    own = q_out is not None or k_out is not None or desc is not None
     if desc is None:
-        desc = _rotary_desc(q.shape, None if k is None else k.shape, tuple(map(int, sections)), interleaved)
-    _int32(positions, (desc.num_axes, desc.batch, desc.seq), "positions")
-    if frequencies.dtype != torch.float32 or frequencies.numel() != sum(desc.sections[:desc.num_axes]):
-        raise ValueError("frequencies: float32 [%d] expected" % sum(desc.sections[:desc.num_axes]))
+        sections = tuple(map(int, sections))
+        desc = _rotary_desc(q.shape, None if k is None else k.shape, sections, bool(interleaved))
+    else:
+        sections = desc.sections[:desc.num_axes]
+    _int32(positions, (len(sections), desc.batch, desc.seq), "positions")
+    if frequencies.dtype != torch.float32 or frequencies.numel() != sum(sections):
+        raise ValueError("frequencies: float32 [%d] expected" % sum(sections))
     if q_out is None:
         q_out = torch.empty_like(q)
     if k_out is None and k is not None:
         k_out = torch.empty_like(k)
-    if own:
+    if not plain:
         d = desc
         _reaches("rotary: q", q, d.batch, d.q_batch_stride, d.seq, d.q_seq_stride, d.q_heads * d.head_dim)
         _reaches("rotary: q_out", q_out, d.batch, d.q_out_batch_stride, d.seq, d.q_out_seq_stride, d.q_heads * d.head_dim)
