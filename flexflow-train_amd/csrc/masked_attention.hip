@@ -120,16 +120,22 @@ static int padded_head(ffk_masked_attention_desc_t const *d) {
 }
 static int64_t rows_of(ffk_masked_attention_desc_t const *d) { return d->seq_q * (d->heads / d->kv_heads); }
 
+static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype);
+// Workgroups of 128 rows or keys below which those of 32, whose four waves share out the other axis, are better.  fp32, bound
+// by its products: as many as CUs (two sequences of 1000 tokens, 8 heads of 64 on 4, causal, 128 workgroups: forward 87 us, and
+// 38 with 32 rows, backward 219 and 153; four sequences, 256 workgroups, not causal, 86 and 116, 285 and 367).  bf16: half as
+// many (two sequences, 8 heads of 128, 128 workgroups, forward 26 us and 37, backward 75 and 80; 8 heads of 256 on 4, 160
+// workgroups, forward 54 and 73; one sequence, 4 heads of 128 on 2, 32 workgroups, forward 25 and 21, backward 99 and 86).
+static int few_workgroups(int dtype) { return dtype == FFK_FLOAT ? kNumCU : kNumCU / 2; }
 // (FFK_OPTION_ATTENTION_VARIANT other than 0 keeps the kernels for many rows and keys at every size.)
-// 32-row groups of a workgroup: 4, or 1 whose four waves share out the keys, where there are no more rows or workgroups
-// of 128 would leave half of the CUs idle.  (fp32 heads past 128 have no such kernel.)
+// 32-row groups of a workgroup: 4, or 1 whose four waves share out the keys, where there are no more rows or few
+// workgroups.  (fp32 heads past 128 have no such kernel.)
 static int row_groups(ffk_masked_attention_desc_t const *d, int dtype) {
   if (dtype == FFK_FLOAT && padded_head(d) > 128) return 4;
   int64_t const rows = rows_of(d);
   if (option(FFK_OPTION_ATTENTION_VARIANT) != 0) return 4;
-  return rows <= 32 || (ceil_div(rows, 128) * d->kv_heads * d->batch < kNumCU / 2) ? 1 : 4;
+  return rows <= 32 || ceil_div(rows, 128) * d->kv_heads * d->batch < few_workgroups(dtype) ? 1 : 4;
 }
-static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype);
 // Parts of the keys, each a workgroup of its own, where few workgroups would run over long keys.  In the kernel of one
 // wave a workgroup (masked_attention_heads_rows.hip) ten waves for every CU, each with 256 keys at least: twice what runs at
 // a time, so that sequences of several lengths even out (16 of 4096 to 8192 keys, 8 key heads of 128: 86 us, with five 90);
@@ -237,12 +243,12 @@ static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype) {
   return dtype == FFK_BF16 && padded_head(d) <= 128 && d->k_seq_stride < (1 << 24) && d->v_seq_stride < (1 << 24) &&
          d->seq_q * d->q_seq_stride * 2 < lim && d->seq_q * d->o_seq_stride * 2 < lim;
 }
-// 32-key groups of a workgroup of the general dK/dV kernel, and whether it is to run in place of the one above: 4, or 1 whose
-// four waves share out the rows, where workgroups of 128 keys would leave half of the CUs idle.
-static int key_groups(ffk_masked_attention_desc_t const *d) {
+// 32-key groups of a workgroup of the general dK/dV kernel, and whether it is to run in place of the one for heads: 4, or 1
+// whose four waves share out the rows, where there are few workgroups.
+static int key_groups(ffk_masked_attention_desc_t const *d, int dtype) {
   if (padded_head(d) > 128) return 4;  // (no registers left for the rows' tiles)
   if (option(FFK_OPTION_ATTENTION_VARIANT) != 0) return 4;
-  return rows_of(d) > 32 && ceil_div(d->seq_kv, 128) * d->kv_heads * d->batch < kNumCU / 2 ? 1 : 4;
+  return rows_of(d) > 32 && ceil_div(d->seq_kv, 128) * d->kv_heads * d->batch < few_workgroups(dtype) ? 1 : 4;
 }
 
 }  // namespace ffk
@@ -343,7 +349,7 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
   int const groups = row_groups(d, dtype);
   if (groups == 4 && heads_kernels(d, dtype)) FFK_HIP(masked_attention_dq_heads(st, p));
   else FFK_HIP(launch_dq(st, p, padded, groups));
-  int const keys = key_groups(d);
+  int const keys = key_groups(d, dtype);
   if (keys == 4 && heads_kernels(d, dtype)) FFK_HIP(masked_attention_dkdv_heads(st, p));
   else FFK_HIP(launch_dkdv(st, p, padded, keys));
   return FFK_OK;
