@@ -645,10 +645,11 @@ int ffk_attention_backward(ffk_stream_t stream, int dtype,
  *     s -= distance_slopes[h] * |p_i - j|        (distance_slopes [heads] fp32 or NULL)
  *   over the keys of its range (key_ranges NULL: all keys), of which causal != 0
  *   leaves those with j <= p_i.  A row that sees no key has o = 0, lse = -inf and
- *   gives and takes no gradient.  What lies in k and v outside of every range of
- *   a workgroup's rows is not read; next to it, a key that is NaN or infinite
- *   must be one that no row sees only if it is more than 127 keys away from all
- *   that are seen, since a masked probability is 0 and 0 times it is not.
+ *   gives and takes no gradient, whatever lies in it.  Keys in front of the first
+ *   and behind the last one that a row of the batch entry sees (padding) may hold
+ *   anything, NaN and infinities too, and get zero gradients; a key between
+ *   them that a row does not see has to be finite all the same (a masked
+ *   probability is 0, and 0 times infinity is none).  Slopes are finite.
  *   Ranges are cut to [0, seq_kv].  distance_slopes and key_ranges have no gradient.
  *   dtype FFK_BF16 (head sizes multiples of 8 up to 256, strides multiples of 8
  *   elements) or FFK_FLOAT (multiples of 4); 16-byte aligned tensors, key_ranges
