@@ -14,6 +14,9 @@
 // pieces in turn 946 us).
 #include "ffk_common.h"
 #include <math.h>
+#include <algorithm>
+#include <memory>
+#include <new>
 
 namespace ffk {
 
@@ -195,6 +198,32 @@ static int check_list(char const *who, int const *dtypes, void const *const *gra
   return FFK_OK;
 }
 
+// Whether no output lies on another output or on another tensor's input: the pieces are worked on in no order.
+static int check_apart(char const *who, int const *dtypes, void const *const *grads, void *const *clipped, int64_t const *elems, int num) {
+  struct Span {
+    uintptr_t begin, end;
+    bool out;
+  };
+  std::unique_ptr<Span[]> const spans(new (std::nothrow) Span[2 * (size_t)num]);
+  FFK_REQUIRE(num == 0 || spans != nullptr, "%s: no host memory", who);
+  int n = 0;
+  for (int i = 0; i < num; i++) {
+    if (elems[i] == 0) continue;
+    uintptr_t const in = reinterpret_cast<uintptr_t>(grads[i]), out = reinterpret_cast<uintptr_t>(clipped[i]);
+    uintptr_t const bytes = (uintptr_t)elems[i] * dtype_size(dtypes[i]);
+    spans[n++] = Span{out, out + bytes, true};
+    if (in != out) spans[n++] = Span{in, in + bytes, false};
+  }
+  std::sort(spans.get(), spans.get() + n, [](Span const &a, Span const &b) { return a.begin < b.begin; });
+  uintptr_t in_end = 0, out_end = 0;
+  for (int i = 0; i < n; i++) {
+    FFK_REQUIRE(spans[i].begin >= out_end && (!spans[i].out || spans[i].begin >= in_end), "%s: tensors overlap", who);
+    uintptr_t &end = spans[i].out ? out_end : in_end;
+    if (spans[i].end > end) end = spans[i].end;
+  }
+  return FFK_OK;
+}
+
 // The tensors from `first` on that one launch takes, as its table; returns the first that it does not.
 static int fill_table(NormTable &a, int const *dtypes, void const *const *grads, void *const *out, int64_t const *elems, int num, int first,
                       int loads) {
@@ -277,6 +306,8 @@ extern "C" int ffk_clip_grad_norm(ffk_stream_t stream, int const *dtypes, void c
   rc = check_list("clip_grad_norm", dtypes, const_cast<void const *const *>(clipped), elems, num_tensors);
   if (rc != FFK_OK) return rc;
   FFK_REQUIRE(max_norm >= 0.0f, "clip_grad_norm: max_norm must not be negative");
+  rc = check_apart("clip_grad_norm", dtypes, grads, clipped, elems, num_tensors);
+  if (rc != FFK_OK) return rc;
   rc = check_workspace("clip_grad_norm", workspace, workspace_bytes, num_tensors);
   if (rc != FFK_OK) return rc;
   hipStream_t const st = as_stream(stream);

@@ -24,8 +24,8 @@ hipError_t masked_attention_dkdv_heads(hipStream_t st, MaskedAttnParams const &p
 constexpr int kRangeThreads = 256;
 
 // One thread a row: the last document that begins at or before the row's position, by bisection over the starts.  Every
-// index stays inside the starts whatever they hold, and the result inside [0, seq_kv].  Bound by the 8 bytes a row it
-// writes.
+// index stays inside the starts whatever they hold, and the result inside [0, seq_kv].  Bound by the latency of the
+// bisection's reads: 64 x 16384 rows, 50 documents, 7.0 us (8 MB written).
 __global__ __launch_bounds__(kRangeThreads) void key_ranges_kernel(int2 *out, int const *starts, int const *prefixes, int64_t rows,
                                                                    FastDiv seq_q, int seq_kv, int docs, int causal, int offset) {
   int64_t const at = (int64_t)blockIdx.x * kRangeThreads + threadIdx.x;
@@ -287,6 +287,7 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
   int const rc = check("masked_attention_forward", dtype, d);
   if (rc != FFK_OK) return rc;
   FFK_REQUIRE(q && k && v && o, "masked_attention_forward: NULL tensor");
+  FFK_REQUIRE(o != q && o != k && o != v, "masked_attention_forward: the output is an input");
   FFK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "masked_attention_forward: tensors must be 16-byte aligned");
   FFK_REQUIRE(reinterpret_cast<uintptr_t>(key_ranges) % 8 == 0, "masked_attention_forward: key_ranges must be 8-byte aligned");
   MaskedAttnParams p = params_of(d, dtype, q, k, v, key_ranges, distance_slopes);
@@ -325,6 +326,10 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
   int const rc = check("masked_attention_backward", dtype, d);
   if (rc != FFK_OK) return rc;
   FFK_REQUIRE(q && k && v && o && d_o && lse && dq && dk && dv, "masked_attention_backward: NULL tensor");
+  // (the dK/dV kernel reads all inputs behind the dQ kernel)
+  for (void const *grad : {dq, dk, dv})
+    FFK_REQUIRE(grad != q && grad != k && grad != v && grad != o && grad != d_o, "masked_attention_backward: a gradient is an input");
+  FFK_REQUIRE(dq != dk && dq != dv && dk != dv, "masked_attention_backward: two gradients are one");
   FFK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(d_o) && aligned16(dq) && aligned16(dk) && aligned16(dv),
               "masked_attention_backward: tensors must be 16-byte aligned");
   FFK_REQUIRE(reinterpret_cast<uintptr_t>(key_ranges) % 8 == 0, "masked_attention_backward: key_ranges must be 8-byte aligned");

