@@ -217,9 +217,9 @@ struct TileRegs {
 
 // The cap's part of a score that is not linear, and its derivative (1 without a cap, where y is the raw product).
 //   fp32: y = tanh(scale raw / cap), score_scale = cap log2(e), derivative 1 - y^2.
-//   bf16: y = -1 / (1 + 2^(cap_in raw)), cap_in = 2 log2(e) scale / cap, on the hardware's exponential and reciprocal: tanh is
-//   1 + 2 y, so score_scale = 2 cap log2(e), shift = cap log2(e), and 1 - tanh^2 = -4 (y + y^2), of which grad_scale has the
-//   -4.  Four vector instructions a score and two for the derivative; about 2^-22 off in absolute terms, which the cap
+//   bf16: y = 1 / (1 + 2^(cap_in raw)), cap_in = -2 log2(e) scale / cap, on the hardware's exponential and reciprocal: tanh is
+//   2 y - 1, so score_scale = 2 cap log2(e), shift = -cap log2(e), and 1 - tanh^2 = 4 (y - y^2), of which grad_scale has the
+//   4.  Four vector instructions a score and two for the derivative; about 2^-22 off in absolute terms, which the cap
 //   multiplies to a few 1e-6 of a score, far below what bf16 scores carry.  (fp32's products take sixteen times as long: it
 //   can have the library's tanh.)
 template <typename T, bool CAP>
@@ -227,14 +227,14 @@ __device__ __forceinline__ float capped(MaskedAttnParams const &p, float raw) {
   if constexpr (!CAP) {
     return raw;
   } else if constexpr (sizeof(T) == 2) {
-    return -__builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * p.cap_in));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * p.cap_in));
   } else {
     return tanhf(raw * p.cap_in);
   }
 }
 template <typename T>
 __device__ __forceinline__ float capped_slope(float y) {
-  return sizeof(T) == 2 ? __builtin_fmaf(y, y, y) : __builtin_fmaf(-y, y, 1.0f);
+  return sizeof(T) == 2 ? __builtin_fmaf(-y, y, y) : __builtin_fmaf(-y, y, 1.0f);
 }
 
 // A wave's smallest and largest of an integer, scalar.

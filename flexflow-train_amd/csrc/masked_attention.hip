@@ -210,10 +210,10 @@ static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, int dtyp
   p.score_scale = d->scale * kLog2e;
   p.grad_scale = d->scale;
   if (p.capped && dtype == FFK_BF16) {
-    p.cap_in = 2.0f * kLog2e * (d->scale / d->score_cap);
+    p.cap_in = -2.0f * kLog2e * (d->scale / d->score_cap);
     p.score_scale = 2.0f * kLog2e * d->score_cap;
-    p.shift = kLog2e * d->score_cap;
-    p.grad_scale = -4.0f * d->scale;
+    p.shift = -kLog2e * d->score_cap;
+    p.grad_scale = 4.0f * d->scale;
   } else if (p.capped) {
     p.cap_in = d->scale / d->score_cap;
     p.score_scale = kLog2e * d->score_cap;

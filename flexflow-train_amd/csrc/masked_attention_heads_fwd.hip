@@ -7,7 +7,7 @@
 //   The loop runs over the union of the rows' ranges.  A wave passes over a tile that none of its rows sees, and ranges
 // are compared element by element only where a tile is not seen whole by all of its rows.
 //   Bound by the issue of vector instructions: 8192 tokens, 16 heads of 128, causal, biased 330 us (0.83 PFLOP/s); 4 x 4096
-// tokens in 3 documents, 32 heads of 128 on 8, causal, capped 374 us; 8 x 512 tokens in 4 documents, 16 heads of 64
+// tokens in 3 documents, 32 heads of 128 on 8, causal, capped 367 us; 8 x 512 tokens in 4 documents, 16 heads of 64
 // 18 us, where it is latency.  (For the second: vector steps fenced between the matrix instructions, as in the dK/dV
 // kernel, 485 us; eight waves and three buffers 430.)
 #include "masked_attention_heads.h"
@@ -189,7 +189,8 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
     float const m = max_across_halves(mx) * p.score_scale;
     float const m_new = m > m_run + kLazy ? m : m_run;
     float const m_use = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every exponential is 0
-    if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
+    // (a row that has seen nothing yet has only zeros to rescale)
+    if (__builtin_amdgcn_ballot_w64(m_new != m_run && m_run != -INFINITY) != 0) {
       float const alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_use);
       l_part *= alpha;
       mma_settled(oacc);
@@ -199,8 +200,8 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
         for (int r = 0; r < 16; r++) oacc[i][r] *= alpha;
 #pragma unroll
       for (int i = 0; i < U / 32; i++) asm volatile("" : "+a"(oacc[i]));
-      m_run = m_new;
     }
+    m_run = m_new;
     bf16x8 pf[4];
     float sum = 0.0f;
 #pragma unroll

@@ -146,15 +146,16 @@ __global__ __launch_bounds__(64) void masked_fwd_rows_kernel(MaskedAttnParams p)
     for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
     float const m_new = fmaxf(m_run, max_across_halves(mx) * p.score_scale);
     float const m_use = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every exponential is 0
-    if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
+    // (a row that has seen nothing yet has only zeros to rescale)
+    if (__builtin_amdgcn_ballot_w64(m_new != m_run && m_run != -INFINITY) != 0) {
       float const alpha = __builtin_amdgcn_exp2f(m_run - m_use);
       l_part *= alpha;
 #pragma unroll
       for (int i = 0; i < U / 32; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) oacc[i][r] *= alpha;
-      m_run = m_new;
     }
+    m_run = m_new;
     float pv[16], sum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; r++) {
