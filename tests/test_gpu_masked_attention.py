@@ -395,6 +395,35 @@ def test_offsets_past_32_bits(ffk):
     check(grads.view(S, stride)[:, D:2 * D].reshape(1, S, 1, D), want, "dv")
 
 
+@pytest.mark.parametrize("D,Sq", [(64, 70), (128, 70), (80, 3)])
+def test_rows_too_far_apart_for_short_offsets(ffk, D, Sq):
+    """Row strides of 2^24 elements, which the tuned kernels' offsets do not reach: the general ones, both forms."""
+    S, H, KH, stride = 130, 2, 1, 1 << 24
+    q, k, v, d_o = make(D, 1, Sq, S, H, KH, D, D, BF)
+    keys, rows = torch.zeros((S, stride), dtype=BF, device="cuda"), torch.zeros((Sq, stride), dtype=BF, device="cuda")
+    keys[:, :D], keys[:, D:2 * D], rows[:, :H * D], rows[:, H * D:2 * H * D] = k[0, :, 0], v[0, :, 0], q[0].flatten(1), d_o[0].flatten(1)
+    desc = ffk.MaskedAttentionDesc(1, H, KH, Sq, S, D, 0, Sq * stride, stride, S * stride, stride, S * stride, stride, Sq * stride, stride,
+                                   S - Sq, 0.125, 20.0, 1)
+    want = attention(q, k, v, 0.125, causal=True, cap=20.0, offset=S - Sq, d_o=d_o, unit=2.0 ** -8)
+    qf, kf = rows.view(-1), keys.view(-1)
+    vf, gf = kf[D:], qf[H * D:]
+    out, dkeys = torch.full_like(rows, 7.0), torch.full_like(keys, 7.0)
+    for variant in (1, 0):
+        say("far apart", D, Sq, variant)
+        ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, variant)
+        try:
+            of, dk = out.view(-1), dkeys.view(-1)
+            o, lse = ffk.masked_attention_forward(qf, kf, vf, 0.125, desc=desc, out=of)
+            ffk.masked_attention_backward(qf, kf, vf, o, gf, lse, 0.125, desc=desc, grads=(of[H * D:], dk, dk[D:]))
+            torch.cuda.synchronize()
+        finally:
+            ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, 0)
+        check(lse, want, "lse")
+        for name, t, at, n in (("o", out, 0, H), ("dq", out, H * D, H), ("dk", dkeys, 0, KH), ("dv", dkeys, D, KH)):
+            check(t[:, at:at + n * D].reshape(1, -1, n, D), want, name, "variant %d, " % variant)
+        assert bool((out[:, 2 * H * D:2 * H * D + 64] == 7.0).all()) and bool((dkeys[:, 2 * D:2 * D + 64] == 7.0).all())
+
+
 def test_another_stream_and_a_replayed_graph(ffk):
     """Ranges, forward and backward captured once and replayed on new inputs, eager calls between the replays."""
     B, S, H, KH, D = 2, 300, 4, 2, 64
