@@ -108,6 +108,13 @@ __device__ __forceinline__ void write_padding(MaskedAttnParams const &p, int b, 
   for (int row = first + t; row < p.padded_rows; row += 256) write_row(p, b, kh, row, 0.0f, 0.0f, 1 << 30, 0, 0.0f, 0);
 }
 
+// bf16: the longest window of keys in which a workgroup of the dQ kernels takes delta from P and dP themselves, in a pass over
+// the keys of its own, in place of from O as it was stored.  O's rounding reaches dS times what a single key holds of O: rows of few
+// keys lose most (dQ and dK of 5 causal tokens with scores to 12: 0.006 of their size off, 0.0027 from P and dP; of
+// 300 tokens 0.0038).  The pass costs two products more: up to 128 keys nothing that a call shows, up to 256 a fifth of
+// dQ for documents of that length (8 x 512 tokens, 16 heads of 64: 21 and 25 us).
+constexpr int kExactDelta = 128;
+
 // ---- one step of 16 of a product, for either type -------------------------
 template <typename T>
 struct Frag;

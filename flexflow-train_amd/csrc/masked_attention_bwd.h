@@ -2,7 +2,7 @@
 // Templates that masked_attention_bwd_*.hip instantiate, so that they compile side by side.
 //
 // Two kernels without atomics, both of which compute P again from the saved log-sum-exp.  The dQ kernel owns 32 RG rows
-// and runs over the keys in their ranges; it also leaves delta = rowsum(O dO) and, for every 32 rows, a summary of their
+// and runs over the keys in their ranges; it also leaves delta = rowsum(O dO) = rowsum(P dP) and, for every 32 rows, a summary of their
 // ranges in memory for the dK/dV kernel, which runs behind it.  That one owns 128 keys of one key head, 32 to a wave, and
 // runs over the rows of all query heads that read it, without the tiles of rows that see none of its keys.
 //   Both kernels together: bf16 heads of 256, 4 x 2000 tokens, 8 heads on 4, causal 742 us (0.22 PFLOP/s of the gradient's
@@ -32,6 +32,7 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
   constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ int window[2][4];
+  __shared__ float delta_parts[4][32];
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
   int const wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int const qw = wave / KW, kw = wave % KW;
@@ -91,7 +92,6 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
   }
   delta += __shfl_xor(delta, 32, 64);
   float const lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + qi] * kLog2e - p.shift;
-  if (h32 == 0 && kw == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope, position);
   if (rb == nrb - 1) write_padding(p, b, kh, nrb * 32 * RG, t);
 
   f32x16 dq[DP / 32];
@@ -112,64 +112,89 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
     tv.store(v_tile(buf), C::kVS, p.Dv, t);
   };
   int const koff = lane_k_off(C::kKS, lane), voff = lane_k_off(C::kVS, lane), toff = turn_off<T>(C::kKS, lane);
-  if (ntiles > 0) {
-    fetch(lo_all);
-    stash(0);
-  }
-  __syncthreads();
-  int cur = 0;
-  for (int it = 0; it < ntiles; it++) {
-    bool const more = it + 1 < ntiles;
-    if (more) fetch(lo_all + (it + 1) * C::kT);
-    int const kv0 = lo_all + it * C::kT + kw * 32;
-    if (kv0 < w_hi_max && kv0 + 32 > w_lo_min) {
-      T const *kt = k_tile(cur) + kw * 32 * C::kKS, *vt = v_tile(cur) + kw * 32 * C::kVS + voff;
-      f32x16 s, dp;
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        s[r] = 0.0f;
-        dp[r] = 0.0f;
-      }
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; kk++) {
-        mma(s, frag_lds(kt + koff + kk * 16), qf[kk]);
-        mma(dp, frag_lds(vt + kk * 16), gf[kk]);
-      }
-      float ds[16];
-      bool const whole = kv0 >= w_lo_max && kv0 + 32 <= w_hi_min;
-      float const distance = (float)(position - (kv0 + 4 * h32));
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        float const y = capped<T, kCap>(p, s[r]);
-        float x = y;
-        if constexpr (kBias) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
-        ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
-        if constexpr (kCap) ds[r] *= capped_slope<T>(y);
-      }
-      if (!whole) {
+  float delta_sum = 0.0f;
+  // all keys; DELTA: the sum of P dP alone
+  auto all_tiles = [&](auto delta_tag) __attribute__((always_inline)) {
+    constexpr bool DELTA = decltype(delta_tag)::value;
+    if (ntiles > 0) {
+      fetch(lo_all);
+      stash(0);
+    }
+    __syncthreads();
+    int cur = 0;
+    for (int it = 0; it < ntiles; it++) {
+      bool const more = it + 1 < ntiles;
+      if (more) fetch(lo_all + (it + 1) * C::kT);
+      int const kv0 = lo_all + it * C::kT + kw * 32;
+      if (kv0 < w_hi_max && kv0 + 32 > w_lo_min) {
+        T const *kt = k_tile(cur) + kw * 32 * C::kKS, *vt = v_tile(cur) + kw * 32 * C::kVS + voff;
+        f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          int const kv = kv0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
-          if (kv < lo || kv >= hi) ds[r] = 0.0f;
+          s[r] = 0.0f;
+          dp[r] = 0.0f;
+        }
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; kk++) {
+          mma(s, frag_lds(kt + koff + kk * 16), qf[kk]);
+          mma(dp, frag_lds(vt + kk * 16), gf[kk]);
+        }
+        float ds[16];
+        bool const whole = kv0 >= w_lo_max && kv0 + 32 <= w_hi_min;
+        float const distance = (float)(position - (kv0 + 4 * h32));
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          float const y = capped<T, kCap>(p, s[r]);
+          float x = y;
+          if constexpr (kBias) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
+          ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (DELTA ? dp[r] : dp[r] - delta);
+          if constexpr (kCap && !DELTA) ds[r] *= capped_slope<T>(y);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            int const kv = kv0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
+            if (kv < lo || kv >= hi) ds[r] = 0.0f;
+          }
+        }
+        if constexpr (DELTA) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) delta_sum += ds[r];
+        } else {
+#pragma unroll
+          for (int s2 = 0; s2 < 2; s2++) {
+            Frag<T> const df = frag_acc(ds + 8 * s2, kp);
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) mma(dq[i], frag_turned(kt + toff, C::kKS, s2, i * 32), df);
+          }
         }
       }
-#pragma unroll
-      for (int s2 = 0; s2 < 2; s2++) {
-        Frag<T> const df = frag_acc(ds + 8 * s2, kp);
-#pragma unroll
-        for (int i = 0; i < DP / 32; i++) mma(dq[i], frag_turned(kt + toff, C::kKS, s2, i * 32), df);
+      if constexpr (C::kBuffers == 2) {
+        if (more) stash(cur ^ 1);
+        __syncthreads();
+        cur ^= 1;
+      } else {
+        __syncthreads();
+        if (more) stash(0);
+        __syncthreads();
       }
     }
-    if constexpr (C::kBuffers == 2) {
-      if (more) stash(cur ^ 1);
-      __syncthreads();
-      cur ^= 1;
-    } else {
-      __syncthreads();
-      if (more) stash(0);
-      __syncthreads();
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (ntiles > 0 && hi_all - lo_all <= kExactDelta) {  // uniform
+      all_tiles(std::true_type{});
+      delta = delta_sum + __shfl_xor(delta_sum, 32, 64);
+      if constexpr (KW > 1) {
+        if (lane < 32) delta_parts[wave][lane] = delta;
+        __syncthreads();
+        delta = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; w++) delta += delta_parts[qw * KW + w][lane & 31];
+      }
     }
   }
+  if (h32 == 0 && kw == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope, position);
+  all_tiles(std::false_type{});
 
   if constexpr (KW > 1) {
     float *const area = reinterpret_cast<float *>(pool);

@@ -6,8 +6,8 @@
 // 16-byte chunks of a row that keeps both ways of reading them free of bank conflicts (that of the dK/dV kernel).  Like
 // the general kernel it leaves delta, the log-sum-exp and the ranges of its rows in memory for the dK/dV kernel, and
 // summaries of the ranges.
-//   Bound by the issue of vector instructions: 8192 tokens, 16 heads of 128, causal, biased 411 us (1.00 PFLOP/s with
-// its three products); 4 x 4096 tokens in 3 documents, 32 heads of 128 on 8, causal, capped 475 us; 8 x 512 tokens in
+//   Bound by the issue of vector instructions: 8192 tokens, 16 heads of 128, causal, biased 420 us (0.98 PFLOP/s with
+// its three products); 4 x 4096 tokens in 3 documents, 32 heads of 128 on 8, causal, capped 490 us; 8 x 512 tokens in
 // 4 documents, 16 heads of 64 21 us.
 #include "masked_attention_heads.h"
 
@@ -65,14 +65,13 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
 #pragma unroll
     for (int e = 0; e < 8; e++) part += (float)of[e] * (float)gf[kk][e];
   }
-  float const delta = part + __shfl_xor(part, 32, 64);
+  float delta = part + __shfl_xor(part, 32, 64);
   float const lse2 = p.lse[((int64_t)b * p.H + head) * p.Sq + qi] * kLog2e - p.shift;
   float slope = 0.0f;
   if constexpr (BIAS) slope = p.slopes[head] * p.slope_unit;
   int const position = p.q_offset + qi;
 
   int const w_lo_min = wave_min_int(lo), w_hi_max = wave_max_int(hi), w_lo_max = wave_max_int(lo), w_hi_min = wave_min_int(hi);
-  if (h32 == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope, position);
   if (lane == 0) {
     window[0][wave] = w_lo_min;
     window[1][wave] = w_hi_max;
@@ -150,6 +149,14 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
   wait_all_vmem_known_to_compiler();
   __syncthreads();
   // 32 keys: S^T = K Q^T, dP^T = V dO^T (rows = keys, column = row), dS, dQ^T += K^T dS^T
+  bool const exact = ntiles > 0 && ntiles * C::kKeys <= kExactDelta;  // uniform
+  // A first pass over the keys then sums P dP; what it leaves in the accumulators is cleared.  (One body for both passes: a
+  // second one, or a way around its products, takes registers that are not there.)
+  bool first_pass = exact;
+  if (exact) {
+    part = 0.0f;
+    delta = 0.0f;
+  }
   auto half_work = [&](int kv0, bf16 const *kt, bf16 const *vt) __attribute__((always_inline)) {
     f32x16 s, dp;
 #pragma unroll
@@ -164,14 +171,25 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
     }
     int const kv_first = kv0 + 4 * h32;
     float const distance = (float)(position - kv_first);
-    float ds[16];
+    float ds[16], y[16];
 #pragma unroll
     for (int r = 0; r < 16; r++) {
-      float const y = capped<bf16, CAP>(p, s[r]);
-      float x = y;
+      y[r] = capped<bf16, CAP>(p, s[r]);
+      float x = y[r];
       if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
       ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
-      if constexpr (CAP) ds[r] *= capped_slope<bf16>(y);
+    }
+    if (first_pass) {  // uniform
+      int const from = lo - kv_first, to = hi - kv_first;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        int const kv = 8 * (r >> 2) + (r & 3);
+        part += kv < from || kv >= to ? 0.0f : ds[r];
+      }
+    }
+    if constexpr (CAP) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) ds[r] *= capped_slope<bf16>(y[r]);
     }
     if (kv0 < w_lo_max || kv0 + 32 > w_hi_min) {
       int const from = lo - kv_first, to = hi - kv_first;
@@ -194,18 +212,31 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
   auto tile_step = [&](int it, auto buffer_tag) __attribute__((always_inline)) {
     constexpr int cur = decltype(buffer_tag)::value;
     int const kv0 = lo_all + it * C::kKeys;
-    if (it + 1 < ntiles) issue_tile(kv0 + C::kKeys, cur ^ 1);
+    // behind the last tile of the first pass the first one again
+    bool const more = it + 1 < ntiles;
+    if (more || first_pass) issue_tile(more ? kv0 + C::kKeys : lo_all, cur ^ 1);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       if (kv0 + 32 * h < w_hi_max && kv0 + 32 * h + 32 > w_lo_min) half_work(kv0 + 32 * h, Ks[cur] + h * 32 * D, Vs[cur] + h * 32 * D);
     }
     wait_vmcnt<0>();  // this wave's part of the next tile has landed
     __syncthreads();
+    if (!more && first_pass) {
+      first_pass = false;
+      delta = part + __shfl_xor(part, 32, 64);
+#pragma unroll
+      for (int i = 0; i < U / 32; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) dq[i][r] = 0.0f;
+    }
   };
-  for (int it = 0; it < ntiles; it += 2) {
-    tile_step(it, std::integral_constant<int, 0>{});
-    if (it + 1 < ntiles) tile_step(it + 1, std::integral_constant<int, 1>{});
+  // two passes over the keys are one run of tiles, of which the second half begins again
+  int const steps = exact ? 2 * ntiles : ntiles;
+  for (int n = 0; n < steps; n += 2) {
+    tile_step(n < ntiles ? n : n - ntiles, std::integral_constant<int, 0>{});
+    if (n + 1 < steps) tile_step(n + 1 < ntiles ? n + 1 : n + 1 - ntiles, std::integral_constant<int, 1>{});
   }
+  if (h32 == 0) write_row(p, b, kh, row, lse2, delta, lo, hi, slope, position);
   if (row < p.R) {
     bf16 *dqp = static_cast<bf16 *>(p.dq) + q_at;
 #pragma unroll

@@ -228,6 +228,26 @@ def test_heads_of_other_sizes(ffk, D, Dv, cap, bias):
             check(lse[:, :H // 2].contiguous(), want, "lse")
 
 
+@pytest.mark.parametrize("S,D", [(2, 64), (5, 32), (9, 256), (33, 128), (100, 80)])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (50.0, True)])
+def test_gradients_of_few_keys(ffk, S, D, cap, bias):
+    """bf16 rows with their probability on few keys: dQ and dK have the roundings of dS and of the result, two of at most 2^-8 a
+    value, spread evenly and apart: sqrt(2 / 3) 2^-8 = 0.0032 of their length, and not that of the stored O besides (which
+    left 0.006)."""
+    q, k, v, d_o = make(S, 8, S, S, 4, 4, D, D, BF, std=3.0)
+    slopes = slopes_of(4) if bias else None
+    want = attention(q, k, v, D ** -0.5, True, cap, None, slopes, 0, d_o, UNIT[BF])
+    for variant in (1, 0):
+        ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, variant)
+        try:
+            got = run(ffk, q, k, v, d_o, D ** -0.5, causal=True, score_cap=cap, distance_slopes=slopes)
+        finally:
+            ffk.set_option(ffk.OPTION_ATTENTION_VARIANT, 0)
+        for name in ("dq", "dk"):
+            off = float((got[name].cpu().double() - want[name]).norm() / want[name].norm())
+            assert off <= 0.0032, (name, variant, off)
+
+
 def test_ranges_and_causal_both_apply(ffk):
     q, k, v, d_o = make(4, 1, 200, 200, 2, 2, 64, 64, BF)
     ranges = torch.tensor([[[i // 2, 200] for i in range(200)]], dtype=torch.int32).cuda()
