@@ -311,7 +311,8 @@ def run(state):
     if own:
         ffk = _ffk()
         if st["op"] == "ranges":
-            return ffk.attention_key_ranges(st["batch"], st["seq"], st["seq"], causal=st["causal"], document_starts=st["starts"], prefix_lengths=st["prefixes"])
+            return ffk.attention_key_ranges(st["batch"], st["seq"], st["seq"], causal=st["causal"], document_starts=st["starts"],
+                                            prefix_lengths=st["prefixes"] if st["causal"] else None)  # all is seen already
         if st["op"] == "rotary":
             q, k = ffk.rotary_forward(st["q"], st["k"], st["positions"], st["frequencies"], st["sections_list"], interleaved=st["interleaved"])
             dq, dk = ffk.rotary_backward(st["dq"], st["dk"], st["positions"], st["frequencies"], st["sections_list"], interleaved=st["interleaved"])
