@@ -7,6 +7,11 @@
 //   P = softmax over the seen keys, O = P V, lse = log sum exp(s); a row that sees nothing: O = 0, lse = -inf
 //   delta_i = O_i . dO_i     dS = P (dO V^T - delta)     dX = dS (1 - tanh^2) scale
 //   dQ = dX K      dK = dX^T Q, dV = P^T dO, summed over the G heads that read the key head
+// A row that sees one key has P = 1 whatever its score, so dS = 0.  dP and delta, sums of the same products in different
+// orders, would leave some 2^-23 of |dO| |v| in its place, and all of dQ and dK of sequences of one position is nothing else.
+// So the dQ kernels let such a row see nothing where dS is masked (score_range), and the dK/dV kernels correct P and dS of
+// the tiles that have one, or, for heads, clear its Q in LDS, which with what write_row leaves of it gives P = 1.  No
+// instruction for it in a loop (a comparison a score took 3% of a capped pass over 4 x 4096 tokens).
 //
 // The G query heads of a key head are one longer axis of rows, r = i G + g: they share the tiles of K and V that a
 // workgroup brings into LDS, the keys' gradients are sums over that one axis (no atomics), and a few query rows still
@@ -24,7 +29,7 @@ namespace ffk {
 // Rows that a summary of ranges covers: the dQ kernels write one for every 32 rows, the dK/dV kernels skip by them.
 struct RangeSummary {
   int lo_min, hi_max;  // every key that some row sees lies in [lo_min, hi_max)
-  int lo_max, hi_min;  // every row sees all of [lo_max, hi_min)
+  int lo_max, hi_min;  // every row sees all of [lo_max, hi_min); nothing is, with (1 << 30) for lo_max, where a row sees one key
 };
 
 // What the dQ kernels leave in memory of every row for the dK/dV kernels: arrays of padded_rows entries, one set for each
@@ -89,17 +94,30 @@ __device__ __forceinline__ void row_range(MaskedAttnParams const &p, int b, int 
   }
 }
 
+// Whether a range is a single key's.
+__device__ __forceinline__ bool one_key(int lo, int hi) { return hi - lo == 1; }
+// The keys whose scores have a gradient in a row that sees [lo, hi): all of them, or none where there is one.
+__device__ __forceinline__ void score_range(int lo, int hi, int &ds_lo, int &ds_hi) {
+  ds_lo = one_key(lo, hi) ? 1 << 30 : lo;
+  ds_hi = one_key(lo, hi) ? 0 : hi;
+}
+// lo_max of a summary, of a wave whose rows see [lo, hi)
+__device__ __forceinline__ int summary_lo_max(int lo, int hi, int w_lo_max) {
+  return __builtin_amdgcn_ballot_w64(one_key(lo, hi)) != 0 ? 1 << 30 : w_lo_max;
+}
+
 __device__ __forceinline__ void write_row(MaskedAttnParams const &p, int b, int kh, int row, float lse2, float delta, int lo, int hi,
                                           float slope, int position) {
   if (row >= p.padded_rows) return;
   float *rows = p.rows + (int64_t)(b * p.KH + kh) * kRowFields * p.padded_rows + row;
   int64_t const n = p.padded_rows;
-  rows[kRowLse2 * n] = lse2;
+  bool const one = one_key(lo, hi);  // (with Q cleared y is 0, or the logistic function's 1/2: score_scale y = -shift)
+  rows[kRowLse2 * n] = one ? -p.shift : lse2;
   rows[kRowDelta * n] = delta;
   rows[kRowLo * n] = __int_as_float(lo);
   rows[kRowHi * n] = __int_as_float(hi);
   if (p.slopes != nullptr) {
-    rows[kRowSlope * n] = slope;
+    rows[kRowSlope * n] = one ? 0.0f : slope;
     rows[kRowPosition * n] = __int_as_float(position);
   }
 }

@@ -50,12 +50,15 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
     lo = 1 << 30;
     hi = 0;
   }
+  int ds_lo, ds_hi;
+  score_range(lo, hi, ds_lo, ds_hi);
   int const w_lo_min = wave_min_int(lo), w_hi_max = wave_max_int(hi), w_lo_max = wave_max_int(lo), w_hi_min = wave_min_int(hi);
+  int const s_lo_max = summary_lo_max(lo, hi, w_lo_max);
   if (lane == 0) {
     window[0][wave] = w_lo_min;
     window[1][wave] = w_hi_max;
     if (kh == 0 && kw == 0 && row0 < p.R)
-      p.summary[(int64_t)b * ((p.R + 31) / 32) + row0 / 32] = RangeSummary{w_lo_min, w_hi_max, w_lo_max, w_hi_min};
+      p.summary[(int64_t)b * ((p.R + 31) / 32) + row0 / 32] = RangeSummary{w_lo_min, w_hi_max, s_lo_max, w_hi_min};
   }
   __syncthreads();
   int const lo_all = __builtin_amdgcn_readfirstlane(min(min(window[0][0], window[0][1]), min(window[0][2], window[0][3])));
@@ -154,7 +157,7 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
 #pragma unroll
           for (int r = 0; r < 16; r++) {
             int const kv = kv0 + 8 * (r >> 2) + 4 * h32 + (r & 3);
-            if (kv < lo || kv >= hi) ds[r] = 0.0f;
+            if (kv < ds_lo || kv >= ds_hi) ds[r] = 0.0f;
           }
         }
         if constexpr (DELTA) {
@@ -431,6 +434,19 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
             if (kv < __float_as_int(lo4[e]) || kv >= __float_as_int(hi4[e])) {
               pv[4 * g + e] = 0.0f;
               if constexpr (kDk) ds[4 * g + e] = 0.0f;
+            }
+          }
+        }
+        if (sum.lo_max == 1 << 30) {  // (rows that see one key, or none)
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            f32x4 const lo4 = rows4(kRowLo, g), hi4 = rows4(kRowHi, g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              if (one_key(__float_as_int(lo4[e]), __float_as_int(hi4[e]))) {
+                pv[4 * g + e] = kv == __float_as_int(lo4[e]) ? 1.0f : 0.0f;
+                if constexpr (kDk) ds[4 * g + e] = 0.0f;
+              }
             }
           }
         }

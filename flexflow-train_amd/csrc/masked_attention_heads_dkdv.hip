@@ -11,7 +11,7 @@
 //   Which tiles: a list in LDS of those with a row that sees one of the 128 keys, from the summaries of ranges, made for
 // 512 tiles at a time.  A wave passes over a tile none of whose rows sees its 32 keys, and compares ranges element by
 // element only where not all rows see all of them.  Rows that see none of the 128 keys are cleared in LDS before use: what
-// lies in them must not meet the zeros of the masked probabilities.
+// lies in them must not meet the zeros of the masked probabilities; so is the Q of those that see one key.
 //   A tile lies in LDS as in memory, [64 rows][D], the 16-byte chunks of a row permuted on the fetching side such that
 // both ways it is read (16 bytes a lane by rows, and turned) are free of bank conflicts.
 //   8192 tokens, 16 heads of 128, causal, biased 630 us (0.87 PFLOP/s with its four products); 4 x 4096 tokens in 3 documents,
@@ -331,14 +331,19 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
       sum = list_sum[min(it + 1, count - 1)];
       bf16 *qt = Qs[cur], *gt = Gs[cur];
       float const *fields = &Rows[cur][0][0];
-      int const *row_lo = reinterpret_cast<int const *>(fields + kRowLo * 64), *row_hi = reinterpret_cast<int const *>(fields + kRowHi * 64);
-      if (lo_max >= kv0 + C::kKeys || hi_min <= kv0) {  // uniform: a row here sees none of the keys
-        int const row = t >> 2;
-        if (row_lo[row] >= kv0 + C::kKeys || row_hi[row] <= kv0) {
+      if (lo_max >= kv0 + C::kKeys || hi_min <= kv0) {  // uniform: a row here sees none of the keys, or one alone
+        int at = t;
+        // Nothing of the addresses below is held in registers through the loop: with it heads of 64 pass the 256 that leave a
+        // SIMD two waves (a pass over 8 x 512 tokens in 4 documents 73 us, and 64).
+        asm volatile("" : "+v"(at));
+        int const row = at >> 2, row_lo = __float_as_int(fields[kRowLo * 64 + row]), row_hi = __float_as_int(fields[kRowHi * 64 + row]);
+        bool const none = row_lo >= kv0 + C::kKeys || row_hi <= kv0;
+        if (none || one_key(row_lo, row_hi)) {
 #pragma unroll
           for (int c = 0; c < D / 32; c++) {
-            *reinterpret_cast<u32x4 *>(qt + row * D + (c * 4 + (t & 3)) * 8) = u32x4{0u, 0u, 0u, 0u};
-            *reinterpret_cast<u32x4 *>(gt + row * D + (c * 4 + (t & 3)) * 8) = u32x4{0u, 0u, 0u, 0u};
+            int const chunk = row * D + (c * 4 + (at & 3)) * 8;
+            *reinterpret_cast<u32x4 *>(qt + chunk) = u32x4{0u, 0u, 0u, 0u};
+            if (none) *reinterpret_cast<u32x4 *>(gt + chunk) = u32x4{0u, 0u, 0u, 0u};
           }
         }
         __syncthreads();

@@ -49,6 +49,8 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
     lo = 1 << 30;
     hi = 0;
   }
+  int ds_lo, ds_hi;
+  score_range(lo, hi, ds_lo, ds_hi);
   int64_t const q_at = (int64_t)b * p.q_bs + (int64_t)qi * p.q_ss + (int64_t)head * dim_qk;
   int64_t const o_at = (int64_t)b * p.o_bs + (int64_t)qi * p.o_ss + (int64_t)head * dim_v;
   bf16 const *qp = static_cast<bf16 const *>(p.q) + q_at, *gp = static_cast<bf16 const *>(p.d_o) + o_at;
@@ -72,11 +74,12 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
   int const position = p.q_offset + qi;
 
   int const w_lo_min = wave_min_int(lo), w_hi_max = wave_max_int(hi), w_lo_max = wave_max_int(lo), w_hi_min = wave_min_int(hi);
+  int const s_lo_max = summary_lo_max(lo, hi, w_lo_max);
   if (lane == 0) {
     window[0][wave] = w_lo_min;
     window[1][wave] = w_hi_max;
     if (kh == 0 && row0 < p.R)
-      p.summary[(int64_t)b * ((p.R + 31) / 32) + row0 / 32] = RangeSummary{w_lo_min, w_hi_max, w_lo_max, w_hi_min};
+      p.summary[(int64_t)b * ((p.R + 31) / 32) + row0 / 32] = RangeSummary{w_lo_min, w_hi_max, s_lo_max, w_hi_min};
   }
   __syncthreads();
   int const lo_all = __builtin_amdgcn_readfirstlane(min(min(window[0][0], window[0][1]), min(window[0][2], window[0][3])));
@@ -180,7 +183,7 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
       ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
     }
     if (first_pass) {  // uniform
-      int const from = lo - kv_first, to = hi - kv_first;
+      int const from = ds_lo - kv_first, to = ds_hi - kv_first;
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         int const kv = 8 * (r >> 2) + (r & 3);
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
       for (int r = 0; r < 16; r++) ds[r] *= capped_slope<bf16>(y[r]);
     }
     if (kv0 < w_lo_max || kv0 + 32 > w_hi_min) {
-      int const from = lo - kv_first, to = hi - kv_first;
+      int const from = ds_lo - kv_first, to = ds_hi - kv_first;
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         int const kv = 8 * (r >> 2) + (r & 3);
