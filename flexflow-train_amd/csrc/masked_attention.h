@@ -50,12 +50,12 @@ struct MaskedAttnParams {
   int padded_rows;                      // R up to whole tiles of 64
   int64_t q_bs, q_ss, k_bs, k_ss, v_bs, v_ss, o_bs, o_ss;
   int q_offset;
-  // A score in powers of two is  score_scale y + shift,  y = capped<T>(raw) - slope_unit slope_h |p_i - j|  (see capped);
+  // A score in powers of two is  score_scale y + shift,  y = capped(raw) - slope_unit slope_h |p_i - j|  (see capped);
   // its derivative by the raw product, over ln 2, is score_scale times the derivative of capped.  What is the same for
   // all scores of a row is taken out of the loops: the shift goes into the log-sum-exp, the gradients' factor to their store.
   float score_scale, shift, slope_unit, grad_scale;
   float cap_in;
-  int capped, causal;
+  int capped, causal;  // capped: how (see capped)
   FastDiv group, heads_div, places_div;  // by G, KH and KH B
   // forward, split over the keys: partial O (unnormalised), maximum and sum of each part
   int splits;
@@ -240,26 +240,41 @@ struct TileRegs {
   }
 };
 
-// The cap's part of a score that is not linear, and its derivative (1 without a cap, where y is the raw product).
-//   fp32: y = tanh(scale raw / cap), score_scale = cap log2(e), derivative 1 - y^2.
-//   bf16: y = 1 / (1 + 2^(cap_in raw)), cap_in = -2 log2(e) scale / cap, on the hardware's exponential and reciprocal: tanh is
-//   2 y - 1, so score_scale = 2 cap log2(e), shift = -cap log2(e), and 1 - tanh^2 = 4 (y - y^2), of which grad_scale has the
-//   4.  Four vector instructions a score and two for the derivative; about 2^-22 off in absolute terms, which the cap
-//   multiplies to a few 1e-6 of a score, far below what bf16 scores carry.  (fp32's products take sixteen times as long: it
-//   can have the library's tanh.)
-template <typename T, bool CAP>
+// The cap's part of a score that is not linear, and its derivative (1 without a cap, where y is the raw product), two ways.
+//   kCapTanh: y = tanh(scale raw / cap), score_scale = cap log2(e), derivative 1 - y^2, by the library's tanh, a few 2^-24 of
+//   itself off.
+//   kCapLogistic: y = 1 / (1 + 2^(cap_in raw)), cap_in = -2 log2(e) scale / cap, on the hardware's exponential and reciprocal:
+//   tanh is 2 y - 1, so score_scale = 2 cap log2(e), shift = -cap log2(e), and 1 - tanh^2 = 4 (y - y^2), of which grad_scale has
+//   the 4.  Four vector instructions a score and two for the derivative.  Scores next to nothing are next to y = 1/2, where a
+//   step of y is 2^-24, so this one is off by up to about 2^-22 cap whatever the score.
+// bf16 takes the second up to a cap of kLogisticCap, 3e-5 of a score there and 1e-5 at 50, far below what bf16 scores carry;
+// past it (at 10^5 scores would be 0.01 off, at 10^8 all the same) the first one, in the general kernels: 4 x 2048 tokens,
+// 16 heads of 128 on 4, causal, 1003 us with gradients, and 506 at a cap of 100.  fp32 takes the first: its products take
+// sixteen times as long.
+enum { kNoCap = 0, kCapLogistic = 1, kCapTanh = 2 };
+constexpr float kLogisticCap = 128.0f;
+template <int CAP>
 __device__ __forceinline__ float capped(MaskedAttnParams const &p, float raw) {
-  if constexpr (!CAP) {
-    return raw;
-  } else if constexpr (sizeof(T) == 2) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * p.cap_in));
-  } else {
-    return tanhf(raw * p.cap_in);
-  }
+  if constexpr (CAP == kNoCap) return raw;
+  else if constexpr (CAP == kCapLogistic) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * p.cap_in));
+  else return tanhf(raw * p.cap_in);
 }
-template <typename T>
+template <int CAP>
 __device__ __forceinline__ float capped_slope(float y) {
-  return sizeof(T) == 2 ? __builtin_fmaf(-y, y, y) : __builtin_fmaf(-y, y, 1.0f);
+  return CAP == kCapLogistic ? __builtin_fmaf(-y, y, y) : __builtin_fmaf(-y, y, 1.0f);
+}
+
+// The general kernels' instances: launch(how the score is capped, and 4 with a bias).
+template <typename T, typename LAUNCH>
+static hipError_t masked_by_score(MaskedAttnParams const &p, LAUNCH launch) {
+  auto const either = [&](auto cap) {
+    constexpr int kCap = decltype(cap)::value;
+    return p.slopes != nullptr ? launch(std::integral_constant<int, kCap | 4>{}) : launch(std::integral_constant<int, kCap>{});
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (p.capped == kCapLogistic) return either(std::integral_constant<int, kCapLogistic>{});
+  }
+  return p.capped != kNoCap ? either(std::integral_constant<int, kCapTanh>{}) : either(std::integral_constant<int, kNoCap>{});
 }
 
 // A wave's smallest and largest of an integer, scalar.

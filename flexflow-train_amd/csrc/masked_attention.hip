@@ -121,6 +121,7 @@ static int padded_head(ffk_masked_attention_desc_t const *d) {
 static int64_t rows_of(ffk_masked_attention_desc_t const *d) { return d->seq_q * (d->heads / d->kv_heads); }
 
 static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype);
+static bool logistic_cap(ffk_masked_attention_desc_t const *d, int dtype) { return dtype == FFK_BF16 && d->score_cap <= kLogisticCap; }
 // Workgroups of 128 rows or keys below which those of 32, whose four waves share out the other axis, are better.  fp32, bound
 // by its products: as many as CUs (two sequences of 1000 tokens, 8 heads of 64 on 4, causal, 128 workgroups: forward 87 us, and
 // 38 with 32 rows, backward 219 and 153; four sequences, 256 workgroups, not causal, 86 and 116, 285 and 367).  bf16: half as
@@ -206,15 +207,15 @@ static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, int dtyp
   p.v_bs = d->v_batch_stride; p.v_ss = d->v_seq_stride;
   p.o_bs = d->o_batch_stride; p.o_ss = d->o_seq_stride;
   p.q_offset = (int)d->query_offset;
-  p.capped = d->score_cap != 0.0f;
+  p.capped = d->score_cap == 0.0f ? kNoCap : logistic_cap(d, dtype) ? kCapLogistic : kCapTanh;
   p.score_scale = d->scale * kLog2e;
   p.grad_scale = d->scale;
-  if (p.capped && dtype == FFK_BF16) {
+  if (p.capped == kCapLogistic) {
     p.cap_in = -2.0f * kLog2e * (d->scale / d->score_cap);
     p.score_scale = 2.0f * kLog2e * d->score_cap;
     p.shift = -kLog2e * d->score_cap;
     p.grad_scale = 4.0f * d->scale;
-  } else if (p.capped) {
+  } else if (p.capped == kCapTanh) {
     p.cap_in = d->scale / d->score_cap;
     p.score_scale = kLog2e * d->score_cap;
   }
@@ -237,10 +238,11 @@ static size_t backward_bytes(ffk_masked_attention_desc_t const *d) {
 }
 
 // The kernels of masked_attention_heads_*.hip: bf16, head sizes up to 128 (64 and 128 themselves, others made longer with
-// zeros), rows that byte offsets below 2^31 reach (of all rows of an entry in the dK/dV kernel, of a tile in the others).
+// zeros), no cap or one by the logistic function, rows that byte offsets below 2^31 reach (of all rows of an entry in the dK/dV
+// kernel, of a tile in the others).
 static bool heads_kernels(ffk_masked_attention_desc_t const *d, int dtype) {
   int64_t const lim = (int64_t)1 << 31;
-  return dtype == FFK_BF16 && padded_head(d) <= 128 && d->k_seq_stride < (1 << 24) && d->v_seq_stride < (1 << 24) &&
+  return dtype == FFK_BF16 && padded_head(d) <= 128 && logistic_cap(d, dtype) && d->k_seq_stride < (1 << 24) && d->v_seq_stride < (1 << 24) &&
          d->seq_q * d->q_seq_stride * 2 < lim && d->seq_q * d->o_seq_stride * 2 < lim;
 }
 // 32-key groups of a workgroup of the general dK/dV kernel, and whether it is to run in place of the one for heads: 4, or 1

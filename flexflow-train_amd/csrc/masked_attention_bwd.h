@@ -29,7 +29,8 @@ template <typename T, int DP, int RG, int EXTRA>
 __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
   using C = MaskedDq<T, DP, RG>;
   constexpr int KW = C::kKW;
-  constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
+  constexpr int kCap = EXTRA & 3;  // kNoCap, kCapLogistic or kCapTanh
+  constexpr bool kBias = (EXTRA & 4) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ int window[2][4];
   __shared__ float delta_parts[4][32];
@@ -147,11 +148,11 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
         float const distance = (float)(position - (kv0 + 4 * h32));
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          float const y = capped<T, kCap>(p, s[r]);
+          float const y = capped<kCap>(p, s[r]);
           float x = y;
           if constexpr (kBias) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
           ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (DELTA ? dp[r] : dp[r] - delta);
-          if constexpr (kCap && !DELTA) ds[r] *= capped_slope<T>(y);
+          if constexpr (kCap != kNoCap && !DELTA) ds[r] *= capped_slope<kCap>(y);
         }
         if (!whole) {
 #pragma unroll
@@ -257,7 +258,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
   // bf16 past 128 columns: the accumulators, half of a lane's registers, stay in accumulation registers, so that the other
   // half holds operands read ahead
   constexpr bool kKept = sizeof(T) == 2 && DP > 128;
-  constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
+  constexpr int kCap = EXTRA & 3;  // kNoCap, kCapLogistic or kCapTanh
+  constexpr bool kBias = (EXTRA & 4) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ __attribute__((aligned(16))) float stats[C::kBuffers][kRowFields][kT];  // integers by their bits
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
@@ -415,13 +417,13 @@ __global__ __launch_bounds__(256) void masked_dkdv_kernel(MaskedAttnParams p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           int const r = 4 * g + e;
-          float const y = capped<T, kCap>(p, s[r]);
+          float const y = capped<kCap>(p, s[r]);
           float x = y;
           if constexpr (kBias) x = __builtin_fmaf(-slope4[e], (float)abs(__float_as_int(position4[e]) - kv), x);
           pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse4[e]));
           if constexpr (kDk) {
             ds[r] = pv[r] * (dp[r] - delta4[e]);
-            if constexpr (kCap) ds[r] *= capped_slope<T>(y);
+            if constexpr (kCap != kNoCap) ds[r] *= capped_slope<kCap>(y);
           }
         }
       }
@@ -560,20 +562,12 @@ static hipError_t masked_dkdv_launch_as(hipStream_t st, MaskedAttnParams const &
 
 template <typename T, int DP, int RG>
 static hipError_t masked_dq_launch(hipStream_t st, MaskedAttnParams const &p) {
-  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
-  return cap && bias ? masked_dq_launch_as<T, DP, RG, 3>(st, p)
-         : cap       ? masked_dq_launch_as<T, DP, RG, 1>(st, p)
-         : bias      ? masked_dq_launch_as<T, DP, RG, 2>(st, p)
-                     : masked_dq_launch_as<T, DP, RG, 0>(st, p);
+  return masked_by_score<T>(p, [&](auto extra) { return masked_dq_launch_as<T, DP, RG, decltype(extra)::value>(st, p); });
 }
 
 template <typename T, int DP, int KG, int WHAT>
 static hipError_t masked_dkdv_launch(hipStream_t st, MaskedAttnParams const &p) {
-  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
-  return cap && bias ? masked_dkdv_launch_as<T, DP, KG, WHAT, 3>(st, p)
-         : cap       ? masked_dkdv_launch_as<T, DP, KG, WHAT, 1>(st, p)
-         : bias      ? masked_dkdv_launch_as<T, DP, KG, WHAT, 2>(st, p)
-                     : masked_dkdv_launch_as<T, DP, KG, WHAT, 0>(st, p);
+  return masked_by_score<T>(p, [&](auto extra) { return masked_dkdv_launch_as<T, DP, KG, WHAT, decltype(extra)::value>(st, p); });
 }
 
 }  // namespace ffk

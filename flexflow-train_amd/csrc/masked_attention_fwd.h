@@ -29,7 +29,8 @@ template <typename T, int DP, int RG, int EXTRA>
 __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
   using C = MaskedFwd<T, DP, RG>;
   constexpr int J = C::kJ, KW = C::kKW;
-  constexpr bool kCap = (EXTRA & 1) != 0, kBias = (EXTRA & 2) != 0;
+  constexpr int kCap = EXTRA & 3;  // kNoCap, kCapLogistic or kCapTanh
+  constexpr bool kBias = (EXTRA & 4) != 0;
   extern __shared__ __attribute__((aligned(16))) uint8_t pool[];
   __shared__ int window[2][4];
   int const t = threadIdx.x, lane = t & 63, h32 = lane >> 5;
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedAttnParams p) {
       for (int j = 0; j < J; j++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          s[j][r] = capped<T, kCap>(p, s[j][r]);
+          s[j][r] = capped<kCap>(p, s[j][r]);
           if constexpr (kBias) s[j][r] = __builtin_fmaf(-slope, fabsf(distance - (float)(j * 32 + 8 * (r >> 2) + (r & 3))), s[j][r]);
         }
       if (kv0 < w_lo_max || kv0 + 32 * J > w_hi_min) {
@@ -266,11 +267,7 @@ static hipError_t masked_fwd_launch_as(hipStream_t st, MaskedAttnParams const &p
 
 template <typename T, int DP, int RG>
 static hipError_t masked_fwd_launch(hipStream_t st, MaskedAttnParams const &p) {
-  bool const cap = p.capped != 0, bias = p.slopes != nullptr;
-  return cap && bias ? masked_fwd_launch_as<T, DP, RG, 3>(st, p)
-         : cap       ? masked_fwd_launch_as<T, DP, RG, 1>(st, p)
-         : bias      ? masked_fwd_launch_as<T, DP, RG, 2>(st, p)
-                     : masked_fwd_launch_as<T, DP, RG, 0>(st, p);
+  return masked_by_score<T>(p, [&](auto extra) { return masked_fwd_launch_as<T, DP, RG, decltype(extra)::value>(st, p); });
 }
 
 }  // namespace ffk

@@ -182,8 +182,8 @@ __global__ __launch_bounds__(256) void masked_dkdv_heads_kernel(MaskedAttnParams
       if constexpr (CAP && k == 0) s[h][u] *= p.cap_in;
       if constexpr (CAP && k == 1) s[h][u] = __builtin_amdgcn_exp2f(s[h][u]);
       if constexpr (CAP && k == 2) s[h][u] += 1.0f;
-      if constexpr (CAP && k == 3) s[h][u] = __builtin_amdgcn_rcpf(s[h][u]);  // capped<bf16, true>
-      if constexpr (k == kScore && CAP) y[h][u] = __builtin_fmaf(-s[h][u], s[h][u], s[h][u]);  // capped_slope<bf16>
+      if constexpr (CAP && k == 3) s[h][u] = __builtin_amdgcn_rcpf(s[h][u]);  // capped<kCapLogistic>
+      if constexpr (k == kScore && CAP) y[h][u] = __builtin_fmaf(-s[h][u], s[h][u], s[h][u]);  // capped_slope<kCapLogistic>
       if constexpr (k == kScore && BIAS) s[h][u] = __builtin_fmaf(-srow[h][g][e], fabsf(far[h][u]), s[h][u]);
       if constexpr (k == kScore + kBias) s[h][u] = __builtin_fmaf(s[h][u], p.score_scale, -lrow[h][g][e]);
       if constexpr (k == kScore + kBias) dp[h][u] -= drow[h][g][e];

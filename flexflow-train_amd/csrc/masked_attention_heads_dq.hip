@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
     float ds[16], y[16];
 #pragma unroll
     for (int r = 0; r < 16; r++) {
-      y[r] = capped<bf16, CAP>(p, s[r]);
+      y[r] = capped<CAP ? kCapLogistic : kNoCap>(p, s[r]);
       float x = y[r];
       if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), x);
       ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.score_scale, -lse2)) * (dp[r] - delta);
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256, 2) void masked_dq_heads_kernel(MaskedAttnParam
     }
     if constexpr (CAP) {
 #pragma unroll
-      for (int r = 0; r < 16; r++) ds[r] *= capped_slope<bf16>(y[r]);
+      for (int r = 0; r < 16; r++) ds[r] *= capped_slope<kCapLogistic>(y[r]);
     }
     if (kv0 < w_lo_max || kv0 + 32 > w_hi_min) {
       int const from = ds_lo - kv_first, to = ds_hi - kv_first;

@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, 2) void masked_fwd_heads_kernel(MaskedAttnPara
       for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          s[j][r] = capped<bf16, CAP>(p, s[j][r]);
+          s[j][r] = capped<CAP ? kCapLogistic : kNoCap>(p, s[j][r]);
           if constexpr (BIAS) s[j][r] = __builtin_fmaf(-slope, fabsf(distance - (float)(j * 32 + 8 * (r >> 2) + (r & 3))), s[j][r]);
         }
     }

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(64) void masked_fwd_rows_kernel(MaskedAttnParams p)
     float const distance = (float)(position - kv_first);
 #pragma unroll
     for (int r = 0; r < 16; r++) {
-      s[r] = capped<bf16, CAP>(p, s[r]);
+      s[r] = capped<CAP ? kCapLogistic : kNoCap>(p, s[r]);
       if constexpr (BIAS) s[r] = __builtin_fmaf(-slope, fabsf(distance - (float)(8 * (r >> 2) + (r & 3))), s[r]);
     }
     if (kv0 < lo_max || kv0 + 32 > hi_min) {  // uniform: not seen whole by all rows

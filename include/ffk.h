@@ -651,6 +651,9 @@ int ffk_attention_backward(ffk_stream_t stream, int dtype,
  *   them that a row does not see has to be finite all the same (a masked
  *   probability is 0, and 0 times infinity is none).  Slopes are finite.
  *   Ranges are cut to [0, seq_kv].  distance_slopes and key_ranges have no gradient.
+ *   score_cap is any that is finite and does not vanish beside scale.  FFK_BF16: up
+ *   to 128 a capped score is within 2^-22 score_cap of its value; past that within
+ *   some 2^-22 of itself, as FFK_FLOAT's are, by kernels that take about twice as long.
  *   dtype FFK_BF16 (head sizes multiples of 8 up to 256, strides multiples of 8
  *   elements) or FFK_FLOAT (multiples of 4); 16-byte aligned tensors, key_ranges
  *   8-byte aligned.  dq, dk, dv have the strides of q, k, v and are overwritten;
