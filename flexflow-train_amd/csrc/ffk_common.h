@@ -270,27 +270,32 @@ __device__ __forceinline__ float storage_round<bf16>(float v) {
 //   row_mirror: lane i of 16 reads lane 15 - i, which lies in the other group of 8.
 // Partners always apply the commutative operation to the same two values, so the lanes agree
 // bit for bit.
-template <int CTRL>
-__device__ __forceinline__ float dpp_read(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+// T: float or int.  (Integers go as integers: a negative one's bits, passed as a float, are a NaN, which the files that are
+// compiled without NaNs do not have.)
+template <int CTRL, typename T>
+__device__ __forceinline__ T dpp_read(T v) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 // swaps the odd 16-lane rows of the first operand with the even rows of the second: with the
 // same value in both, the results hold rows {0,0,2,2} and {1,1,3,3}
-template <typename F>
-__device__ __forceinline__ float swap_rows(float v, F f) {
-  auto const a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+template <typename T, typename F>
+__device__ __forceinline__ T swap_rows(T v, F f) {
+  unsigned const u = __builtin_bit_cast(unsigned, v);
+  auto const a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return f(__builtin_bit_cast(T, (unsigned)a[0]), __builtin_bit_cast(T, (unsigned)a[1]));
 }
 // the same for the two 32-lane halves
-template <typename F>
-__device__ __forceinline__ float swap_halves(float v, F f) {
-  auto const b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+template <typename T, typename F>
+__device__ __forceinline__ T swap_halves(T v, F f) {
+  unsigned const u = __builtin_bit_cast(unsigned, v);
+  auto const b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return f(__builtin_bit_cast(T, (unsigned)b[0]), __builtin_bit_cast(T, (unsigned)b[1]));
 }
 // LANES: over aligned groups of 16 or 32 lanes instead, which leave out the last swaps.
-template <int LANES = 64, typename F>
-__device__ __forceinline__ float wave_reduce(float v, F f) {
+template <int LANES = 64, typename T, typename F>
+__device__ __forceinline__ T wave_reduce(T v, F f) {
   static_assert(LANES == 16 || LANES == 32 || LANES == 64, "rows of lanes");
+  static_assert(sizeof(T) == 4, "one register a lane");
   v = f(v, dpp_read<0xB1>(v));   // quad_perm [1,0,3,2]
   v = f(v, dpp_read<0x4E>(v));   // quad_perm [2,3,0,1]
   v = f(v, dpp_read<0x141>(v));  // row_half_mirror

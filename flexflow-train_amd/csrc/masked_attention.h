@@ -279,10 +279,11 @@ static hipError_t masked_by_score(MaskedAttnParams const &p, LAUNCH launch) {
 
 // A wave's smallest and largest of an integer, scalar.
 __device__ __forceinline__ int wave_min_int(int v) {
-  float const r = wave_reduce(__int_as_float(v), [](float a, float b) { return __int_as_float(min(__float_as_int(a), __float_as_int(b))); });
-  return __builtin_amdgcn_readfirstlane(__float_as_int(r));
+  return __builtin_amdgcn_readfirstlane(wave_reduce(v, [](int a, int b) { return min(a, b); }));
 }
-__device__ __forceinline__ int wave_max_int(int v) { return -wave_min_int(-v); }
+__device__ __forceinline__ int wave_max_int(int v) {
+  return __builtin_amdgcn_readfirstlane(wave_reduce(v, [](int a, int b) { return max(a, b); }));
+}
 
 // acc += a b on an accumulator that stays in accumulation registers: left to itself the compiler keeps some of a wave's
 // values in the wrong kind of register and moves them there and back in every tile.  It does not see that results take
