@@ -25,6 +25,7 @@ constexpr int kNormWorkgroups = 1024;  // of a launch for the norm, at most: fou
 constexpr int kNormTensors = 96;       // of a launch (the table travels as its argument)
 constexpr int64_t kNormKept = 128 << 20;  // bytes of a list up to which its tensors are to stay in the caches
 constexpr int kNormLoads = 8, kClipLoads = 4;  // 16-byte loads of a thread in a piece
+constexpr int64_t kClipPieces = (1 << 24) - 1;  // of a launch for the clipping, each a workgroup: 2^32 threads are too many
 
 // elements of a piece
 __host__ __device__ constexpr int piece_elems(int loads, bool is_bf16) { return loads * kNormThreads * (is_bf16 ? 8 : 4); }
@@ -191,7 +192,7 @@ static int check_list(char const *who, int const *dtypes, void const *const *gra
   FFK_REQUIRE(num == 0 || (dtypes != nullptr && grads != nullptr && elems != nullptr), "%s: NULL list", who);
   for (int i = 0; i < num; i++) {
     FFK_REQUIRE(dtypes[i] == FFK_FLOAT || dtypes[i] == FFK_BF16, "%s: dtype %d of tensor %d not supported (FLOAT or BF16)", who, dtypes[i], i);
-    FFK_REQUIRE(elems[i] >= 0 && elems[i] < ((int64_t)1 << 40), "%s: bad size of tensor %d", who, i);
+    FFK_REQUIRE(elems[i] >= 0 && elems[i] <= kClipPieces * piece_elems(kClipLoads, dtypes[i] == FFK_BF16), "%s: bad size of tensor %d", who, i);
     FFK_REQUIRE(elems[i] == 0 || grads[i] != nullptr, "%s: tensor %d is NULL", who, i);
     FFK_REQUIRE(reinterpret_cast<uintptr_t>(grads[i]) % dtype_size(dtypes[i]) == 0, "%s: tensor %d is not aligned to its elements", who, i);
   }
@@ -224,16 +225,17 @@ static int check_apart(char const *who, int const *dtypes, void const *const *gr
   return FFK_OK;
 }
 
-// The tensors from `first` on that one launch takes, as its table; returns the first that it does not.
+// The tensors from `first` on that one launch takes, as its table: of up to `most` pieces, which no tensor has more of.  Returns
+// the first that it does not take.
 static int fill_table(NormTable &a, int const *dtypes, void const *const *grads, void *const *out, int64_t const *elems, int num, int first,
-                      int loads) {
+                      int loads, int64_t most) {
   a.tensors = 0;
   int64_t pieces = 0;
   int i = first;
   for (; i < num && a.tensors < kNormTensors; i++) {
     if (elems[i] == 0) continue;
     int64_t const more = ceil_div(elems[i], piece_elems(loads, dtypes[i] == FFK_BF16));
-    if (a.tensors > 0 && pieces + more > (1 << 28)) break;
+    if (pieces + more > most) break;
     int const t = a.tensors++;
     a.in[t] = grads[i];
     a.out[t] = out != nullptr ? out[i] : nullptr;
@@ -252,7 +254,7 @@ static int launch_squares(hipStream_t st, int const *dtypes, void const *const *
   int64_t bytes = 0;
   for (int i = 0; i < num; i++) bytes += elems[i] * (int64_t)dtype_size(dtypes[i]);
   for (int first = 0; first < num;) {
-    first = fill_table(a, dtypes, grads, nullptr, elems, num, first, kNormLoads);
+    first = fill_table(a, dtypes, grads, nullptr, elems, num, first, kNormLoads, INT32_MAX);  // (a whole table has fewer)
     int const pieces = a.first_piece[a.tensors], grid = pieces < kNormWorkgroups ? pieces : kNormWorkgroups;
     if (grid == 0) continue;
     if (bytes <= kNormKept) square_sum_kernel<false><<<dim3((unsigned)grid), kNormThreads, 0, st>>>(a, partial + count);
@@ -276,10 +278,10 @@ static int check_workspace(char const *who, void const *workspace, size_t bytes,
 using namespace ffk;
 
 extern "C" size_t ffk_grad_norm_workspace_bytes(int num_tensors) {
-  // a launch's table ends early where its pieces would pass 2^28, at 2^41 bytes or more: one tensor then fills it
+  // every launch of the norm has a whole table but the last (its pieces are taken in turn, whatever their number)
+  static_assert(kNormTensors * kClipPieces * kClipLoads / kNormLoads < INT32_MAX, "pieces of a table");
   int64_t const n = num_tensors > 0 ? num_tensors : 1;
-  int64_t const launches = ceil_div(n, kNormTensors) + 1;
-  return (size_t)launches * kNormWorkgroups * sizeof(double);
+  return (size_t)ceil_div(n, kNormTensors) * kNormWorkgroups * sizeof(double);
 }
 
 extern "C" int ffk_global_grad_norm(ffk_stream_t stream, int const *dtypes, void const *const *grads, int64_t const *elems, int num_tensors,
@@ -324,7 +326,7 @@ extern "C" int ffk_clip_grad_norm(ffk_stream_t stream, int const *dtypes, void c
   }
   NormTable a;
   for (int first = 0; first < num_tensors;) {
-    first = fill_table(a, dtypes, grads, clipped, elems, num_tensors, first, kClipLoads);
+    first = fill_table(a, dtypes, grads, clipped, elems, num_tensors, first, kClipLoads, kClipPieces);
     int const pieces = a.first_piece[a.tensors];
     if (pieces == 0) continue;
     clip_kernel<<<dim3((unsigned)pieces), kNormThreads, 0, st>>>(a, partial, count, max_norm, norm);

@@ -923,8 +923,8 @@ int ffk_adam_update(ffk_stream_t stream, int grad_dtype, float alpha_t,
  *     outputs that overlap each other or another tensor's input are
  *     FFK_ERR_INVALID.
  * dtypes (FFK_FLOAT / FFK_BF16), grads, clipped, elems: host arrays of
- * num_tensors entries; tensors of any size, 0 among them, aligned to their
- * elements.  Squares are summed in 64 bits in a fixed order.  A norm that is
+ * num_tensors entries; tensors of any size below 256 GB, 0 among them, aligned to
+ * their elements.  Squares are summed in 64 bits in a fixed order.  A norm that is
  * infinite or NaN scales as the formula says (factor 0 or NaN).
  * workspace: ffk_grad_norm_workspace_bytes(num_tensors) bytes, 8-byte aligned
  * (FFK_ERR_WORKSPACE); scratch, calls that overlap need one each.             */

@@ -1,0 +1,35 @@
+"""Sizes past what one launch takes (2^32 threads) are refused by masked attention, rotary positions and the gradient norm before
+any launch, and the largest that fit are not (no device is touched: the addresses are made up)."""
+import ctypes
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up")
+AT = [ctypes.c_void_p((i + 1) << 24) for i in range(16)]
+
+
+def lists(dtypes, elems):
+    n = len(dtypes)
+    return (ctypes.c_int * n)(*dtypes), (ctypes.c_void_p * n)(*[(i + 1) << 44 for i in range(n)]), (ctypes.c_int64 * n)(*elems), n
+
+
+def test_gradients(ffk):
+    """A workgroup of 256 threads scales 16 KB: tensors below 2^24 of those, 256 GB."""
+    lib = ffk.lib()
+    for dtype, size in ((ffk.BF16, 2), (ffk.FLOAT, 4)):
+        most = ((1 << 38) - (1 << 14)) // size
+        for elems, rc in ((most, ffk.ERR_WORKSPACE), (most + 1, ffk.ERR_INVALID), (1 << 37, ffk.ERR_INVALID), (1 << 39, ffk.ERR_INVALID)):
+            d, g, e, n = lists([dtype, dtype], [5, elems])
+            # (what is not refused for its size stops at the scratch that is missing)
+            assert lib.ffk_global_grad_norm(None, d, g, e, n, AT[0], None, 0) == rc, elems
+            assert lib.ffk_clip_grad_norm(None, d, g, g, e, n, 1.0, AT[0], None, 0) == rc, elems
+
+
+def test_scratch_of_the_norm_holds_every_launch(ffk):
+    """1024 sums of 64 bits for each table of 96 tensors; a table is never cut short by the tensors' sizes: 96 of the largest
+    are below 2^31 pieces of 32 KB."""
+    size = ffk.lib().ffk_grad_norm_workspace_bytes
+    for n in (1, 96, 97, 500, 9600, 9601):
+        assert size(n) >= -(-n // 96) * 1024 * 8
+    assert 96 * ((1 << 38) >> 15) < 1 << 31
