@@ -156,7 +156,16 @@ static size_t split_bytes(ffk_masked_attention_desc_t const *d, int splits) {
   return splits <= 1 ? 0 : (size_t)splits * d->batch * d->kv_heads * rows_of(d) * (dv + 2) * sizeof(float);
 }
 
-static int check(char const *who, int dtype, ffk_masked_attention_desc_t const *d) {
+static int key_groups(ffk_masked_attention_desc_t const *d, int dtype);
+// Whether every launch has fewer than the 2^32 threads that the runtime takes.  (Parts of the keys multiply few workgroups only.)
+static bool launches_fit(ffk_masked_attention_desc_t const *d, int dtype, bool backward) {
+  int64_t const places = d->kv_heads * d->batch, lim = (int64_t)1 << 32;
+  int const groups = row_groups(d, dtype), threads = !backward && groups == 1 && heads_kernels(d, dtype) ? 64 : 256;
+  auto const fits = [&](int64_t tiles, int threads) { return tiles * places < lim / threads; };  // (below 2^25 and 2^30)
+  return fits(ceil_div(rows_of(d), 32 * groups), threads) && (!backward || fits(ceil_div(d->seq_kv, 32 * key_groups(d, dtype)), 256));
+}
+
+static int check(char const *who, int dtype, ffk_masked_attention_desc_t const *d, bool backward) {
   FFK_REQUIRE(d != nullptr, "%s: NULL descriptor", who);
   FFK_REQUIRE(dtype == FFK_BF16 || dtype == FFK_FLOAT, "%s: dtype %d not supported (the entry point takes FLOAT or BF16)", who, dtype);
   FFK_REQUIRE(d->batch > 0 && d->heads > 0 && d->kv_heads > 0 && d->seq_q > 0 && d->seq_kv > 0, "%s: bad shape", who);
@@ -169,8 +178,6 @@ static int check(char const *who, int dtype, ffk_masked_attention_desc_t const *
               "%s: sizes must be below 2^30", who);
   FFK_REQUIRE(rows_of(d) < lim, "%s: seq_q * heads / kv_heads must be below 2^30", who);
   FFK_REQUIRE(d->batch * d->heads < lim, "%s: batch * heads must be below 2^30", who);
-  FFK_REQUIRE((double)(rows_of(d) + d->seq_kv) / 32 * (double)d->kv_heads * (double)d->batch + (double)d->kv_heads * (double)d->batch < 1073741824.0,
-              "%s: too many workgroups", who);
   FFK_REQUIRE(d->q_seq_stride % unit == 0 && d->k_seq_stride % unit == 0 && d->v_seq_stride % unit == 0 && d->o_seq_stride % unit == 0 &&
                   d->q_batch_stride % unit == 0 && d->k_batch_stride % unit == 0 && d->v_batch_stride % unit == 0 && d->o_batch_stride % unit == 0,
               "%s: strides must be multiples of %d elements", who, (int)unit);
@@ -182,6 +189,7 @@ static int check(char const *who, int dtype, ffk_masked_attention_desc_t const *
   FFK_REQUIRE(d->scale > 0.0f && isfinite(d->scale), "%s: scale must be positive and finite", who);
   FFK_REQUIRE(d->score_cap >= 0.0f && isfinite(d->score_cap) && (d->score_cap == 0.0f || (isfinite(d->scale / d->score_cap * 4.0f) && isfinite(d->score_cap * 4.0f))),
               "%s: score_cap must be 0 (none) or positive, finite and not vanishing beside scale", who);
+  FFK_REQUIRE(launches_fit(d, dtype, backward), "%s: too many workgroups", who);
   return FFK_OK;
 }
 
@@ -279,14 +287,14 @@ extern "C" int ffk_attention_key_ranges(ffk_stream_t stream, int64_t batch, int6
 }
 
 extern "C" size_t ffk_masked_attention_forward_workspace_bytes(ffk_masked_attention_desc_t const *d, int dtype) {
-  if (check("masked_attention_forward", dtype, d) != FFK_OK) return 0;
+  if (check("masked_attention_forward", dtype, d, false) != FFK_OK) return 0;
   return split_bytes(d, key_splits(d, dtype));
 }
 
 extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_masked_attention_desc_t const *d, void const *q,
                                             void const *k, void const *v, int32_t const *key_ranges, float const *distance_slopes,
                                             void *o, float *lse, void *workspace, size_t workspace_bytes) {
-  int const rc = check("masked_attention_forward", dtype, d);
+  int const rc = check("masked_attention_forward", dtype, d, false);
   if (rc != FFK_OK) return rc;
   FFK_REQUIRE(q && k && v && o, "masked_attention_forward: NULL tensor");
   FFK_REQUIRE(o != q && o != k && o != v, "masked_attention_forward: the output is an input");
@@ -317,7 +325,7 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
 }
 
 extern "C" size_t ffk_masked_attention_backward_workspace_bytes(ffk_masked_attention_desc_t const *d, int dtype) {
-  if (check("masked_attention_backward", dtype, d) != FFK_OK) return 0;
+  if (check("masked_attention_backward", dtype, d, true) != FFK_OK) return 0;
   return backward_bytes(d);
 }
 
@@ -325,7 +333,7 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
                                              void const *k, void const *v, int32_t const *key_ranges, float const *distance_slopes,
                                              void const *o, void const *d_o, float const *lse, void *dq, void *dk, void *dv,
                                              void *workspace, size_t workspace_bytes) {
-  int const rc = check("masked_attention_backward", dtype, d);
+  int const rc = check("masked_attention_backward", dtype, d, true);
   if (rc != FFK_OK) return rc;
   FFK_REQUIRE(q && k && v && o && d_o && lse && dq && dk && dv, "masked_attention_backward: NULL tensor");
   // (the dK/dV kernel reads all inputs behind the dQ kernel)

@@ -33,3 +33,34 @@ def test_scratch_of_the_norm_holds_every_launch(ffk):
     for n in (1, 96, 97, 500, 9600, 9601):
         assert size(n) >= -(-n // 96) * 1024 * 8
     assert 96 * ((1 << 38) >> 15) < 1 << 31
+
+
+def desc(ffk, B, H, KH, Sq, Skv, D, **more):
+    d = ffk.MaskedAttentionDesc(B, H, KH, Sq, Skv, D, 0, Sq * H * D, H * D, Skv * KH * D, KH * D, Skv * KH * D, KH * D, Sq * H * D, H * D, 0, 0.125, 0.0, 0)
+    for name, value in more.items():
+        setattr(d, name, value)
+    return d
+
+
+ATTENTION = [  # dtype, (B, H, KH, Sq, Skv, D), whether forward and backward fit
+    # 64 threads for 32 rows of one sequence and key head in the forward, 256 in the backward
+    ("BF16", ((1 << 21) - 1, 8, 8, 1, 1, 64), True, True), ("BF16", (1 << 21, 8, 8, 1, 1, 64), True, False),
+    ("BF16", ((1 << 23) - 1, 8, 8, 1, 1, 64), True, False), ("BF16", (1 << 23, 8, 8, 1, 1, 64), False, False),
+    # 256 for them in the kernels of any head size
+    ("BF16", ((1 << 21) - 1, 8, 8, 1, 1, 256), True, True), ("BF16", (1 << 21, 8, 8, 1, 1, 256), False, False),
+    ("FLOAT", (1 << 21, 8, 8, 1, 1, 64), False, False),
+    # 256 for 128 rows, and for 128 keys
+    ("BF16", ((1 << 14) - 1, 8, 8, 16384, 64, 8), True, True), ("BF16", (1 << 14, 8, 8, 16384, 64, 8), False, False),
+    ("BF16", ((1 << 14) - 1, 8, 8, 64, 16384, 8), True, True), ("BF16", (1 << 14, 8, 8, 64, 16384, 8), True, False),
+]
+
+
+@pytest.mark.parametrize("dtype,shape,forward,backward", ATTENTION)
+def test_attention(ffk, dtype, shape, forward, backward):
+    lib, d, dtype = ffk.lib(), desc(ffk, *shape), getattr(ffk, dtype)
+    # (what is not refused for its size stops at a tensor that is missing)
+    rc = lib.ffk_masked_attention_forward(None, dtype, ctypes.byref(d), None, AT[1], AT[2], None, None, AT[3], AT[4], None, 0)
+    assert rc == ffk.ERR_INVALID and (b"NULL tensor" if forward else b"too many workgroups") in lib.ffk_last_error()
+    rc = lib.ffk_masked_attention_backward(None, dtype, ctypes.byref(d), None, *AT[1:3], None, None, *AT[3:9], AT[9], 1 << 62)
+    assert rc == ffk.ERR_INVALID and (b"NULL tensor" if backward else b"too many workgroups") in lib.ffk_last_error()
+    assert (lib.ffk_masked_attention_backward_workspace_bytes(ctypes.byref(d), dtype) > 0) == backward
