@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryParams p) 
 }
 
 template <typename T, int N>
-static hipError_t rotary_launch(hipStream_t st, RotaryParams &p, bool interleaved, bool copy_rest) {
+static int rotary_launch(char const *who, hipStream_t st, RotaryParams &p, bool interleaved, bool copy_rest) {
   p.turning = interleaved && N > 1 ? 2 * p.half / N : p.half / N;
   p.units = p.turning + (copy_rest ? (p.head_dim - 2 * p.half) / N : 0);
   p.units_div = make_fast_div((uint32_t)p.units);
@@ -165,10 +165,14 @@ static hipError_t rotary_launch(hipStream_t st, RotaryParams &p, bool interleave
   if (want > room) want = room;
   if (want < 1) want = 1;
   p.tokens_per_wg = (int)want;
+  // (2^32 threads are more than a launch takes)
+  FFK_REQUIRE(ceil_div(p.tokens, want) < ((int64_t)1 << 32) / kRotaryThreads, "%s: too many workgroups (%lld tokens, %lld to each)", who,
+              (long long)p.tokens, (long long)want);
   dim3 const grid((unsigned)ceil_div(p.tokens, want));
   if (interleaved) rotary_kernel<T, N, true><<<grid, kRotaryThreads, 0, st>>>(p);
   else rotary_kernel<T, N, false><<<grid, kRotaryThreads, 0, st>>>(p);
-  return hipGetLastError();
+  FFK_CHECK_LAUNCH();
+  return FFK_OK;
 }
 
 static int rotary_any(char const *who, ffk_stream_t stream, int dtype, ffk_rotary_desc_t const *d, void const *q, void const *k,
@@ -236,20 +240,16 @@ static int rotary_any(char const *who, ffk_stream_t stream, int dtype, ffk_rotar
   while (n > 1 && (bits % n != 0 || at % (uint64_t)(n * size) != 0)) n /= 2;
   bool const copy_rest = (!q_in_place || !k_in_place) && 2 * half < d->head_dim;
   hipStream_t const st = as_stream(stream);
-  hipError_t e;
   bool const inter = d->interleaved != 0;
   if (dtype == FFK_BF16) {
-    e = n == 8   ? rotary_launch<bf16, 8>(st, p, inter, copy_rest)
-        : n == 4 ? rotary_launch<bf16, 4>(st, p, inter, copy_rest)
-        : n == 2 ? rotary_launch<bf16, 2>(st, p, inter, copy_rest)
-                 : rotary_launch<bf16, 1>(st, p, inter, copy_rest);
-  } else {
-    e = n == 4   ? rotary_launch<float, 4>(st, p, inter, copy_rest)
-        : n == 2 ? rotary_launch<float, 2>(st, p, inter, copy_rest)
-                 : rotary_launch<float, 1>(st, p, inter, copy_rest);
+    return n == 8   ? rotary_launch<bf16, 8>(who, st, p, inter, copy_rest)
+           : n == 4 ? rotary_launch<bf16, 4>(who, st, p, inter, copy_rest)
+           : n == 2 ? rotary_launch<bf16, 2>(who, st, p, inter, copy_rest)
+                    : rotary_launch<bf16, 1>(who, st, p, inter, copy_rest);
   }
-  FFK_HIP(e);
-  return FFK_OK;
+  return n == 4   ? rotary_launch<float, 4>(who, st, p, inter, copy_rest)
+         : n == 2 ? rotary_launch<float, 2>(who, st, p, inter, copy_rest)
+                  : rotary_launch<float, 1>(who, st, p, inter, copy_rest);
 }
 
 }  // namespace ffk

@@ -64,3 +64,13 @@ def test_attention(ffk, dtype, shape, forward, backward):
     rc = lib.ffk_masked_attention_backward(None, dtype, ctypes.byref(d), None, *AT[1:3], None, None, *AT[3:9], AT[9], 1 << 62)
     assert rc == ffk.ERR_INVALID and (b"NULL tensor" if backward else b"too many workgroups") in lib.ffk_last_error()
     assert (lib.ffk_masked_attention_backward_workspace_bytes(ctypes.byref(d), dtype) > 0) == backward
+
+
+@pytest.mark.parametrize("batch,seq,heads,dim", [(1 << 14, 1 << 10, 16, 1024), (1 << 12, 1 << 15, 1, 4096), (1 << 25, 8, 40, 128)])
+def test_rotary(ffk, batch, seq, heads, dim):
+    """A workgroup of 256 threads takes one token of many heads, or of many pairs, or a few of others."""
+    n = heads * dim
+    d = ffk.RotaryDesc(batch, seq, heads, 0, dim, seq * n, n, 0, 0, seq * n, n, 0, 0, 1, (ffk.c_i64 * 4)(dim // 2), 0)
+    for entry in (ffk.lib().ffk_rotary_forward, ffk.lib().ffk_rotary_backward):
+        rc = entry(None, ffk.BF16, ctypes.byref(d), AT[0], None, AT[4], AT[5], AT[2], None)
+        assert rc == ffk.ERR_INVALID and b"too many workgroups" in ffk.lib().ffk_last_error()
