@@ -193,6 +193,12 @@ static int check(char const *who, int dtype, ffk_masked_attention_desc_t const *
   return FFK_OK;
 }
 
+// Biases are added in units of the raw product, or of the cap's tanh (slope_unit): one of up to 2^27 has to be a number there.
+static int check_slopes(char const *who, MaskedAttnParams const &p) {
+  FFK_REQUIRE(p.slopes == nullptr || p.slope_unit < 0x1p100f, "%s: scale, or score_cap, vanishes beside distance slopes", who);
+  return FFK_OK;
+}
+
 static MaskedAttnParams params_of(ffk_masked_attention_desc_t const *d, int dtype, void const *q, void const *k, void const *v, int32_t const *ranges,
                                   float const *slopes) {
   MaskedAttnParams p = {};
@@ -301,6 +307,7 @@ extern "C" int ffk_masked_attention_forward(ffk_stream_t stream, int dtype, ffk_
   FFK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "masked_attention_forward: tensors must be 16-byte aligned");
   FFK_REQUIRE(reinterpret_cast<uintptr_t>(key_ranges) % 8 == 0, "masked_attention_forward: key_ranges must be 8-byte aligned");
   MaskedAttnParams p = params_of(d, dtype, q, k, v, key_ranges, distance_slopes);
+  if (int const bad = check_slopes("masked_attention_forward", p)) return bad;
   p.o = o;
   p.lse = lse;
   hipStream_t const st = as_stream(stream);
@@ -349,6 +356,7 @@ extern "C" int ffk_masked_attention_backward(ffk_stream_t stream, int dtype, ffk
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
   }
   MaskedAttnParams p = params_of(d, dtype, q, k, v, key_ranges, distance_slopes);
+  if (int const bad = check_slopes("masked_attention_backward", p)) return bad;
   p.o = const_cast<void *>(o);
   p.d_o = d_o;
   p.lse = const_cast<float *>(lse);

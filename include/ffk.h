@@ -649,7 +649,8 @@ int ffk_attention_backward(ffk_stream_t stream, int dtype,
  *   and behind the last one that a row of the batch entry sees (padding) may hold
  *   anything, NaN and infinities too, and get zero gradients; a key between
  *   them that a row does not see has to be finite all the same (a masked
- *   probability is 0, and 0 times infinity is none).  Slopes are finite.
+ *   probability is 0, and 0 times infinity is none).  Slopes are finite; beside
+ *   them scale, or score_cap where there is one, is above 2^-100.
  *   Ranges are cut to [0, seq_kv].  distance_slopes and key_ranges have no gradient.
  *   score_cap is any that is finite and does not vanish beside scale.  FFK_BF16: up
  *   to 128 a capped score is within 2^-22 score_cap of its value; past that within

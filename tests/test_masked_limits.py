@@ -74,3 +74,15 @@ def test_rotary(ffk, batch, seq, heads, dim):
     for entry in (ffk.lib().ffk_rotary_forward, ffk.lib().ffk_rotary_backward):
         rc = entry(None, ffk.BF16, ctypes.byref(d), AT[0], None, AT[4], AT[5], AT[2], None)
         assert rc == ffk.ERR_INVALID and b"too many workgroups" in ffk.lib().ffk_last_error()
+
+
+@pytest.mark.parametrize("scale,cap", [(1e-39, 0.0), (1e-38, 0.0), (1e-36, 0.0), (1e-38, 1e-36)])
+def test_scales_that_leave_no_room_for_slopes(ffk, scale, cap):
+    """Biases are added in units of the raw product (or of the cap's tanh): 0.5 * 7 over a scale of 1e-38 is no number there."""
+    lib, d = ffk.lib(), desc(ffk, 2, 4, 2, 16, 16, 64, scale=scale, score_cap=cap)
+    for dtype in (ffk.BF16, ffk.FLOAT):
+        rc = lib.ffk_masked_attention_forward(None, dtype, ctypes.byref(d), *AT[:3], None, AT[10], AT[3], AT[4], None, 0)
+        assert rc == ffk.ERR_INVALID and b"slopes" in lib.ffk_last_error()
+        need = lib.ffk_masked_attention_backward_workspace_bytes(ctypes.byref(d), dtype)
+        rc = lib.ffk_masked_attention_backward(None, dtype, ctypes.byref(d), *AT[:3], None, AT[10], *AT[3:9], AT[9], need)
+        assert rc == ffk.ERR_INVALID and b"slopes" in lib.ffk_last_error()
