@@ -12,6 +12,8 @@
 // better: 50 MB of fp32, norm and clipping 28 us and 30).  For the clipping every piece of 16 KB is a workgroup of its own, which asks
 // for its piece first and adds up the norm while that is on its way (2.4 GB: 830 us, 5.8 TB/s; 2048 workgroups that take
 // pieces in turn 946 us).
+//   Past a table of 96 tensors every workgroup of the clipping reads another 8 KB of sums for each 96: 2.4 GB of bf16 in 54, 300
+// and 1200 tensors take 840, 1065 and 1823 us, the norm's launches 351, 368 and 408.
 #include "ffk_common.h"
 #include <math.h>
 #include <algorithm>
@@ -155,8 +157,8 @@ __device__ __forceinline__ void piece_scaled(T const *p, T *q, int n, float fact
   }
 }
 
-// Every workgroup adds up the norm for itself from the thousand partial sums, which the caches hold: no third launch
-// between the norm and the scaling.  A tensor that stays as it is, in place, is not touched; its pieces are not asked for
+// Every workgroup adds up the norm for itself from the partial sums, a thousand for each table, which the caches hold:
+// no third launch between the norm and the scaling.  A tensor that stays as it is, in place, is not touched; its pieces are not asked for
 // before that is known.
 __global__ __launch_bounds__(kNormThreads) void clip_kernel(NormTable a, double const *partial, int count, float max_norm, float *norm) {
   __shared__ double lds[4];

@@ -11,7 +11,7 @@
 // orders, would leave some 2^-23 of |dO| |v| in its place, and all of dQ and dK of sequences of one position is nothing else.
 // So the dQ kernels let such a row see nothing where dS is masked (score_range), and the dK/dV kernels correct P and dS of
 // the tiles that have one, or, for heads, clear its Q in LDS, which with what write_row leaves of it gives P = 1.  No
-// instruction for it in a loop (a comparison a score took 3% of a capped pass over 4 x 4096 tokens).
+// instruction for it in a loop (a comparison a score took 2 to 4 % of a capped pass over 4 x 4096 tokens).
 //
 // The G query heads of a key head are one longer axis of rows, r = i G + g: they share the tiles of K and V that a
 // workgroup brings into LDS, the keys' gradients are sums over that one axis (no atomics), and a few query rows still
@@ -246,8 +246,8 @@ struct TileRegs {
 //   kCapLogistic: y = 1 / (1 + 2^(cap_in raw)), cap_in = -2 log2(e) scale / cap, on the hardware's exponential and reciprocal:
 //   tanh is 2 y - 1, so score_scale = 2 cap log2(e), shift = -cap log2(e), and 1 - tanh^2 = 4 (y - y^2), of which grad_scale has
 //   the 4.  Four vector instructions a score and two for the derivative.  Scores next to nothing are next to y = 1/2, where a
-//   step of y is 2^-24, so this one is off by up to about 2^-22 cap whatever the score.
-// bf16 takes the second up to a cap of kLogisticCap, 3e-5 of a score there and 1e-5 at 50, far below what bf16 scores carry;
+//   step of y is 2^-24, so this one is off by up to 2^-21 cap whatever the score.
+// bf16 takes the second up to a cap of kLogisticCap, 6e-5 there and 2e-5 at 50, far below what bf16 scores carry;
 // past it (at 10^5 scores would be 0.01 off, at 10^8 all the same) the first one, in the general kernels: 4 x 2048 tokens,
 // 16 heads of 128 on 4, causal, 1003 us with gradients, and 506 at a cap of 100.  fp32 takes the first: its products take
 // sixteen times as long.

@@ -12,7 +12,7 @@ hipError_t masked_attention_dq_bf16(hipStream_t st, MaskedAttnParams const &p, i
 hipError_t masked_attention_dq_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
 hipError_t masked_attention_dkdv_bf16(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
 hipError_t masked_attention_dkdv_f32(hipStream_t st, MaskedAttnParams const &p, int padded, int groups);
-// bf16, head sizes 64 and 128: masked_attention_heads_{fwd,dq,dkdv}.hip
+// bf16 heads up to 128 (heads_kernels below): masked_attention_heads_{fwd,rows,dq,dkdv}.hip
 hipError_t masked_attention_fwd_heads(hipStream_t st, MaskedAttnParams const &p);
 hipError_t masked_attention_fwd_rows(hipStream_t st, MaskedAttnParams const &p);  // few rows
 hipError_t masked_attention_dq_heads(hipStream_t st, MaskedAttnParams const &p);
@@ -127,6 +127,9 @@ static bool logistic_cap(ffk_masked_attention_desc_t const *d, int dtype) { retu
 // 38 with 32 rows, backward 219 and 153; four sequences, 256 workgroups, not causal, 86 and 116, 285 and 367).  bf16: half as
 // many (two sequences, 8 heads of 128, 128 workgroups, forward 26 us and 37, backward 75 and 80; 8 heads of 256 on 4, 160
 // workgroups, forward 54 and 73; one sequence, 4 heads of 128 on 2, 32 workgroups, forward 25 and 21, backward 99 and 86).
+//   Rows over a longer cache are where this is wrong in fp32, whose keys come in parts for either: 16, 32, 64, 128 and 256 rows of
+// 32 heads of 128 on 8 over 8192 keys, forward, 42, 76, 125, 230 and 449 us, and 86, 89, 92, 155 and 289 with 128 rows to a
+// workgroup.  In bf16 (32 rows in one wave, in parts, or 128 and whole keys) 20, 29, 54, 84 and 122 us, and 158 to 161.
 static int few_workgroups(int dtype) { return dtype == FFK_FLOAT ? kNumCU : kNumCU / 2; }
 // (FFK_OPTION_ATTENTION_VARIANT other than 0 keeps the kernels for many rows and keys at every size.)
 // 32-row groups of a workgroup: 4, or 1 whose four waves share out the keys, where there are no more rows or few

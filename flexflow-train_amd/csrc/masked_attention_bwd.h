@@ -1,13 +1,15 @@
 // Masked attention, backward: any head size, either type (see masked_attention.h for the mathematics and layouts).
-// Templates that masked_attention_bwd_*.hip instantiate, so that they compile side by side.
+// Templates that masked_attention_{dq,dkdv}_*.hip instantiate, so that they compile side by side.
 //
 // Two kernels without atomics, both of which compute P again from the saved log-sum-exp.  The dQ kernel owns 32 RG rows
 // and runs over the keys in their ranges; it also leaves delta = rowsum(O dO) = rowsum(P dP) and, for every 32 rows, a summary of their
 // ranges in memory for the dK/dV kernel, which runs behind it.  That one owns 128 keys of one key head, 32 to a wave, and
 // runs over the rows of all query heads that read it, without the tiles of rows that see none of its keys.
-//   Both kernels together: bf16 heads of 256, 4 x 2000 tokens, 8 heads on 4, causal 742 us (0.22 PFLOP/s of the gradient's
-// products; dV and dK are launches of their own there, which leaves one of them its accumulators in registers); fp32,
-// 4 x 2000 tokens, 8 heads of 64, causal 713 us (57 TFLOP/s).
+//   Both kernels together: bf16 heads of 256, 4 x 2000 tokens, 8 heads on 4, causal 740 us (0.22 PFLOP/s of the gradient's
+// five products; dV and dK are launches of their own there, which leaves one of them its accumulators in registers, and S is
+// computed three times and dP twice: eight products); fp32, 4 x 2000 tokens, 8 heads of 64, causal 713 us (57 TFLOP/s of five,
+// 80 of the seven that are computed).  What else keeps them from the large products' rates has not been measured: tiles pass
+// through registers, and fp32 reads turned fragments an element at a time.
 #pragma once
 #include "masked_attention.h"
 
@@ -232,8 +234,6 @@ __global__ __launch_bounds__(256) void masked_dq_kernel(MaskedAttnParams p) {
         store4(dqp + d, dq[i][4 * g] * p.grad_scale, dq[i][4 * g + 1] * p.grad_scale, dq[i][4 * g + 2] * p.grad_scale, dq[i][4 * g + 3] * p.grad_scale);
     }
 }
-
-// What a row brings along into LDS: its range, statistics, slope and position.
 
 template <typename T, int DP, int KG>
 struct MaskedDkdv {

@@ -5,8 +5,9 @@
 // turn (their sums meet in LDS at the end).  Keys and values pass through LDS in tiles of 32 J KW rows, the next tile
 // on its way in registers meanwhile.  The loop runs over the union of the rows' ranges only; a wave skips a tile that none
 // of its rows sees, and compares ranges element by element only where a tile is not seen whole by all of them.
-//   bf16 heads of 256, 4 x 2000 tokens, 8 heads on 4, causal: 164 us (0.40 PFLOP/s), bound by LDS reads and one wave to a SIMD;
-// fp32, 4 x 2000 tokens, 8 heads of 64, causal: 214 us (77 TFLOP/s), by the fp32 matrix instructions.
+//   bf16 heads of 256, 4 x 2000 tokens, 8 heads on 4, causal: 158 us (0.41 PFLOP/s), bound by LDS reads and one wave to a SIMD;
+// fp32, 4 x 2000 tokens, 8 heads of 64, causal: 214 us (77 TFLOP/s), half the rate of the fp32 matrix instructions, of which
+// masked tiles at the diagonal take some, and single-element reads of V's turned fragments the rest or not: not measured.
 #pragma once
 #include "masked_attention.h"
 

@@ -645,15 +645,16 @@ int ffk_attention_backward(ffk_stream_t stream, int dtype,
  *     s -= distance_slopes[h] * |p_i - j|        (distance_slopes [heads] fp32 or NULL)
  *   over the keys of its range (key_ranges NULL: all keys), of which causal != 0
  *   leaves those with j <= p_i.  A row that sees no key has o = 0, lse = -inf and
- *   gives and takes no gradient, whatever lies in it.  Keys in front of the first
- *   and behind the last one that a row of the batch entry sees (padding) may hold
- *   anything, NaN and infinities too, and get zero gradients; a key between
- *   them that a row does not see has to be finite all the same (a masked
+ *   gives and takes no gradient, whatever lies in it; the score of one that sees a
+ *   single key has none: its dq is 0, and nothing is added to dk.  Keys in front of
+ *   the first and behind the last one that a row of the batch entry sees (padding)
+ *   may hold anything, NaN and infinities too, and get zero gradients; a key
+ *   between them that a row does not see has to be finite all the same (a masked
  *   probability is 0, and 0 times infinity is none).  Slopes are finite; beside
  *   them scale, or score_cap where there is one, is above 2^-100.
  *   Ranges are cut to [0, seq_kv].  distance_slopes and key_ranges have no gradient.
  *   score_cap is any that is finite and does not vanish beside scale.  FFK_BF16: up
- *   to 128 a capped score is within 2^-22 score_cap of its value; past that within
+ *   to 128 a capped score is within 2^-21 score_cap of its value; past that within
  *   some 2^-22 of itself, as FFK_FLOAT's are, by kernels that take about twice as long.
  *   dtype FFK_BF16 (head sizes multiples of 8 up to 256, strides multiples of 8
  *   elements) or FFK_FLOAT (multiples of 4); 16-byte aligned tensors, key_ranges
